@@ -153,6 +153,13 @@ SIGNATURES = {
     "flame_pinned_pool_stats": (None, [_vp, C.POINTER(_sz), C.POINTER(_sz)]),
     "flame_offload_probe": (_i, [_sz, _i, C.POINTER(LinkProbe)]),
     "flame_offload_policy_plan_blocks": (_i, [C.POINTER(PolicyInput), C.POINTER(PolicyBlock), _sz, _i, C.POINTER(C.c_int32), C.POINTER(PolicyBlockPlan)]),
+    "flame_fp8_quant_2d": (_i, [_vp, _sz, _sz, _sz, _vp, _vp, _i, _vp, _vp, _sz, _vp]),
+    "flame_fp8_dequant_2d": (_i, [_vp, _sz, _vp, _i, _vp, _i, _sz, _sz, _vp]),
+    "flame_fp8_product": (_i, [_vp, _sz, _vp, _i, _vp, _sz, _vp, _i, _i, _vp, _sz, _i, _sz, _sz, _sz, _vp]),
+    "flame_group_norm_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _i]),
+    "flame_group_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _f, _i, _i, _vp, _sz, _vp]),
+    "flame_group_norm_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _i, _i, _vp, _sz, _vp]),
+    "flame_dropout": (_i, [_vp, _vp, _vp, _sz, _i, _d, C.c_uint64, _vp, C.c_uint64, _vp]),
     "flame_offload_policy_plan": (_i, [C.POINTER(PolicyInput), C.POINTER(PolicyTensor), _sz, C.POINTER(C.c_int32), C.POINTER(_d)]),
 }
 

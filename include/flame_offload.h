@@ -533,6 +533,68 @@ FlameOffloadStatus flame_restore_arena_release(FlameRestoreArena* arena, uint64_
 FlameOffloadStatus flame_restore_arena_reset(FlameRestoreArena* arena);
 FlameOffloadStatus flame_restore_arena_stats(const FlameRestoreArena* arena, FlameRestoreArenaStats* out);
 
+/* ------------------------------------------------------------------------
+ * 8. Operators next to the path (new).  All of them: 0 or a cudaError_t value, with a text in flame_offload_last_error()
+ *    where an argument is refused; a few launches on `stream` and nothing else (no allocation, no synchronisation, no
+ *    atomics: the same inputs give the same bits), so that they can be recorded in a CUDA graph once each has been called
+ *    on the device; outputs must not overlap inputs.
+ *
+ * 8a. Matrix product of FP8 E4M3 operands (OCP codes) with one fp32 scale for each block of 128.
+ *     rows:    a scale for 1 x 128 elements of a row,    scales [rows, ceil(cols/128)]
+ *     columns: a scale for 128 x 1 elements of a column, scales [ceil(rows/128), cols]
+ *     tiles:   a scale for 128 x 128 elements,           scales [ceil(rows/128), ceil(cols/128)]
+ *     (a block at an edge uses its real elements.)  Codes are row-major, 16-byte aligned, with a row stride that is a
+ *     multiple of 16 bytes; what lies between a row's end and the next row does not matter.
+ *     scale = absmax/448 (NaN ignored); code = e4m3_rne_sat(x * (1/scale)), each step rounded to fp32: for rows of a
+ *     contiguous matrix with cols % 128 == 0 the codes' values are those of flame_act_quant_fp8_b128 with
+ *     FLAME_ACT_FP8_OCP.  A NaN element has a NaN code, a block with an infinity gives NaN in the products it enters.
+ *     Codes of the reference's encoder (flame_act_quant_fp8_b128 without that flag) are no operands: there 0x7F is 480.
+ * ---------------------------------------------------------------------- */
+enum { FLAME_FP8_BLOCKS_ROWS = 1, FLAME_FP8_BLOCKS_COLUMNS = 2, FLAME_FP8_BLOCKS_TILES = 3 };
+
+/* BF16 [rows, cols] with x_stride elements from row to row -> codes.  `blocks`: what goes to codes / scales, ROWS or TILES,
+ * or 0 for nothing; column_codes / column_scales (both or neither NULL): the same matrix with COLUMNS blocks, from the same
+ * read (not beside TILES).  code_stride: bytes from row to row of both, all of them writable: a row's padding up to a multiple
+ * of 8 bytes gets zeros. */
+int flame_fp8_quant_2d(const void* x_bf16, size_t rows, size_t cols, size_t x_stride, void* codes, void* scales, int blocks,
+                       void* column_codes, void* column_scales, size_t code_stride, void* stream);
+/* codes -> BF16 or F32 (out_dtype: FLAME_OFFLOAD_DTYPE_*), out [rows, cols] contiguous: code * scale, rounded once */
+int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scales, int blocks, void* out, int out_dtype,
+                         size_t rows, size_t cols, void* stream);
+/* C [M, N] = sum over blocks of the contraction of scale_a * scale_b * (product of the codes), fp32 sums, rounded once to
+ * c_dtype (BF16 or F32); c_stride elements from row to row of C.  The operands:
+ *     a ROWS [M, K],    b ROWS or TILES [N, K], b_transposed 1:  C = A B^T   (a linear layer)
+ *     a ROWS [M, K],    b TILES [K, N],         b_transposed 0:  C = A B     (its input gradient)
+ *     a COLUMNS [K, M], b COLUMNS [K, N],       b_transposed 0:  C = A^T B   (its weight gradient)
+ * K == 0 gives zeros. */
+int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales, int a_blocks, const void* b_codes, size_t b_stride,
+                      const void* b_scales, int b_blocks, int b_transposed, void* c, size_t c_stride, int c_dtype, size_t M,
+                      size_t N, size_t K, void* stream);
+
+/* 8b. Group norm with an activation on a channels-last BF16 tensor x [B, L, C] (contiguous): C / G neighbouring channels a
+ *     group, mean and variance over L x C/G elements, h = (x - mean) * rstd * weight + bias, y = h or silu(h), fp32 inside.
+ *     weight, bias [C]: param_dtype (FLAME_OFFLOAD_DTYPE_*), NULL = 1 and 0.  stats [B, G, 2] fp32 receives mean and
+ *     rstd = 1/sqrt(variance + eps), which the backward pass reads.  codes / code_scales (may be NULL; C % 128 == 0): FP8
+ *     codes of y with ROWS blocks ([B*L, C], stride C).  workspace: flame_group_norm_workspace_bytes, 16-byte aligned,
+ *     free again when the call's work is done.
+ *     backward: dx [B, L, C] BF16; dweight, dbias [C] param_dtype, NULL = not wanted. */
+enum { FLAME_ACTIVATION_NONE = 0, FLAME_ACTIVATION_SILU = 1 };
+size_t flame_group_norm_workspace_bytes(size_t B, size_t L, size_t C, size_t G, int backward);
+int flame_group_norm(const void* x_bf16, const void* weight, const void* bias, void* y_bf16, void* codes, void* code_scales,
+                     void* stats, size_t B, size_t L, size_t C, size_t G, float eps, int activation, int param_dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int flame_group_norm_backward(const void* x_bf16, const void* dy_bf16, const void* weight, const void* bias, const void* stats,
+                              void* dx_bf16, void* dweight, void* dbias, size_t B, size_t L, size_t C, size_t G, int activation,
+                              int param_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* 8c. Dropout whose mask is a function of (seed, offset, element index) and never stored: y = kept ? x / (1 - p) : 0, plus
+ *     residual where it is not NULL; dtype BF16 or F32, fp32 inside.  An element is dropped when its 32 random bits (Philox
+ *     4x32-10; csrc/dropout.cu defines them) are under round(p * 2^32); p == 1 drops everything.  The backward pass is the same
+ *     call on the gradient without a residual.  seed_device (may be NULL): one 64-bit seed in device memory, read instead of
+ *     `seed` when the kernel runs, so that a recorded graph can be replayed with another seed. */
+int flame_dropout(const void* x, const void* residual, void* y, size_t n, int dtype, double p, uint64_t seed,
+                  const void* seed_device, uint64_t offset, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,336 @@
+"""FP8 block quantiser, product and linear layer against 64-bit arithmetic."""
+import pytest
+import torch
+
+from flame_b200 import InvalidInput, InvalidShape, Unsupported, _lib
+from flame_b200.fp8_product import Fp8Blocks, fp8_linear, fp8_matmul, quantize_fp8, quantize_fp8_both
+
+pytestmark = pytest.mark.gpu
+
+
+def up(n, unit=128):
+    return (n + unit - 1) // unit * unit
+
+
+def spread(scales, shape, blocks):
+    """fp32 scales of each element, as 64-bit numbers."""
+    r, c = shape
+    s = scales.double()
+    if blocks != "rows":
+        s = s.repeat_interleave(128, 0)[:r]
+    if blocks != "columns":
+        s = s.repeat_interleave(128, 1)[:, :c]
+    return s
+
+
+def numbers(q):
+    return q.codes.contiguous().view(torch.float8_e4m3fn).to(torch.float64) * spread(q.scales, q.shape, q.blocks)
+
+
+def reference_quantise(x, blocks):
+    """The definition, each step one binary32 operation on the CPU."""
+    r, c = x.shape
+    down, across = {"rows": (1, 128), "columns": (128, 1), "tiles": (128, 128)}[blocks]
+    v = torch.zeros(up(r, down), up(c, across))
+    v[:r, :c] = x.float().cpu()
+    t = v.view(v.shape[0] // down, down, v.shape[1] // across, across)
+    amax = torch.where(t.isnan(), torch.zeros(()), t.abs()).amax((1, 3), keepdim=True)
+    scale = amax / torch.full_like(amax, 448.0)
+    inv = torch.where(scale == 0, torch.zeros(()), 1 / scale)
+    y = torch.where(inv > 3e38, t / scale, t * inv)
+    y = torch.where(y.isnan(), y, y.clamp(-448, 448))
+    codes = y.to(torch.float8_e4m3fn).view(torch.uint8).reshape(v.shape)[:r, :c]
+    return codes, scale.reshape(t.shape[0], t.shape[2])
+
+
+def integers(shape, device, seed, blocks):
+    """Operands whose products and sums are exact in binary32: integers up to 8, scales 1/4 to 4."""
+    g = torch.Generator(device=device).manual_seed(seed)
+    v = torch.randint(-8, 9, shape, device=device, generator=g).float()
+    ld = max(16, up(shape[1], 16))
+    codes = torch.full((shape[0], ld), 0x7F, dtype=torch.uint8, device=device)     # NaN behind every row's end
+    codes[:, :shape[1]] = v.to(torch.float8_e4m3fn).view(torch.uint8)
+    ss = (shape[0] if blocks == "rows" else up(shape[0]) // 128, shape[1] if blocks == "columns" else up(shape[1]) // 128)
+    scales = torch.exp2(torch.randint(-2, 3, ss, device=device, generator=g).float())
+    return Fp8Blocks(codes[:, :shape[1]], scales, blocks)
+
+
+PRODUCTS = ["nt_tiles", "nt_rows", "nn_tiles", "tn_columns"]
+
+
+def operands(kind, m, n, k, make):
+    if kind == "nt_tiles":
+        return make((m, k), "rows"), make((n, k), "tiles"), True
+    if kind == "nt_rows":
+        return make((m, k), "rows"), make((n, k), "rows"), True
+    if kind == "nn_tiles":
+        return make((m, k), "rows"), make((k, n), "tiles"), False
+    return make((k, m), "columns"), make((k, n), "columns"), False
+
+
+def expected(a, b, transpose_b):
+    x, y = numbers(a), numbers(b)
+    return (x.T if a.blocks == "columns" else x) @ (y.T if transpose_b else y)
+
+
+SIZES = [(1, 1, 1), (1, 2048, 2048), (3, 130, 257), (17, 1000, 129), (64, 64, 64), (127, 255, 383), (128, 128, 128), (129, 256, 640),
+         (256, 512, 1024), (300, 77, 2000), (513, 384, 96), (1000, 713, 1331), (2, 5000, 300), (1024, 16, 4096)]
+
+
+@pytest.mark.parametrize("blocks", ["rows", "columns", "tiles"])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 128), (5, 7), (128, 128), (130, 300), (257, 1331), (384, 512)])
+def test_quantise_gives_the_defined_codes(cuda_device, shape, blocks):
+    g = torch.Generator(device=cuda_device).manual_seed(shape[0] * 1000 + shape[1])
+    x = (torch.randn(shape, device=cuda_device, generator=g) * torch.exp2(torch.randint(-6, 7, shape, device=cuda_device, generator=g).float())).to(torch.bfloat16)
+    x[shape[0] // 2:, :] *= 0                       # blocks of zeros among them
+    q = quantize_fp8(x, blocks)
+    codes, scales = reference_quantise(x, blocks)
+    assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), scales)
+    for dtype in (torch.float32, torch.bfloat16):
+        want = (q.codes.contiguous().view(torch.float8_e4m3fn).float() * spread(q.scales, q.shape, blocks).float()).to(dtype)
+        assert torch.equal(q.dequantize(dtype), want)
+    if blocks == "rows":
+        both = quantize_fp8_both(x)
+        assert torch.equal(both[0].codes, q.codes) and torch.equal(both[0].scales, q.scales)
+        col = quantize_fp8(x, "columns")
+        assert torch.equal(both[1].codes, col.codes) and torch.equal(both[1].scales, col.scales)
+
+
+def test_quantise_equals_the_block_codec_on_whole_rows(cuda_device):
+    """For a contiguous matrix whose rows are whole blocks the codes are those of the flat codec with the OCP encoder."""
+    x = torch.randn(37, 384, device=cuda_device).to(torch.bfloat16)
+    codes = torch.empty(x.numel(), dtype=torch.uint8, device=cuda_device)
+    scales = torch.empty(x.numel() // 128, dtype=torch.float32, device=cuda_device)
+    assert _lib.lib().flame_act_quant_fp8_b128(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel(), 1, torch.cuda.current_stream().cuda_stream) == 0
+    q = quantize_fp8(x)
+    assert torch.equal(q.codes.reshape(-1), codes) and torch.equal(q.scales.reshape(-1), scales)
+
+
+def test_quantise_extremes(cuda_device):
+    """Tiny blocks (the reciprocal of the scale overflows), infinities and NaN, each in a block of its own."""
+    x = torch.randn(6, 128, device=cuda_device)
+    x[1] *= 1e-37
+    x[2] = 0
+    x[2, 5] = float("nan")
+    x[3, 7] = float("inf")
+    x[4, 9] = float("nan")
+    x = x.to(torch.bfloat16)
+    x[5] = -0.0
+    q = quantize_fp8(x)
+    codes, scales = reference_quantise(x, "rows")
+    assert torch.equal(q.scales.cpu(), scales)
+    is_nan = (codes & 0x7F) == 0x7F
+    assert torch.equal((q.codes.cpu() & 0x7F) == 0x7F, is_nan) and torch.equal(q.codes.cpu()[~is_nan], codes[~is_nan])
+    y = fp8_matmul(q, quantize_fp8(torch.randn(64, 128, device=cuda_device).to(torch.bfloat16), "tiles"), transpose_b=True)
+    finite = torch.isfinite(y).all(dim=1).cpu().tolist()
+    assert finite == [True, True, False, False, False, True] and bool((y[5] == 0).all())
+
+
+def test_quantise_reads_strided_rows(cuda_device):
+    wide = torch.randn(70, 400, device=cuda_device).to(torch.bfloat16)
+    for lo, hi in ((0, 256), (8, 136), (3, 259), (1, 2)):
+        x = wide[:, lo:hi]
+        a, b = quantize_fp8(x), quantize_fp8(x.contiguous())
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    a, b = quantize_fp8(wide[::2, :64]), quantize_fp8(wide[::2, :64].contiguous())
+    assert torch.equal(a.codes, b.codes)
+
+
+@pytest.mark.parametrize("kind", PRODUCTS)
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_product_of_integers_is_exact(cuda_device, kind, m, n, k):
+    """Sums of at most 128 products up to 64 and their multiples of 1/16 up to 2^4: every partial sum is a binary32 number as long as
+    K * 64 * 16 * 16 < 2^24 * 16, so any order of summation gives the same result, and every element can be compared for equality."""
+    a, b, t = operands(kind, m, n, k, lambda s, bl: integers(s, cuda_device, m + 3 * n + 7 * k + len(bl), bl))
+    got = fp8_matmul(a, b, transpose_b=t, dtype=torch.float32)
+    want = expected(a, b, t)
+    assert torch.equal(got.double(), want)
+    assert torch.equal(fp8_matmul(a, b, transpose_b=t), want.float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", PRODUCTS)
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (129, 257, 1000), (640, 768, 4096)])
+def test_product_of_reals(cuda_device, kind, m, n, k):
+    """Tolerance: the tensor cores add 32 products at a time to a binary32 number; an addition that keeps 22 bits below its largest
+    operand errs by 2^-22 of the sum of magnitudes at most.  K/32 of those, K/128 fused multiply-adds, and the rounding of the result."""
+    g = torch.Generator(device=cuda_device).manual_seed(m + n + k)
+
+    def make(shape, blocks):
+        x = torch.randn(shape, device=cuda_device, generator=g) * torch.exp2(torch.randint(-3, 4, (shape[0], 1), device=cuda_device, generator=g).float())
+        return quantize_fp8(x.to(torch.bfloat16), blocks)
+
+    a, b, t = operands(kind, m, n, k, make)
+    want = expected(a, b, t)
+    x, y = numbers(a).abs(), numbers(b).abs()
+    size = (x.T if a.blocks == "columns" else x) @ (y.T if t else y)
+    steps = k / 32 + k / 128 + 2
+    assert bool(((fp8_matmul(a, b, transpose_b=t, dtype=torch.float32).double() - want).abs() <= steps * 2.0 ** -22 * size).all())
+    assert bool(((fp8_matmul(a, b, transpose_b=t).double() - want).abs() <= steps * 2.0 ** -22 * size + 2.0 ** -8 * want.abs()).all())
+
+
+@pytest.mark.parametrize("kind", PRODUCTS)
+def test_product_leaves_what_lies_beside_the_result(cuda_device, kind):
+    """The C entry with rows of C further apart than N, and rows behind the last one."""
+    m, n, k = 130, 131, 200
+    a, b, t = operands(kind, m, n, k, lambda s, bl: integers(s, cuda_device, 5, bl))
+    ids = {"rows": 1, "columns": 2, "tiles": 3}
+    for dtype, code in ((torch.bfloat16, 0), (torch.float32, 1)):
+        c = torch.full((m + 3, n + 9), 7.0, dtype=dtype, device=cuda_device)
+        assert _lib.lib().flame_fp8_product(a.codes.data_ptr(), a.stride, a.scales.data_ptr(), ids[a.blocks], b.codes.data_ptr(), b.stride,
+                                            b.scales.data_ptr(), ids[b.blocks], int(t), c.data_ptr(), n + 9, code, m, n, k,
+                                            torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(c[:m, :n], expected(a, b, t).to(dtype))
+        assert bool((c[m:] == 7).all()) and bool((c[:, n:] == 7).all())
+
+
+def test_empty_products(cuda_device):
+    def blank(r, c, bl):
+        ss = (r if bl == "rows" else up(r) // 128, c if bl == "columns" else up(c) // 128)
+        return Fp8Blocks(torch.zeros(r, up(c, 16), dtype=torch.uint8, device=cuda_device)[:, :c], torch.zeros(ss, device=cuda_device), bl)
+
+    for m, n, k in ((0, 5, 7), (5, 0, 7), (5, 7, 0), (0, 0, 0)):
+        y = fp8_matmul(blank(m, k, "rows"), blank(n, k, "tiles"), transpose_b=True)
+        assert y.shape == (m, n) and bool((y == 0).all())
+    x = torch.randn(0, 64, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(32, 64, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    fp8_linear(x, w).sum().backward()
+    assert x.grad.shape == (0, 64) and bool((w.grad == 0).all())
+
+
+def linear_reference(x, w, dy):
+    def q(t, blocks):
+        c, s = reference_quantise(t, blocks)
+        return c.view(torch.float8_e4m3fn).to(torch.float64) * spread(s, t.shape, blocks)
+
+    wq = q(w, "tiles")
+    return q(x, "rows") @ wq.T, q(dy, "rows") @ wq, q(dy, "columns").T @ q(x, "columns")
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 16, 16), (64, 128, 256), (200, 130, 77), (513, 300, 257)])
+def test_linear_and_its_gradients(cuda_device, m, n, k):
+    g = torch.Generator(device=cuda_device).manual_seed(m * n + k)
+    x = torch.randn(m, k, device=cuda_device, generator=g).to(torch.bfloat16).requires_grad_(True)
+    w = (torch.randn(n, k, device=cuda_device, generator=g) * k ** -0.5).to(torch.bfloat16).requires_grad_(True)
+    dy = torch.randn(m, n, device=cuda_device, generator=g).to(torch.bfloat16)
+    y = fp8_linear(x, w)
+    y.backward(dy)
+    wants = linear_reference(x.detach(), w.detach(), dy)
+    # binary32 sums of up to 513 terms, then one rounding: 2^-8 of the value, and 2^-14 of the norm for elements that cancel
+    for got, want in zip((y, x.grad, w.grad), wants):
+        err = (got.detach().double().cpu() - want).abs()
+        assert bool((err <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * want.abs().max()).all())
+    # against differences of the layer with the weight's quantised values, in the direction v: the quantisation of dy moves an
+    # element by at most 2^-4 of itself
+    v = torch.randn(m, k, device=cuda_device, generator=g).double().cpu()
+    wq = numbers(quantize_fp8(w.detach(), "tiles")).cpu()
+    loss = lambda t: float(((t @ wq.T) * dy.double().cpu()).sum())  # noqa: E731
+    x64 = x.detach().double().cpu()
+    slope = (loss(x64 + 0.5 * v) - loss(x64 - 0.5 * v))
+    bound = float(((v @ wq.T).abs() * dy.double().cpu().abs()).sum()) * 2.0 ** -4 + float((v.abs() * x.grad.double().cpu().abs()).sum()) * 2.0 ** -8
+    assert abs(slope - float((x.grad.double().cpu() * v).sum())) <= bound
+    # a frozen weight gives the same output and input gradient
+    x2 = x.detach().clone().requires_grad_(True)
+    y2 = fp8_linear(x2, quantize_fp8(w.detach(), "tiles"), codes=quantize_fp8(x2.detach()))
+    y2.backward(dy)
+    assert torch.equal(y2, y) and torch.equal(x2.grad, x.grad)
+
+
+def test_linear_over_leading_dimensions_and_broadcast_gradients(cuda_device):
+    x = torch.randn(2, 3, 5, 64, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(48, 64, device=cuda_device, dtype=torch.bfloat16, requires_grad=True)
+    y = fp8_linear(x, w)
+    assert y.shape == (2, 3, 5, 48)
+    y.sum().backward()                     # the gradient that arrives is an expanded scalar
+    x2, w2 = x.detach().view(30, 64).requires_grad_(True), w.detach().clone().requires_grad_(True)
+    fp8_linear(x2, w2).backward(torch.ones(30, 48, dtype=torch.bfloat16, device=cuda_device))
+    assert torch.equal(x.grad.view(30, 64), x2.grad) and torch.equal(w.grad, w2.grad)
+    only_x = x.detach().requires_grad_(True)
+    fp8_linear(only_x, w.detach()).sum().backward()
+    assert torch.equal(only_x.grad, x.grad)
+    only_w = w.detach().clone().requires_grad_(True)
+    fp8_linear(x.detach(), only_w).sum().backward()
+    assert torch.equal(only_w.grad, w.grad)
+    shared = x.detach().requires_grad_(True)       # one tensor in two calls: gradients add up
+    (fp8_linear(shared, w.detach()).sum() + fp8_linear(shared, w.detach()).sum()).backward()
+    assert torch.allclose(shared.grad.float(), 2 * x.grad.float(), rtol=2.0 ** -7)
+    v = torch.randn(64, device=cuda_device, dtype=torch.bfloat16)
+    assert torch.equal(fp8_linear(v, w.detach()), fp8_linear(v.view(1, 64), w.detach())[0])
+
+
+def test_same_bits_every_time_on_any_stream_and_in_a_graph(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x = torch.randn(77, 1024, device=cuda_device, generator=g).to(torch.bfloat16)
+    w = quantize_fp8(torch.randn(512, 1024, device=cuda_device, generator=g).to(torch.bfloat16), "tiles")
+    want = fp8_linear(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ys = [fp8_linear(x, w) for _ in range(4)]
+    here = [fp8_linear(x, w) for _ in range(4)]          # two streams at once
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in ys + here)
+    graph, x_in = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        y = fp8_linear(x_in, w)
+    for seed in (4, 5):
+        x_in.copy_(torch.randn(77, 1024, device=cuda_device, generator=g))
+        graph.replay()
+        assert torch.equal(y, fp8_linear(x_in, w))
+
+
+def test_a_training_step_recorded_in_a_graph(cuda_device):
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    x, w, dy = (torch.randn(s, device=cuda_device, generator=g).to(torch.bfloat16) for s in ((130, 256), (384, 256), (130, 384)))
+
+    def step(a, b):
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        y = fp8_linear(a, b)
+        return (y.detach(),) + torch.autograd.grad(y, (a, b), dy)
+
+    step(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, w)
+    x.copy_(torch.randn(130, 256, device=cuda_device, generator=g))
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(got, step(x, w)))
+
+
+def test_refusals(cuda_device):
+    x = torch.randn(8, 64, device=cuda_device, dtype=torch.bfloat16)
+    w = torch.randn(16, 64, device=cuda_device, dtype=torch.bfloat16)
+    qx, qw = quantize_fp8(x), quantize_fp8(w, "tiles")
+    with pytest.raises(InvalidShape, match="do not fit"):
+        fp8_linear(x, w[:, :32])
+    with pytest.raises(InvalidInput, match="BF16"):
+        fp8_linear(x, w.float())
+    with pytest.raises(InvalidShape):
+        fp8_linear(x.float(), w)
+    with pytest.raises(InvalidInput, match="one device|on the GPU"):
+        fp8_linear(x.cpu(), w)
+    with pytest.raises(Unsupported, match="along the contraction"):
+        fp8_matmul(quantize_fp8(x, "columns"), qw, transpose_b=True)
+    with pytest.raises(Unsupported):
+        fp8_matmul(qw, qw)
+    with pytest.raises(InvalidShape):
+        fp8_matmul(qx, quantize_fp8(w[:, :32].contiguous(), "tiles"), transpose_b=True)
+    with pytest.raises(Unsupported, match="input gradient"):
+        fp8_linear(x.clone().requires_grad_(True), quantize_fp8(w, "rows"))
+    with pytest.raises(InvalidShape, match="rows of x"):
+        fp8_linear(x, w, codes=quantize_fp8(x[:4]))
+    with pytest.raises(InvalidInput, match="neighbours"):
+        quantize_fp8(x.t())
+    with pytest.raises(InvalidInput, match="rows must not overlap"):
+        quantize_fp8(x[:1].expand(8, 64))
+    with pytest.raises(InvalidInput, match="multiple of 16"):
+        Fp8Blocks(torch.zeros(4, 20, dtype=torch.uint8, device=cuda_device), torch.zeros(4, 1, device=cuda_device), "rows")
+    with pytest.raises(InvalidShape, match="expected"):
+        Fp8Blocks(qx.codes, torch.zeros(8, 2, device=cuda_device), "rows")
+    lib = _lib.lib()
+    args = [qx.codes.data_ptr(), 64, qx.scales.data_ptr(), 1, qw.codes.data_ptr(), 64, qw.scales.data_ptr(), 3, 1, x.data_ptr(), 16, 0, 8, 16, 64, None]
+    for at, value, text in ((1, 60, "stride"), (3, 2, "contraction"), (10, 8, "stride"), (11, 5, "BF16 or F32"), (0, None, "null"), (0, qx.codes.data_ptr() + 8, "misaligned"),
+                            (12, 1 << 40, "too large")):
+        bad = list(args)
+        bad[at] = value
+        assert lib.flame_fp8_product(*bad) == 1 and text in _lib.last_error(), (at, _lib.last_error())
