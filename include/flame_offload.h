@@ -570,6 +570,9 @@ int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scal
 int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales, int a_blocks, const void* b_codes, size_t b_stride,
                       const void* b_scales, int b_blocks, int b_transposed, void* c, size_t c_stride, int c_dtype, size_t M,
                       size_t N, size_t K, void* stream);
+/* How often a wait inside a product's kernel on the current device gave up after two seconds since the library was loaded, in
+ * which case that product's result is wrong.  0 unless something else is broken.  Waits for the device. */
+int flame_fp8_product_faults(unsigned int* count);
 
 /* 8b. Group norm with an activation on a channels-last BF16 tensor x [B, L, C] (contiguous): C / G neighbouring channels a
  *     group, mean and variance over L x C/G elements, h = (x - mean) * rstd * weight + bias, y = h or silu(h), fp32 inside.

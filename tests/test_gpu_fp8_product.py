@@ -74,7 +74,8 @@ def expected(a, b, transpose_b):
 
 
 SIZES = [(1, 1, 1), (1, 2048, 2048), (3, 130, 257), (17, 1000, 129), (64, 64, 64), (127, 255, 383), (128, 128, 128), (129, 256, 640),
-         (256, 512, 1024), (300, 77, 2000), (513, 384, 96), (1000, 713, 1331), (2, 5000, 300), (1024, 16, 4096)]
+         (256, 512, 1024), (300, 77, 2000), (513, 384, 96), (1000, 713, 1331), (2, 5000, 300), (1024, 16, 4096),
+         (2100, 2600, 520), (19000, 250, 130), (100, 37890, 257), (2304, 4864, 1000)]     # more tiles than SMs
 
 
 @pytest.mark.parametrize("blocks", ["rows", "columns", "tiles"])
@@ -295,6 +296,12 @@ def test_a_training_step_recorded_in_a_graph(cuda_device):
     x.copy_(torch.randn(130, 256, device=cuda_device, generator=g))
     graph.replay()
     assert all(torch.equal(p, q) for p, q in zip(got, step(x, w)))
+
+
+def test_no_wait_ran_out(cuda_device):
+    import ctypes
+    n = ctypes.c_uint(7)
+    assert _lib.lib().flame_fp8_product_faults(ctypes.byref(n)) == 0 and n.value == 0
 
 
 def test_refusals(cuda_device):
