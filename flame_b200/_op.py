@@ -1,17 +1,21 @@
-"""What the operator modules share: argument checks, the device a call runs on, and the translation of the library's codes."""
+"""What the operator modules share: the device a call runs on, and the translation of the library's codes.
+
+These modules run once for every layer and step, and at small sizes the host decides how long that takes: messages are built only
+when something is refused, and a call that nobody differentiates leaves no autograd node.
+"""
 from __future__ import annotations
 
+import functools
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .errors import CudaError, InvalidInput
 
 DTYPE = {torch.bfloat16: 0, torch.float32: 1}     # FLAME_OFFLOAD_DTYPE_*
 
-
-def need(cond: bool, message: str, error=InvalidInput) -> None:
-    if not cond:
-        raise error(message)
+_FUNCTIONS: dict = {}
 
 
 def on_gpu(what: str, *tensors) -> torch.device:
@@ -20,26 +24,60 @@ def on_gpu(what: str, *tensors) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        need(isinstance(t, torch.Tensor), f"{what}: expected a tensor, got {type(t).__name__}")
-        need(t.is_cuda, f"{what}: the tensors must be on the GPU")
-        need(device is None or t.device == device, f"{what}: the tensors must be on one device")
-        device = t.device
+        if not isinstance(t, torch.Tensor):
+            raise InvalidInput(f"{what}: expected a tensor, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise InvalidInput(f"{what}: the tensors must be on the GPU")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise InvalidInput(f"{what}: the tensors must be on one device")
     return device
+
+
+def function(name: str):
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.lib(), name)
+    return fn
 
 
 def call(name: str, device: torch.device, *args) -> None:
     """`name`(*args, stream) on the current stream of `device`, whichever device is the current one."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = function(name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    if rc == 1:
-        raise InvalidInput(_lib.last_error() or f"{name}: invalid argument")
-    if rc != 0:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        if rc == 1:
+            raise InvalidInput(_lib.last_error() or f"{name}: invalid argument")
         raise CudaError(f"{name} failed ({rc})")
 
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def recorded(*tensors) -> bool:
+    """Whether autograd records a call on these tensors (None is skipped)."""
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def first_order(f):
+    """A backward that gives first derivatives: a second one is refused by autograd.  The wrapper that says so costs a third of a small
+    call's time, so only a backward pass that is itself recorded (``create_graph=True``) goes through it."""
+    recorded_form = once_differentiable(f)
+
+    @functools.wraps(f)
+    def backward(ctx, *grads):
+        return recorded_form(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
+
+    return staticmethod(backward)

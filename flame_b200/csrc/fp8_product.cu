@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "codec_kernels.cuh"
 #include "common.h"
 #include "fp8_device.cuh"
@@ -26,7 +28,9 @@ constexpr int kBlock = 128;
 // columns (one shuffle and eight partial maxima through shared memory), or of the tile.  The source is read once for both.
 constexpr int kQuantThreads = 256;
 
-struct QuantArgs {
+enum : uint32_t { kQuantRows = 1, kQuantTiles = 2, kQuantColumns = 4, kQuantWide = 8 };   // kQuantWide: 16-byte loads are possible
+
+struct QuantJob {
   const __nv_bfloat16* x;
   size_t x_stride;
   uint32_t rows, cols;
@@ -36,16 +40,22 @@ struct QuantArgs {
   float* col_scales;
   size_t code_stride;
   uint32_t tiles_across;     // ceil(cols / 128)
+  uint32_t tiles;
+  uint32_t mode;
 };
+// Up to two matrices in a launch: a layer's input and weight, or its output gradient and input.
+struct QuantJobs { QuantJob job[2]; };
 
-// kVec: 16-byte loads (rows start on 16 bytes and cols % 8 == 0)
-template <bool kVec, bool kRows, bool kCols, bool kTile>
-__global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_constant__ QuantArgs a) {
+__global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_constant__ QuantJobs jobs) {
   pdl_prologue();
   __shared__ float part[8][kBlock];
-  const uint32_t tm = blockIdx.x / a.tiles_across, tn = blockIdx.x % a.tiles_across;
+  const bool second = blockIdx.x >= jobs.job[0].tiles;
+  const QuantJob& a = jobs.job[second];
+  const uint32_t tile = blockIdx.x - (second ? jobs.job[0].tiles : 0);
+  const uint32_t tm = tile / a.tiles_across, tn = tile % a.tiles_across;
   const uint32_t t = threadIdx.x, lr = t >> 4, lc = t & 15;
   const uint32_t col = tn * kBlock + lc * 8;
+  const bool wide = a.mode & kQuantWide;
   uint4 raw[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -53,7 +63,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_c
     raw[j] = make_uint4(0u, 0u, 0u, 0u);
     if (row < a.rows && col < a.cols) {
       const __nv_bfloat16* src = a.x + (size_t)row * a.x_stride + col;
-      if (kVec) {
+      if (wide) {
         raw[j] = *reinterpret_cast<const uint4*>(src);
       } else {
         uint32_t w[4] = {0u, 0u, 0u, 0u};
@@ -73,22 +83,13 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_c
     const uint32_t row = tm * kBlock + lr + 16 * j;
     if (row < a.rows && col < a.cols) *reinterpret_cast<uint2*>(codes + (size_t)row * a.code_stride + col) = c;   // the row's padding gets zeros
   };
-  float cmax[8];
+  if (a.mode & kQuantRows) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) cmax[i] = 0.0f;
-  float tmax = 0.0f;
+    for (int j = 0; j < 8; ++j) {
+      float f[8], m = 0.0f;
+      unpack(j, f);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float f[8], m = 0.0f;
-    unpack(j, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = fabsf(f[i]);
-      if (kRows || kTile) m = fmaxf(m, v);
-      if (kCols) cmax[i] = fmaxf(cmax[i], v);
-    }
-    if (kTile) tmax = fmaxf(tmax, m);
-    if (kRows) {
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
       float s;
@@ -97,7 +98,15 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_c
       if (lc == 0 && row < a.rows) a.row_scales[(size_t)row * a.tiles_across + tn] = s;
     }
   }
-  if (kTile) {
+  if (a.mode & kQuantTiles) {
+    float tmax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float f[8];
+      unpack(j, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, fabsf(f[i]));
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xFFFFFFFFu, tmax, d));
     if ((t & 31) == 0) part[0][t >> 5] = tmax;
@@ -113,7 +122,17 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_c
     }
     if (t == 0) a.row_scales[(size_t)tm * a.tiles_across + tn] = s.scale;
   }
-  if (kCols) {
+  if (a.mode & kQuantColumns) {
+    float cmax[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cmax[i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float f[8];
+      unpack(j, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cmax[i] = fmaxf(cmax[i], fabsf(f[i]));
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) cmax[i] = fmaxf(cmax[i], __shfl_xor_sync(0xFFFFFFFFu, cmax[i], 16));
     if ((t & 16) == 0) {
@@ -189,27 +208,32 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 }
 
 // ---- product ------------------------------------------------------------------------
-// One pass over the contraction in blocks of 128.  Roles of a thread block (11 warps):
-//   warps 0-7  epilogue: per block of the contraction they read the tensor cores' sums from tensor memory (32 rows x BN/2 columns a
-//              warp, a thread is a row) and add them to fp32 registers with the block's scales;
-//   warp 8     copies tiles of both operands to shared memory (TMA, 128-byte swizzle, out-of-range elements are zeros);
-//   warp 9     issues tcgen05.mma kind::f8f6f4, four of them (32 deep each) for a block of 128, into one of two accumulators;
-//   warp 10    fetches the block's scales, one block ahead, and puts them into shared memory.
+// One pass over the contraction in blocks of 128.  Roles of a thread block (20 warps):
+//   warps 0-15  epilogue: per block of the contraction they read the tensor cores' sums from tensor memory (32 rows x a quarter of the
+//               columns a warp, a thread is a row) and add them to fp32 registers with the block's scales;
+//   warp 16     copies tiles of both operands to shared memory (TMA, 128-byte swizzle, out-of-range elements are zeros);
+//   warps 17, 18 issue tcgen05.mma kind::f8f6f4, four of them (32 deep each) for a block of 128; each has an accumulator of its own and
+//               takes every other block, so that one's waits pass while the other's products run;
+//   warp 19     copies the blocks' scales to a ring in shared memory (asynchronous 4-byte copies, three blocks ahead).
 // Operands lie in shared memory as they lie in global memory: along the contraction (K-major) or along the rows of C (MN-major,
 // the weight of the input gradient and both operands of the weight gradient), which the matrix descriptor says; nothing is
 // transposed.  A block's sum is scaled by one fused multiply-add a number, which is why each block needs an accumulator of its own
 // in tensor memory: two take turns, so that the tensor cores work on one while the other is read.
 //
-// Few tiles (serving, one token): a cluster of up to eight thread blocks shares a tile of C, each takes a range of the
-// contraction, and their sums are joined through distributed shared memory in the order of the ranks.
+// Two forms.  kPair, for many tiles: the two SMs of a pair work on one tile of 256 x 256 (cta_group::2), each holds half of either
+// operand, the leader issues the products for both.  Without it a block has a tile of 128 x 128, and where tiles are few (serving,
+// one token) a cluster of up to eight blocks shares one: each takes a range of the contraction, and their sums are joined through
+// distributed shared memory in the order of the ranks.
 //
-// Every wait gives up after two seconds: the kernel then counts the fault (flame_fp8_product_faults), waits for its own copies and
-// returns its tensor memory.
-constexpr int kEpiWarps = 8;
+// Every wait gives up after two seconds: the kernel then counts the fault (flame_fp8_product_faults), leaves its copies time to land
+// and returns its tensor memory.
+constexpr int kEpiWarps = 16;
 constexpr int kProductThreads = 32 * (kEpiWarps + 4);
-constexpr int kTileM = 128;
-constexpr int kStagePitch = 80;                 // bytes from row to row of a warp's output staging: 64 and 16 against bank conflicts
-constexpr int kStageBytes = 32 * kStagePitch;
+constexpr int kTileM = 128;                     // rows of a thread block
+constexpr int kStages = 6;
+constexpr int kSlots = 8;                       // blocks of scales in shared memory
+constexpr int kStagePitch = 36;                 // bytes from row to row of a warp's output staging: 32 and 4 against bank conflicts
+constexpr int kStagingBytes = 32 * kStagePitch;
 
 __device__ unsigned int g_wait_faults;
 
@@ -221,18 +245,19 @@ struct ProductArgs {
   uint32_t M, N, K;
   uint32_t sa_stride, sb_stride;   // floats between rows of the scale arrays
   uint32_t tiles_m, tiles_n, blocks_k;
-  uint32_t vec;                    // rows of C start on 16 bytes
+  uint32_t wide;                   // rows of C start on 32 bytes
 };
 
-template <int BN, int STAGES>
 struct ProductSmem {
-  static constexpr int kA = kTileM * kBlock, kB = BN * kBlock, kStage = kA + kB;
-  static constexpr int kScales = (kTileM + BN) * 4;                  // of one block of the contraction
-  static constexpr int kOffScales = STAGES * kStage;
-  static constexpr int kOffStaging = kOffScales + 2 * kScales;
-  static constexpr int kOffBars = kOffStaging + kEpiWarps * kStageBytes;
-  static constexpr int kBytes = kOffBars + 256 + 1024;               // and room to start on 1024 bytes
+  static constexpr int kOperand = kTileM * kBlock, kStage = 2 * kOperand;   // 128 x 128 bytes of either operand
+  static constexpr int kScales = (kTileM + 256) * 4;                        // of one block of the contraction
+  static constexpr int kOffScales = kStages * kStage;
+  static constexpr int kOffStaging = kOffScales + kSlots * kScales;
+  static constexpr int kOffBars = kOffStaging + kEpiWarps * kStagingBytes;
+  static constexpr int kBytes = kOffBars + 512 + 1024;                      // and room to start on 1024 bytes
 };
+static_assert(ProductSmem::kBytes <= 227 * 1024, "shared memory of a thread block");
+static_assert(kTileM * (128 + 4) * 4 <= kStages * ProductSmem::kStage, "a tile's sums fit over the pipeline's buffers");
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
@@ -257,8 +282,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
     }
   }
 }
+// kPair: the barrier may be the other block's of the pair
+template <bool kPair>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+  if constexpr (kPair)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
@@ -270,13 +301,37 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
   const uint64_t lead = kMn ? (kBlock * kBlock) >> 4 : 1, stride = 1024 >> 4;
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | (lead << 16) | (stride << 32) | (1ull << 46) | (2ull << 61);
 }
+template <bool kPair>
 __device__ __forceinline__ void mma_fp8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p; }"
-               ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+  if constexpr (kPair)
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p; }"
+                 ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+  else
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p; }"
+                 ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
+// One arrival when the products issued so far are done; in a pair, at the same barrier of both blocks.
+template <bool kPair>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (kPair)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// At a barrier of another block of the cluster.  Releases at the scope of this block, which orders the reads of the scales before
+// their place is written again; what it tells the other block is that tensor memory has been read, which tcgen05's own fences
+// order.  (A release at cluster scope took 1,300 cycles for each block of the contraction.)
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Four bytes from global to shared memory, zero where there is nothing to copy.
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4u : 0u) : "memory");
+}
+
 // The wait belongs to the same statement: nothing else tells the compiler that the registers are not there before it.
 __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -289,26 +344,6 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync_all() {
@@ -316,9 +351,8 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float4 peer_load4(uint32_t addr, uint32_t rank) {
-  uint32_t at;
+  const uint32_t at = at_rank(addr, rank);
   float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
   return v;
 }
@@ -335,265 +369,261 @@ __device__ __forceinline__ void tile_at(const ProductArgs& p, uint32_t t, uint32
 }
 
 template <typename T>
-__device__ __forceinline__ void to_bytes16(const float* v, uint4& o) {
+__device__ __forceinline__ uint32_t to_word(const float* v) {      // 4 bytes of C
   if constexpr (sizeof(T) == 2) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-    o = make_uint4(w[0], w[1], w[2], w[3]);
+    uint32_t w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(v[1]), "f"(v[0]));
+    return w;
   } else {
-    o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    return __float_as_uint(v[0]);
   }
 }
 
-template <bool kAmn, bool kBmn, bool kBvec, int BN, int STAGES, typename T>
+template <bool kPair, bool kAmn, bool kBmn, bool kBvec, typename T>
 __global__ void __launch_bounds__(kProductThreads, 1)
 fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ ProductArgs p) {
-  using S = ProductSmem<BN, STAGES>;
-  constexpr int kHalf = BN / 2;                                  // columns of an epilogue warp
-  constexpr uint32_t kTmemCols = 2 * BN;
+  using S = ProductSmem;
+  constexpr int kN = kPair ? 256 : 128;                          // columns of the tile
+  constexpr int kRows = kPair ? 256 : 128;                       // rows of the tile
+  constexpr int kCols = kN / 4;                                  // columns of an epilogue warp
+  constexpr uint32_t kTmemCols = 2 * kN;
   // D fp32, A and B e4m3, major-ness, N / 8, M / 16
-  constexpr uint32_t kIdesc = (1u << 4) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) | ((uint32_t)(BN / 8) << 17) | ((uint32_t)(kTileM / 16) << 24);
+  constexpr uint32_t kIdesc = (1u << 4) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) | ((uint32_t)(kN / 8) << 17) | ((uint32_t)(kRows / 16) << 24);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   const uint32_t base = smem_addr(smem);
   const uint32_t bars = base + S::kOffBars;
   auto full = [&](uint32_t s) { return bars + 8 * s; };
-  auto empty = [&](uint32_t s) { return bars + 8 * (STAGES + s); };
-  auto acc_full = [&](uint32_t b) { return bars + 8 * (2 * STAGES + b); };
-  auto acc_empty = [&](uint32_t b) { return bars + 8 * (2 * STAGES + 2 + b); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffBars + 8 * (2 * STAGES + 4));
+  auto empty = [&](uint32_t s) { return bars + 8 * (kStages + s); };
+  auto acc_full = [&](uint32_t b) { return bars + 8 * (2 * kStages + b); };
+  auto acc_empty = [&](uint32_t b) { return bars + 8 * (2 * kStages + 2 + b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffBars + 8 * (2 * kStages + 4));
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t splits = BN == 128 ? cluster_size() : 1, rank = BN == 128 ? cluster_rank() : 0;   // the large tile is never split
-  const uint32_t worker = blockIdx.x / splits, workers = gridDim.x / splits;
+  const uint32_t group = cluster_size(), rank = cluster_rank();  // a pair, or the blocks that share a tile's contraction
+  const uint32_t splits = kPair ? 1 : group, split = kPair ? 0 : rank;
+  const uint32_t worker = blockIdx.x / group, workers = gridDim.x / group;
   const uint32_t tiles = p.tiles_m * p.tiles_n;
-  const uint32_t kb0 = (uint32_t)((uint64_t)p.blocks_k * rank / splits), kb1 = (uint32_t)((uint64_t)p.blocks_k * (rank + 1) / splits);
+  const uint32_t kb0 = (uint32_t)((uint64_t)p.blocks_k * split / splits), kb1 = (uint32_t)((uint64_t)p.blocks_k * (split + 1) / splits);
+  const uint32_t row_off = kPair ? rank * kTileM : 0;            // of this block in the tile
+  bool ok = true;
 
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < STAGES; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
-    for (uint32_t b = 0; b < 2; ++b) { bar_init(acc_full(b), 2); bar_init(acc_empty(b), kEpiWarps); }
+    for (uint32_t s = 0; s < kStages; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
+    // an accumulator is full when the products are done and the block's scales are there
+    for (uint32_t b = 0; b < 2; ++b) { bar_init(acc_full(b), 2); bar_init(acc_empty(b), kPair ? 2 * kEpiWarps : kEpiWarps); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if (warp == kEpiWarps + 1) {
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tmem_fence_before();
   __syncthreads();
+  if (kPair) cluster_sync_all();      // the other block's barriers are ready
   tmem_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_prologue();
 
-  // The epilogue's sums need more registers than an equal share: 384 threads start with 168 each, 64,512 together; four warps go
-  // down to 88 and eight up to 208, 64,512 again.
+  // The epilogue's sums need more registers than an equal share: 640 threads start with 96 each, 61,440 together; four warps go down
+  // to 32 and sixteen up to 112, 61,440 again.
   if (warp < kEpiWarps) {
-    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const uint32_t quarter = warp & 3, half = warp >> 2;
+    if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    const uint32_t quarter = warp & 3, col_off = (warp >> 2) * kCols;
     const uint32_t row = quarter * 32 + lane;
+    const uint32_t release = at_rank(acc_empty(0), kPair ? 0 : rank);
     uint32_t it = 0;
-    bool ok = true;
     for (uint32_t t = worker; ok && t < tiles; t += workers) {
       uint32_t tm, tn;
       tile_at(p, t, tm, tn);
-      const uint32_t m0 = tm * kTileM + quarter * 32;
-      const uint32_t n0 = tn * BN + half * kHalf;
-      const bool rows_live = m0 < p.M && n0 < p.N;
-      uint64_t acc[kHalf / 2];
+      const uint32_t m0 = tm * kRows + row_off + quarter * 32;
+      const uint32_t n0 = tn * kN + col_off;
+      const bool live = m0 < p.M && n0 < p.N;
+      float acc[kCols];
 #pragma unroll
-      for (int i = 0; i < kHalf / 2; ++i) acc[i] = 0ull;
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
       for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t b = it & 1;
-        if (!(ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_full(b), (it >> 1) & 1)))) break;   // one answer for the warp
-        if (rows_live) {
-          tmem_fence_after();
-          const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + b * S::kScales);
-          const float sa = sc[row];
-          const uint32_t src = tmem + b * BN + half * kHalf + (quarter << 21);   // lane 32 * quarter in the upper 16 bits
-          uint64_t s2 = 0;
-          if (kBvec) s2 = pack2(__float_as_uint(sa), __float_as_uint(sa));
+        ok = ok && bar_wait(acc_full(b), (it >> 1) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
+        __syncwarp();
+        tmem_fence_after();
+        if (live) {
+          const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + it % kSlots * S::kScales);
+          const uint32_t src = tmem + b * kN + col_off + (quarter << 21);   // lane 32 * quarter in the upper 16 bits
+          const float sa = kBvec ? sc[row] : sc[row] * sc[kTileM + col_off / kBlock];
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 32) {
-            if (!kBvec && c % kBlock == 0) {
-              const uint32_t w = __float_as_uint(sa * sc[kTileM + (half * kHalf + c) / kBlock]);
-              s2 = pack2(w, w);
-            }
+          for (int c = 0; c < kCols; c += 32) {
             uint32_t v[32];
             tmem_load32(v, src + c);
+            if (c + 32 == kCols) {       // all is in registers: the accumulator is free for the block after the next
+              tmem_fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive_cluster(release + 8 * b);
+            }
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              uint64_t x0 = pack2(v[2 * i], v[2 * i + 1]), x1 = pack2(v[2 * i + 2], v[2 * i + 3]);
-              if (kBvec) {
-                const uint4 w = *reinterpret_cast<const uint4*>(sc + kTileM + half * kHalf + c + 2 * i);
-                x0 = mul2(x0, pack2(w.x, w.y));
-                x1 = mul2(x1, pack2(w.z, w.w));
-              }
-              acc[c / 2 + i] = fma2(x0, s2, acc[c / 2 + i]);
-              acc[c / 2 + i + 1] = fma2(x1, s2, acc[c / 2 + i + 1]);
+            for (int i = 0; i < 32; i += 4) {
+              float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+              if (kBvec) w = *reinterpret_cast<const float4*>(sc + kTileM + col_off + c + i);
+              acc[c + i] = fmaf(kBvec ? __uint_as_float(v[i]) * w.x : __uint_as_float(v[i]), sa, acc[c + i]);
+              acc[c + i + 1] = fmaf(kBvec ? __uint_as_float(v[i + 1]) * w.y : __uint_as_float(v[i + 1]), sa, acc[c + i + 1]);
+              acc[c + i + 2] = fmaf(kBvec ? __uint_as_float(v[i + 2]) * w.z : __uint_as_float(v[i + 2]), sa, acc[c + i + 2]);
+              acc[c + i + 3] = fmaf(kBvec ? __uint_as_float(v[i + 3]) * w.w : __uint_as_float(v[i + 3]), sa, acc[c + i + 3]);
             }
           }
-          tmem_fence_before();
+        } else if (lane == 0) {
+          bar_arrive_cluster(release + 8 * b);
         }
-        __syncwarp();
-        if (lane == 0) bar_arrive(acc_empty(b));
       }
-      if (BN != 128 || splits == 1) {
-        if (!rows_live || !ok) continue;
-        // 64 bytes of each of the warp's 32 rows at a time go through shared memory, so that neighbouring lanes write neighbouring columns
-        constexpr int kCols = 64 / sizeof(T), kPer = 16 / sizeof(T);
-        uint8_t* st = smem + S::kOffStaging + warp * kStageBytes;
+      if (kPair || splits == 1) {
+        if (!live) continue;
+        constexpr int kPer = 32 / sizeof(T);       // columns in 32 bytes
         const uint32_t rows = p.M - m0 < 32 ? p.M - m0 : 32;
+        T* out = static_cast<T*>(p.c) + (size_t)m0 * p.c_stride + n0;
+        uint8_t* st = smem + S::kOffStaging + warp * kStagingBytes;
 #pragma unroll
-        for (int c = 0; c < kHalf; c += kCols) {
-          if (n0 + c >= p.N) break;
-          float f[kCols];
+        for (int c = 0; c < kCols; c += kPer) {
+          uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < kCols / 2; ++i) { const float2 u = unpack2(acc[c / 2 + i]); f[2 * i] = u.x; f[2 * i + 1] = u.y; }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 o;
-            to_bytes16<T>(f + j * kPer, o);
-            *reinterpret_cast<uint4*>(st + lane * kStagePitch + 16 * j) = o;
-          }
-          __syncwarp();
-          T* out = static_cast<T*>(p.c) + (size_t)m0 * p.c_stride + n0 + c;
-          const uint32_t cols = p.N - (n0 + c) < (uint32_t)kCols ? p.N - (n0 + c) : kCols;
-          if (p.vec && cols == (uint32_t)kCols) {
-#pragma unroll
-            for (int r8 = 0; r8 < 32; r8 += 8) {
-              const uint32_t r = r8 + lane / 4, j = lane % 4;
-              if (r < rows) *reinterpret_cast<uint4*>(out + (size_t)r * p.c_stride + j * kPer) = *reinterpret_cast<const uint4*>(st + r * kStagePitch + 16 * j);
-            }
+          for (int i = 0; i < 8; ++i) w[i] = to_word<T>(acc + c + i * kPer / 8);
+          if (n0 + c >= p.N) {
+          } else if (p.wide && n0 + c + kPer <= p.N) {
+            // a whole sector of a row from each lane
+            if (lane < rows)
+              asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + (size_t)lane * p.c_stride + c), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                           "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
           } else {
-            constexpr uint32_t kRowsAtOnce = 32 / kCols;
-            for (uint32_t r = lane / kCols; r < rows; r += kRowsAtOnce) {
-              const uint32_t j = lane % kCols;
-              if (j < cols) out[(size_t)r * p.c_stride + j] = reinterpret_cast<const T*>(st + r * kStagePitch)[j];
-            }
-          }
-          __syncwarp();
-        }
-      } else {
-        // this block's share of the tile, over the pipeline's buffers: every copy has landed and every product has been read
-        float* mine = reinterpret_cast<float*>(smem) + (size_t)row * (BN + 4) + half * kHalf;
-        if (rows_live) {
+            // rows that start anywhere: through shared memory, so that neighbouring lanes write neighbouring columns
 #pragma unroll
-          for (int i = 0; i < kHalf / 2; i += 2) {
-            const float2 u = unpack2(acc[i]), w = unpack2(acc[i + 1]);
-            *reinterpret_cast<float4*>(mine + 2 * i) = make_float4(u.x, u.y, w.x, w.y);
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(st + lane * kStagePitch + 4 * i) = w[i];
+            __syncwarp();
+            const uint32_t cols = p.N - (n0 + c) < (uint32_t)kPer ? p.N - (n0 + c) : kPer, j = lane % kPer;
+            if (j < cols)
+              for (uint32_t r = lane / kPer; r < rows; r += 32 / kPer) out[(size_t)r * p.c_stride + c + j] = reinterpret_cast<const T*>(st + r * kStagePitch)[j];
+            __syncwarp();
           }
         }
+      } else if (live) {
+        // this block's share of the tile, over the pipeline's buffers: every copy has landed and every product has been read
+        float* mine = reinterpret_cast<float*>(smem) + (size_t)row * (kN + 4) + col_off;
+#pragma unroll
+        for (int i = 0; i < kCols; i += 4) *reinterpret_cast<float4*>(mine + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
       }
     }
   } else {
-    if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
+    if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if (warp == kEpiWarps) {
       if (lane == 0) {
         uint32_t it = 0;
-        bool ok = true;
-        for (uint32_t t = worker; ok && t < tiles; t += workers) {
+        for (uint32_t t = worker; t < tiles; t += workers) {
           uint32_t tm, tn;
           tile_at(p, t, tm, tn);
+          const int32_t m = (int32_t)(tm * kRows + row_off), n = (int32_t)(tn * kN + (kPair ? rank * kBlock : 0));
           for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-            const uint32_t s = it % STAGES, round = it / STAGES;
-            if (!(ok = bar_wait(empty(s), (round & 1) ^ 1))) break;
-            bar_expect(full(s), S::kStage);
-            const uint32_t sa = base + s * S::kStage, sb = sa + S::kA;
-            const int32_t k = (int32_t)(kb * kBlock), m = (int32_t)(tm * kTileM), n = (int32_t)(tn * BN);
-            if (kAmn) tma_load(sa, &map_a, m, k, full(s));
-            else tma_load(sa, &map_a, k, m, full(s));
-            if (kBmn) {
-#pragma unroll
-              for (int j = 0; j < BN / kBlock; ++j) tma_load(sb + j * kBlock * kBlock, &map_b, n + j * kBlock, k, full(s));
-            } else {
-              tma_load(sb, &map_b, k, n, full(s));
-            }
+            const uint32_t s = it % kStages;
+            if (!(ok = ok && bar_wait(empty(s), ((it / kStages) & 1) ^ 1))) continue;
+            // the leader's barrier counts the bytes of both blocks
+            if (!kPair || rank == 0) bar_expect(full(s), kPair ? 2 * S::kStage : S::kStage);
+            const uint32_t bar = kPair ? at_rank(full(s), 0) : full(s);
+            const uint32_t sa = base + s * S::kStage, sb = sa + S::kOperand;
+            const int32_t k = (int32_t)(kb * kBlock);
+            tma_load<kPair>(sa, &map_a, kAmn ? m : k, kAmn ? k : m, bar);
+            tma_load<kPair>(sb, &map_b, kBmn ? n : k, kBmn ? k : n, bar);
           }
         }
-        if (!ok)      // nothing may be in flight when the block ends
-          for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) bar_wait(full(i % STAGES), (i / STAGES) & 1);
       }
-      __syncwarp();
-    } else if (warp == 9) {
-      if (lane == 0) {
-        uint32_t it = 0;
-        bool ok = true;
-        for (uint32_t t = worker; ok && t < tiles; t += workers) {
-          for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-            const uint32_t s = it % STAGES, b = it & 1;
-            if (!(ok = bar_wait(acc_empty(b), ((it >> 1) & 1) ^ 1))) break;
-            if (!(ok = bar_wait(full(s), (it / STAGES) & 1))) break;
-            tmem_fence_after();
-            const uint32_t sa = base + s * S::kStage, sb = sa + S::kA;
-            // 32 deep a step: 32 bytes along a K-major row, 32 rows of 128 bytes of an MN-major tile
+    } else if (warp <= kEpiWarps + 2) {
+      if (lane == 0 && (!kPair || rank == 0)) {
+        const uint32_t b = warp - (kEpiWarps + 1);     // the accumulator; this warp's blocks are b, b + 2, ...
+        const uint32_t mine = tiles > worker ? (tiles - worker + workers - 1) / workers * (kb1 - kb0) : 0;   // of all the block's tiles
+        for (uint32_t it = b; it < mine; it += 2) {
+          const uint32_t s = it % kStages;
+          if (!(ok = ok && bar_wait(full(s), (it / kStages) & 1) && bar_wait(acc_empty(b), ((it >> 1) & 1) ^ 1))) continue;
+          tmem_fence_after();
+          const uint32_t sa = base + s * S::kStage, sb = sa + S::kOperand;
+          // 32 deep a step: 32 bytes along a K-major row, 32 rows of 128 bytes of an MN-major tile
 #pragma unroll
-            for (int j = 0; j < kBlock / 32; ++j)
-              mma_fp8(tmem + b * BN, smem_desc<kAmn>(sa + j * (kAmn ? 32 * kBlock : 32)), smem_desc<kBmn>(sb + j * (kBmn ? 32 * kBlock : 32)), kIdesc, j > 0);
-            mma_commit(empty(s));
-            mma_commit(acc_full(b));
-          }
+          for (int j = 0; j < kBlock / 32; ++j)
+            mma_fp8<kPair>(tmem + b * kN, smem_desc<kAmn>(sa + j * (kAmn ? 32 * kBlock : 32)), smem_desc<kBmn>(sb + j * (kBmn ? 32 * kBlock : 32)), kIdesc, j > 0);
+          mma_commit<kPair>(empty(s));
+          mma_commit<kPair>(acc_full(b));
         }
-        if (!ok && it > 0) bar_wait(empty((it - 1) % STAGES), ((it - 1) / STAGES) & 1);
       }
-      __syncwarp();
-    } else if (warp == 10) {
+    } else {
+      // Copies run kAhead blocks ahead.  When block i - 2 has its products, every warp of the epilogue has given block i - 4's accumulator
+      // back, which it does after its last use of block i - 5's scales: their place in the ring is free for block i + 3's.
+      constexpr uint32_t kAhead = 3;
+      static_assert(kSlots == kAhead + 5, "the argument above");
+      uint32_t t_copy = worker, kb_copy = kb1, slot_at = base + S::kOffScales, a_left = 0, b_left = 0;
+      const float *pa = p.sa, *pb = p.sb;
+      // from one row (column) of the tile to the 32nd after it, and from one block of the contraction to the next
+      const size_t a32 = kAmn ? 32 : 32 * (size_t)p.sa_stride, b32 = kBmn ? 32 : 32 * (size_t)p.sb_stride;
+      auto copy_next = [&]() {
+        if (kb_copy == kb1 && t_copy < tiles) {      // a new tile: this lane's first row and column of scales
+          uint32_t tm, tn;
+          tile_at(p, t_copy, tm, tn);
+          t_copy += workers;
+          kb_copy = kb0;
+          const uint32_t m = tm * kRows + row_off + lane, n = kBvec ? tn * kN + lane : tn * (kN / kBlock) + lane;
+          const uint32_t n_end = kBvec ? p.N : (p.N + kBlock - 1) / kBlock;
+          a_left = m < p.M ? p.M - m : 0;            // the lane's rows are live while 32 * i < a_left
+          b_left = n < n_end ? n_end - n : 0;
+          pa = p.sa + (a_left == 0 ? 0 : kAmn ? (size_t)kb0 * p.sa_stride + m : (size_t)m * p.sa_stride + kb0);
+          pb = p.sb + (b_left == 0 ? 0 : kBmn ? (size_t)kb0 * p.sb_stride + n : (size_t)n * p.sb_stride + kb0);
+        }
+        if (kb_copy < kb1) {
+#pragma unroll
+          for (uint32_t i = 0; i < kTileM / 32; ++i) copy4(slot_at + (i * 32 + lane) * 4, i * 32 < a_left ? pa + i * a32 : p.sa, i * 32 < a_left);
+          if constexpr (kBvec) {
+#pragma unroll
+            for (uint32_t i = 0; i < kN / 32; ++i) copy4(slot_at + (kTileM + i * 32 + lane) * 4, i * 32 < b_left ? pb + i * b32 : p.sb, i * 32 < b_left);
+          } else if (lane < kN / kBlock) {
+            copy4(slot_at + (kTileM + lane) * 4, b_left ? pb : p.sb, b_left != 0);
+          }
+          if (a_left) pa += kAmn ? p.sa_stride : 1;
+          if (b_left) pb += kBmn ? p.sb_stride : 1;
+          ++kb_copy;
+        }
+        slot_at = slot_at + S::kScales == base + S::kOffScales + kSlots * S::kScales ? base + S::kOffScales : slot_at + S::kScales;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      for (uint32_t i = 0; i < kAhead; ++i) copy_next();
       uint32_t it = 0;
-      bool ok = true;
-      constexpr int kNb = kBvec ? BN / 32 : 1;
-      for (uint32_t t = worker; ok && t < tiles; t += workers) {
-        uint32_t tm, tn;
-        tile_at(p, t, tm, tn);
-        float a[kTileM / 32], bsc[kNb];
-        auto fetch = [&](uint32_t kb) {
-#pragma unroll
-          for (int i = 0; i < kTileM / 32; ++i) {
-            const uint32_t m = tm * kTileM + i * 32 + lane;
-            a[i] = m < p.M ? __ldg(p.sa + (kAmn ? (size_t)kb * p.sa_stride + m : (size_t)m * p.sa_stride + kb)) : 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < kNb; ++i) {
-            if (kBvec) {
-              const uint32_t n = tn * BN + i * 32 + lane;
-              bsc[i] = n < p.N ? __ldg(p.sb + (kBmn ? (size_t)kb * p.sb_stride + n : (size_t)n * p.sb_stride + kb)) : 0.0f;
-            } else {
-              const uint32_t nb = tn * (BN / kBlock) + lane;
-              bsc[i] = lane < BN / kBlock && nb * kBlock < p.N ? __ldg(p.sb + (kBmn ? (size_t)kb * p.sb_stride + nb : (size_t)nb * p.sb_stride + kb)) : 0.0f;
-            }
-          }
-        };
-        if (kb0 < kb1) fetch(kb0);
+      for (uint32_t t = worker; t < tiles; t += workers)
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t b = it & 1;
-          if (!(ok = __all_sync(0xFFFFFFFFu, bar_wait(acc_empty(b), ((it >> 1) & 1) ^ 1)))) break;
-          float* sc = reinterpret_cast<float*>(smem + S::kOffScales + b * S::kScales);
-#pragma unroll
-          for (int i = 0; i < kTileM / 32; ++i) sc[i * 32 + lane] = a[i];
-          if (kBvec) {
-#pragma unroll
-            for (int i = 0; i < kNb; ++i) sc[kTileM + i * 32 + lane] = bsc[i];
-          } else if (lane < BN / kBlock) {
-            sc[kTileM + lane] = bsc[0];
-          }
+          if (it >= 2) ok = ok && bar_wait(acc_full(b), ((it >> 1) & 1) ^ 1);
+          __syncwarp();
+          copy_next();
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");   // block `it` has landed
           __syncwarp();
           if (lane == 0) bar_arrive(acc_full(b));
-          if (kb + 1 < kb1) fetch(kb + 1);
         }
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   }
 
+  if (!ok) {      // a wait ran out: the copies and products in flight get a millisecond to end
+    const uint64_t since = clock_ns();
+    while (clock_ns() - since < 1000000ull) {}
+  }
   __syncwarp();
-  if (BN == 128 && splits > 1) {      // one tile for each cluster
+  if (!kPair && splits > 1) {      // one tile for each cluster
     cluster_sync_all();
     if (warp < kEpiWarps && worker < tiles) {
       uint32_t tm, tn;
       tile_at(p, worker, tm, tn);
+      constexpr uint32_t kEpiThreads = 32 * kEpiWarps;
       const uint32_t rows = p.M - tm * kTileM < (uint32_t)kTileM ? p.M - tm * kTileM : kTileM;
-      for (uint32_t i = rank * 256 + threadIdx.x; i < rows * (BN / 4); i += splits * 256) {
-        const uint32_t r = i / (BN / 4), c = i % (BN / 4) * 4, n = tn * BN + c;
+      for (uint32_t i = rank * kEpiThreads + threadIdx.x; i < rows * (kN / 4); i += splits * kEpiThreads) {
+        const uint32_t r = i / (kN / 4), c = i % (kN / 4) * 4, n = tn * kN + c;
         if (n >= p.N) continue;
-        const uint32_t at = base + (r * (BN + 4) + c) * 4;
+        const uint32_t at = base + (r * (kN + 4) + c) * 4;
         float4 sum = peer_load4(at, 0);
         for (uint32_t k = 1; k < splits; ++k) {
           const float4 v = peer_load4(at, k);
@@ -610,12 +640,15 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       }
     }
     __syncwarp();
-    cluster_sync_all();   // nobody's shared memory goes away while it is read
   }
   tmem_fence_before();
   __syncthreads();
+  if (kPair || splits > 1) cluster_sync_all();   // nobody's shared or tensor memory goes away while another block of the cluster uses it
   tmem_fence_after();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  if (warp == kEpiWarps + 1) {
+    if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -629,12 +662,12 @@ EncodeTiled encode_tiled() {
   }();
   return f;
 }
-// rows x cols bytes, `stride` bytes from row to row, copied as 128 columns x `high` rows
-bool byte_matrix(CUtensorMap* map, const uint8_t* p, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t high) {
+// rows x cols bytes, `stride` bytes from row to row, copied as 128 x 128
+bool byte_matrix(CUtensorMap* map, const uint8_t* p, uint64_t rows, uint64_t cols, uint64_t stride) {
   const EncodeTiled f = encode_tiled();
   if (!f) return false;
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride};
-  const cuuint32_t box[2] = {kBlock, high}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {kBlock, kBlock}, one[2] = {1, 1};
   return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -645,25 +678,29 @@ struct Operands {
   size_t a_stride, b_stride;
 };
 
-template <bool kAmn, bool kBmn, bool kBvec, int BN, int STAGES, typename T>
-cudaError_t launch_tiles(const Operands& o, ProductArgs p, uint32_t splits, uint32_t blocks, cudaStream_t stream) {
+template <bool kPair, bool kAmn, bool kBmn, bool kBvec, typename T>
+cudaError_t launch_tiles(const Operands& o, const ProductArgs& p, uint32_t group, uint32_t blocks, cudaStream_t stream) {
   CUtensorMap map_a, map_b;
-  const bool ok = byte_matrix(&map_a, o.a, kAmn ? p.K : p.M, kAmn ? p.M : p.K, o.a_stride, kTileM) &&
-                  byte_matrix(&map_b, o.b, kBmn ? p.K : p.N, kBmn ? p.N : p.K, o.b_stride, kBmn ? kBlock : BN);
+  const bool ok = byte_matrix(&map_a, o.a, kAmn ? p.K : p.M, kAmn ? p.M : p.K, o.a_stride) && byte_matrix(&map_b, o.b, kBmn ? p.K : p.N, kBmn ? p.N : p.K, o.b_stride);
   if (!ok) return cudaErrorNotSupported;
-  auto kern = fp8_product_kernel<kAmn, kBmn, kBvec, BN, STAGES, T>;
-  constexpr int kSmem = ProductSmem<BN, STAGES>::kBytes;
-  if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) return e;
+  auto kern = fp8_product_kernel<kPair, kAmn, kBmn, kBvec, T>;
+  static std::atomic<uint64_t> allowed{0};     // a bit for each device on which the kernel may use this much shared memory
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ProductSmem::kBytes)) return e;
+    if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kProductThreads);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = ProductSmem::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (splits > 1) {
+  if (group > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = splits;
+    attr[n].val.clusterDim.x = group;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
@@ -681,18 +718,19 @@ template <bool kAmn, bool kBmn, bool kBvec, typename T>
 cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stream) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  p.tiles_m = (p.M + kTileM - 1) / kTileM;
   p.blocks_k = (p.K + kBlock - 1) / kBlock;
-  p.vec = (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && (p.c_stride * sizeof(T)) % 16 == 0;
+  p.wide = (reinterpret_cast<uintptr_t>(p.c) & 31u) == 0 && (p.c_stride * sizeof(T)) % 32 == 0;
+  const uint32_t pairs = (uint32_t)sms / 2;
+  p.tiles_m = (p.M + 255) / 256;
   p.tiles_n = (p.N + 255) / 256;
-  uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-  if (tiles >= (uint64_t)sms) return launch_tiles<kAmn, kBmn, kBvec, 256, 4, T>(o, p, 1, (uint32_t)sms, stream);
+  if ((uint64_t)p.tiles_m * p.tiles_n >= pairs) return launch_tiles<true, kAmn, kBmn, kBvec, T>(o, p, 2, 2 * pairs, stream);
+  p.tiles_m = (p.M + 127) / 128;
   p.tiles_n = (p.N + 127) / 128;
-  tiles = (uint64_t)p.tiles_m * p.tiles_n;
+  const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
   uint32_t splits = 1;
   while (splits < 8 && tiles * splits * 2 <= (uint64_t)sms && splits * 2 <= p.blocks_k) splits *= 2;
   const uint32_t blocks = splits > 1 ? (uint32_t)tiles * splits : (uint32_t)(tiles < (uint64_t)sms ? tiles : (uint64_t)sms);
-  return launch_tiles<kAmn, kBmn, kBvec, 128, 5, T>(o, p, splits, blocks, stream);
+  return launch_tiles<false, kAmn, kBmn, kBvec, T>(o, p, splits, blocks, stream);
 }
 
 template <bool kAmn, bool kBmn, bool kBvec>
@@ -706,6 +744,59 @@ int refuse(const char* who, const char* what) {
   return (int)cudaErrorInvalidValue;
 }
 constexpr uint64_t kMostSize = 0x7FFFFFFFull / 2;
+size_t up16(size_t n) { return n == 0 ? 16 : (n + 15) / 16 * 16; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+uint64_t blocks_of(uint64_t n) { return (n + kBlock - 1) / kBlock; }
+// codes and, on the next 256 bytes, scales
+size_t codes_bytes(size_t rows, size_t cols, uint32_t mode) {
+  return up256(rows * up16(cols)) + up256((mode == kQuantColumns ? blocks_of(rows) * cols : rows * blocks_of(cols)) * sizeof(float));
+}
+
+// What is wrong with a BF16 matrix as a source of codes; NULL: nothing.
+const char* quant_source(const void* x, size_t rows, size_t cols, size_t stride) {
+  if (rows > kMostSize || cols > kMostSize || blocks_of(rows) * blocks_of(cols) > 0x3FFFFFFFull) return "matrix too large";
+  if (stride < cols) return "a stride is smaller than the row";
+  if (rows == 0 || cols == 0) return nullptr;
+  if (!x) return "null tensor";
+  return al(x, 2) ? nullptr : "misaligned tensor";
+}
+QuantJob quant_job(const void* x, size_t rows, size_t cols, size_t x_stride, uint32_t mode, void* row_codes, void* row_scales, void* col_codes, void* col_scales,
+                   size_t code_stride) {
+  QuantJob a;
+  a.x = static_cast<const __nv_bfloat16*>(x); a.x_stride = x_stride; a.rows = (uint32_t)rows; a.cols = (uint32_t)cols;
+  a.row_codes = static_cast<uint8_t*>(row_codes); a.row_scales = static_cast<float*>(row_scales);
+  a.col_codes = static_cast<uint8_t*>(col_codes); a.col_scales = static_cast<float*>(col_scales);
+  a.code_stride = code_stride; a.tiles_across = (uint32_t)blocks_of(cols);
+  a.tiles = (uint32_t)(blocks_of(rows) * blocks_of(cols));
+  a.mode = mode | (al(x, 16) && x_stride % 8 == 0 && cols % 8 == 0 ? kQuantWide : 0u);
+  return a;
+}
+cudaError_t launch_quant(const QuantJob& a, const QuantJob& b, cudaStream_t stream) {
+  QuantJobs jobs;
+  jobs.job[0] = a;
+  jobs.job[1] = b;
+  return launch_after(fp8_quant_kernel, a.tiles + b.tiles, kQuantThreads, 0, stream, jobs);
+}
+
+enum class Product { kNtTiles, kNtRows, kNnTiles, kTnColumns };
+cudaError_t product(Product kind, const void* a, size_t a_stride, const void* sa, const void* b, size_t b_stride, const void* sb, void* c, size_t c_stride, bool f32,
+                    size_t M, size_t N, size_t K, cudaStream_t s) {
+  if (K == 0) {   // an empty sum
+    const size_t size = f32 ? 4 : 2;
+    return cudaMemset2DAsync(c, c_stride * size, 0, N * size, M, s);
+  }
+  const Operands o = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b), a_stride, b_stride};
+  ProductArgs p = {};
+  p.sa = static_cast<const float*>(sa); p.sb = static_cast<const float*>(sb);
+  p.c = c; p.c_stride = c_stride;
+  p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K;
+  p.sa_stride = kind == Product::kTnColumns ? (uint32_t)M : (uint32_t)blocks_of(K);
+  p.sb_stride = kind == Product::kTnColumns ? (uint32_t)N : (uint32_t)blocks_of(kind == Product::kNnTiles ? N : K);
+  if (kind == Product::kNtTiles) return launch_product<false, false, false>(o, p, f32, s);
+  if (kind == Product::kNtRows) return launch_product<false, false, true>(o, p, f32, s);
+  if (kind == Product::kNnTiles) return launch_product<false, true, false>(o, p, f32, s);
+  return launch_product<true, true, true>(o, p, f32, s);
+}
 
 }  // namespace
 }  // namespace flame_b200
@@ -720,26 +811,16 @@ int flame_fp8_quant_2d(const void* x, size_t rows, size_t cols, size_t x_stride,
   const bool tile = blocks == FLAME_FP8_BLOCKS_TILES, row = blocks == FLAME_FP8_BLOCKS_ROWS, col = column_codes != nullptr;
   if (!tile && !row && blocks != 0) return refuse(who, "blocks must be 0, FLAME_FP8_BLOCKS_ROWS or FLAME_FP8_BLOCKS_TILES");
   if (tile && col) return refuse(who, "tiles and columns are not made in one call");
-  if (rows > kMostSize || cols > kMostSize) return refuse(who, "matrix too large");
-  if (x_stride < cols || code_stride < cols || code_stride % 16 != 0) return refuse(who, "a stride is smaller than the row, or the code stride is no multiple of 16");
+  if (const char* what = quant_source(x, rows, cols, x_stride)) return refuse(who, what);
+  if (code_stride < cols || code_stride % 16 != 0) return refuse(who, "the code stride is smaller than the row, or no multiple of 16");
   if (rows == 0 || cols == 0) return 0;
   if (!tile && !row && !col) return refuse(who, "nothing to make");
-  if (!x || ((tile || row) && (!codes || !scales)) || (col && !column_scales)) return refuse(who, "null tensor");
-  if (!al(x, 2) || !al(codes, 16) || !al(column_codes, 16) || !al(scales, 4) || !al(column_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  const uint64_t down = (rows + 127) / 128, across = (cols + 127) / 128;
-  if (down * across > 0x7FFFFFFFull) return refuse(who, "matrix too large");
+  if (((tile || row) && (!codes || !scales)) || (col && !column_scales)) return refuse(who, "null tensor");
+  if (!al(codes, 16) || !al(column_codes, 16) || !al(scales, 4) || !al(column_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
-  QuantArgs a;
-  a.x = static_cast<const __nv_bfloat16*>(x); a.x_stride = x_stride; a.rows = (uint32_t)rows; a.cols = (uint32_t)cols;
-  a.row_codes = static_cast<uint8_t*>(codes); a.row_scales = static_cast<float*>(scales);
-  a.col_codes = static_cast<uint8_t*>(column_codes); a.col_scales = static_cast<float*>(column_scales);
-  a.code_stride = code_stride; a.tiles_across = (uint32_t)across;
-  const bool vec = al(x, 16) && x_stride % 8 == 0 && cols % 8 == 0;
-  auto go = [&](auto kern) { return (int)launch_after(kern, (unsigned)(down * across), kQuantThreads, 0, (cudaStream_t)stream, a); };
-  if (tile) return vec ? go(fp8_quant_kernel<true, false, false, true>) : go(fp8_quant_kernel<false, false, false, true>);
-  if (row && col) return vec ? go(fp8_quant_kernel<true, true, true, false>) : go(fp8_quant_kernel<false, true, true, false>);
-  if (row) return vec ? go(fp8_quant_kernel<true, true, false, false>) : go(fp8_quant_kernel<false, true, false, false>);
-  return vec ? go(fp8_quant_kernel<true, false, true, false>) : go(fp8_quant_kernel<false, false, true, false>);
+  const QuantJob a = quant_job(x, rows, cols, x_stride, (tile ? kQuantTiles : 0u) | (row ? kQuantRows : 0u) | (col ? kQuantColumns : 0u), codes, scales,
+                               column_codes, column_scales, code_stride);
+  return (int)launch_quant(a, QuantJob{}, (cudaStream_t)stream);
 }
 
 int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scales, int blocks, void* out, int out_dtype, size_t rows,
@@ -768,40 +849,91 @@ int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scal
 int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales, int a_blocks, const void* b_codes, size_t b_stride,
                       const void* b_scales, int b_blocks, int b_transposed, void* c, size_t c_stride, int c_dtype, size_t M, size_t N, size_t K, void* stream) {
   const char* who = "flame_fp8_product";
-  const bool nt_tiles = a_blocks == FLAME_FP8_BLOCKS_ROWS && b_blocks == FLAME_FP8_BLOCKS_TILES && b_transposed;
-  const bool nt_rows = a_blocks == FLAME_FP8_BLOCKS_ROWS && b_blocks == FLAME_FP8_BLOCKS_ROWS && b_transposed;
-  const bool nn_tiles = a_blocks == FLAME_FP8_BLOCKS_ROWS && b_blocks == FLAME_FP8_BLOCKS_TILES && !b_transposed;
-  const bool tn_cols = a_blocks == FLAME_FP8_BLOCKS_COLUMNS && b_blocks == FLAME_FP8_BLOCKS_COLUMNS && !b_transposed;
-  if (!nt_tiles && !nt_rows && !nn_tiles && !tn_cols)
-    return refuse(who, "the blocks of both operands must run along the contraction: rows x rows^T, rows x tiles^T, rows x tiles or columns^T x columns");
+  Product kind;
+  if (a_blocks == FLAME_FP8_BLOCKS_ROWS && b_blocks == FLAME_FP8_BLOCKS_TILES) kind = b_transposed ? Product::kNtTiles : Product::kNnTiles;
+  else if (a_blocks == FLAME_FP8_BLOCKS_ROWS && b_blocks == FLAME_FP8_BLOCKS_ROWS && b_transposed) kind = Product::kNtRows;
+  else if (a_blocks == FLAME_FP8_BLOCKS_COLUMNS && b_blocks == FLAME_FP8_BLOCKS_COLUMNS && !b_transposed) kind = Product::kTnColumns;
+  else return refuse(who, "the blocks of both operands must run along the contraction: rows x rows^T, rows x tiles^T, rows x tiles or columns^T x columns");
   if (c_dtype != FLAME_OFFLOAD_DTYPE_BF16 && c_dtype != FLAME_OFFLOAD_DTYPE_F32) return refuse(who, "the output is BF16 or F32");
   if (M > kMostSize || N > kMostSize || K > kMostSize) return refuse(who, "matrix too large");
-  const size_t a_row = tn_cols ? M : K, b_row = b_transposed ? K : N;
+  const size_t a_row = kind == Product::kTnColumns ? M : K, b_row = b_transposed ? K : N;
   if (a_stride < a_row || b_stride < b_row || a_stride % 16 != 0 || b_stride % 16 != 0 || c_stride < N) return refuse(who, "a stride is smaller than its row, or a code stride no multiple of 16");
   if (M == 0 || N == 0) return 0;
   if (!c || !al(c, c_dtype == FLAME_OFFLOAD_DTYPE_F32 ? 4 : 2)) return refuse(who, "null or misaligned output");
-  if (K == 0) {   // an empty sum
-    const size_t size = c_dtype == FLAME_OFFLOAD_DTYPE_F32 ? 4 : 2;
-    return (int)cudaMemset2DAsync(c, c_stride * size, 0, N * size, M, (cudaStream_t)stream);
-  }
-  if (!a_codes || !b_codes || !a_scales || !b_scales) return refuse(who, "null tensor");
+  if (K != 0 && (!a_codes || !b_codes || !a_scales || !b_scales)) return refuse(who, "null tensor");
   if (!al(a_codes, 16) || !al(b_codes, 16) || !al(a_scales, 4) || !al(b_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  if (((M + 63) / 64) * ((N + 63) / 64) > 0x7FFFFFFFull) return refuse(who, "matrix too large");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
-  const Operands o = {static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(b_codes), a_stride, b_stride};
-  ProductArgs p = {};
-  p.sa = static_cast<const float*>(a_scales); p.sb = static_cast<const float*>(b_scales);
-  p.c = c; p.c_stride = c_stride;
-  p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K;
-  auto blocks_of = [](size_t n) { return (uint32_t)((n + 127) / 128); };
-  p.sa_stride = tn_cols ? (uint32_t)M : blocks_of(K);
-  p.sb_stride = tn_cols ? (uint32_t)N : nn_tiles ? blocks_of(N) : blocks_of(K);
-  const bool f32 = c_dtype == FLAME_OFFLOAD_DTYPE_F32;
+  return (int)product(kind, a_codes, a_stride, a_scales, b_codes, b_stride, b_scales, c, c_stride, c_dtype == FLAME_OFFLOAD_DTYPE_F32, M, N, K, (cudaStream_t)stream);
+}
+
+size_t flame_fp8_linear_workspace_bytes(size_t M, size_t N, size_t K, int backward) {
+  if (M > kMostSize || N > kMostSize || K > kMostSize) return 0;
+  return backward ? codes_bytes(M, N, kQuantRows) + codes_bytes(M, N, kQuantColumns) + codes_bytes(M, K, kQuantColumns) : codes_bytes(M, K, kQuantRows);
+}
+
+int flame_fp8_linear(const void* x, size_t x_stride, const void* x_codes, size_t x_code_stride, const void* x_scales, const void* w,
+                     size_t w_stride, void* w_codes, size_t w_code_stride, void* w_scales, int w_blocks, void* y, size_t M, size_t N,
+                     size_t K, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "flame_fp8_linear";
+  if (w_blocks != FLAME_FP8_BLOCKS_TILES && (w_blocks != FLAME_FP8_BLOCKS_ROWS || w)) return refuse(who, "the blocks of a weight are tiles, or rows where it is given as codes");
+  if (!x_codes)
+    if (const char* what = quant_source(x, M, K, x_stride)) return refuse(who, what);
+  if (w)
+    if (const char* what = quant_source(w, N, K, w_stride)) return refuse(who, what);
+  if (M > kMostSize || N > kMostSize || K > kMostSize) return refuse(who, "matrix too large");
+  if (w_code_stride < K || w_code_stride % 16 != 0 || (x_codes && (x_code_stride < K || x_code_stride % 16 != 0))) return refuse(who, "a code stride is smaller than the row, or no multiple of 16");
+  if (N == 0 || (M == 0 && !w)) return 0;
+  if ((M > 0 && !y) || (K > 0 && (!w_codes || !w_scales)) || (x_codes && !x_scales)) return refuse(who, "null tensor");
+  if (!al(y, 2) || !al(w_codes, 16) || !al(w_scales, 4) || !al(x_codes, 16) || !al(x_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
+  if (!x_codes && M > 0 && K > 0 && (!workspace || !al(workspace, 256) || workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, 0)))
+    return refuse(who, "workspace too small, or not on 256 bytes");
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
   cudaStream_t s = (cudaStream_t)stream;
-  if (nt_tiles) return (int)launch_product<false, false, false>(o, p, f32, s);
-  if (nt_rows) return (int)launch_product<false, false, true>(o, p, f32, s);
-  if (nn_tiles) return (int)launch_product<false, true, false>(o, p, f32, s);
-  return (int)launch_product<true, true, true>(o, p, f32, s);
+  QuantJob jobs[2] = {};
+  int n = 0;
+  if (!x_codes && M > 0 && K > 0) {
+    x_code_stride = up16(K);
+    x_codes = workspace;
+    x_scales = static_cast<uint8_t*>(workspace) + up256(M * x_code_stride);
+    jobs[n++] = quant_job(x, M, K, x_stride, kQuantRows, const_cast<void*>(x_codes), const_cast<void*>(x_scales), nullptr, nullptr, x_code_stride);
+  }
+  if (w && K > 0) jobs[n++] = quant_job(w, N, K, w_stride, kQuantTiles, w_codes, w_scales, nullptr, nullptr, w_code_stride);
+  if (n > 0)
+    if (const cudaError_t e = launch_quant(jobs[0], jobs[1], s)) return (int)e;
+  if (M == 0) return 0;
+  return (int)product(w_blocks == FLAME_FP8_BLOCKS_TILES ? Product::kNtTiles : Product::kNtRows, x_codes, x_code_stride, x_scales, w_codes, w_code_stride, w_scales, y, N,
+                      false, M, N, K, s);
+}
+
+int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, size_t x_stride, const void* w_codes, size_t w_code_stride,
+                              const void* w_scales, void* dx, void* dw, size_t M, size_t N, size_t K, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  const char* who = "flame_fp8_linear_backward";
+  if (const char* what = quant_source(dy, M, N, dy_stride)) return refuse(who, what);
+  if (dw)
+    if (const char* what = quant_source(x, M, K, x_stride)) return refuse(who, what);
+  if (K > kMostSize) return refuse(who, "matrix too large");
+  if (dx && (w_code_stride < K || w_code_stride % 16 != 0)) return refuse(who, "a code stride is smaller than the row, or no multiple of 16");
+  if ((!dx && !dw) || K == 0) return 0;
+  if (dx && M > 0 && N > 0 && (!w_codes || !w_scales)) return refuse(who, "null tensor");
+  if (!al(dx, 2) || !al(dw, 2) || !al(w_codes, 16) || !al(w_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
+  if (M > 0 && N > 0 && (!workspace || !al(workspace, 256) || workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, 1)))
+    return refuse(who, "workspace too small, or not on 256 bytes");
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  cudaStream_t s = (cudaStream_t)stream;
+  const size_t ldn = up16(N), ldk = up16(K);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  uint8_t *rows = at, *cols = at + codes_bytes(M, N, kQuantRows), *xcols = cols + codes_bytes(M, N, kQuantColumns);
+  uint8_t *row_scales = rows + up256(M * ldn), *col_scales = cols + up256(M * ldn), *xcol_scales = xcols + up256(M * ldk);
+  if (M > 0 && N > 0) {
+    const QuantJob a = quant_job(dy, M, N, dy_stride, (dx ? kQuantRows : 0u) | (dw ? kQuantColumns : 0u), rows, row_scales, cols, col_scales, ldn);
+    const QuantJob b = dw ? quant_job(x, M, K, x_stride, kQuantColumns, nullptr, nullptr, xcols, xcol_scales, ldk) : QuantJob{};
+    if (const cudaError_t e = launch_quant(a, b, s)) return (int)e;
+  }
+  if (dx && M > 0)
+    if (const cudaError_t e = product(Product::kNnTiles, rows, ldn, row_scales, w_codes, w_code_stride, w_scales, dx, K, false, M, K, N, s)) return (int)e;
+  if (dw && N > 0) return (int)product(Product::kTnColumns, cols, ldn, col_scales, xcols, ldk, xcol_scales, dw, K, false, N, K, M, s);
+  return 0;
 }
 
 int flame_fp8_product_faults(unsigned int* count) {

@@ -18,10 +18,9 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _op
-from ._op import need
+from .errors import InvalidInput
 
 
 def _launch(x, residual, p, seed, offset):
@@ -40,8 +39,7 @@ class _Dropout(torch.autograd.Function):
         ctx.save_for_backward(*((seed,) if ctx.seed is None else ()))
         return _launch(x, residual, p, seed, offset)
 
-    @staticmethod
-    @once_differentiable
+    @_op.first_order
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
@@ -56,16 +54,22 @@ def dropout(x: torch.Tensor, p: float, *, seed: Union[int, torch.Tensor], offset
 
     ``p`` is exact to 2^-32.  A dropped element is 0 whatever it was, infinities and NaN included."""
     _op.on_gpu("dropout", x, residual)
-    need(x.dtype in _op.DTYPE, "dropout: BF16 or F32 tensors")
-    need(x.is_contiguous(), "dropout: x must be contiguous")
-    need(0.0 <= float(p) <= 1.0, f"dropout: p must be in [0, 1], got {p}")
-    need(isinstance(offset, int) and 0 <= offset < 1 << 64, "dropout: offset must be an integer in [0, 2^64)")
+    if x.dtype not in _op.DTYPE:
+        raise InvalidInput("dropout: BF16 or F32 tensors")
+    if not x.is_contiguous():
+        raise InvalidInput("dropout: x must be contiguous")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise InvalidInput(f"dropout: p must be in [0, 1], got {p}")
+    if not (isinstance(offset, int) and 0 <= offset < 1 << 64):
+        raise InvalidInput("dropout: offset must be an integer in [0, 2^64)")
     if isinstance(seed, torch.Tensor):
-        need(seed.device == x.device and seed.dtype == torch.int64 and seed.numel() == 1,
-             "dropout: a seed tensor holds one int64 on the device of x")
-    else:
-        need(isinstance(seed, int) and 0 <= seed < 1 << 64, "dropout: seed must be an integer in [0, 2^64) or a tensor")
-    if residual is not None:
-        need(residual.dtype == x.dtype and residual.shape == x.shape and residual.is_contiguous(),
-             "dropout: residual must be contiguous, with the type and shape of x")
-    return _Dropout.apply(x, residual, float(p), seed, offset)
+        if not (seed.device == x.device and seed.dtype == torch.int64 and seed.numel() == 1):
+            raise InvalidInput("dropout: a seed tensor holds one int64 on the device of x")
+    elif not (isinstance(seed, int) and 0 <= seed < 1 << 64):
+        raise InvalidInput("dropout: seed must be an integer in [0, 2^64) or a tensor")
+    if residual is not None and not (residual.dtype == x.dtype and residual.shape == x.shape and residual.is_contiguous()):
+        raise InvalidInput("dropout: residual must be contiguous, with the type and shape of x")
+    if not _op.recorded(x, residual):
+        return _launch(x, residual, p, seed, offset)
+    return _Dropout.apply(x, residual, p, seed, offset)

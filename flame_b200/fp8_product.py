@@ -13,15 +13,13 @@ operands: there code 0x7F stands for 480.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _op
-from ._op import need
-from .errors import InvalidShape, Unsupported
+from .errors import InvalidInput, InvalidShape, Unsupported
 
 BLOCK = 128
 _BLOCKS = {"rows": 1, "columns": 2, "tiles": 3}     # FLAME_FP8_BLOCKS_*
@@ -35,40 +33,39 @@ def _scales_shape(rows: int, cols: int, blocks: str) -> Tuple[int, int]:
     return (rows if blocks == "rows" else _blocks_of(rows), cols if blocks == "columns" else _blocks_of(cols))
 
 
-@dataclass(frozen=True)
+def _padded(cols: int) -> int:
+    return max(16, (cols + 15) // 16 * 16)
+
+
 class Fp8Blocks:
     """An FP8 matrix: uint8 ``codes`` [rows, cols] whose rows start 16 bytes or a multiple of it apart, and fp32 ``scales``:
     [rows, ceil(cols/128)] for "rows", [ceil(rows/128), cols] for "columns", [ceil(rows/128), ceil(cols/128)] for "tiles"."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    blocks: str
+    __slots__ = ("codes", "scales", "blocks", "shape", "stride")
 
-    def __post_init__(self):
-        need(self.blocks in _BLOCKS, f"Fp8Blocks: blocks must be one of {', '.join(_BLOCKS)}")
-        c, s = self.codes, self.scales
-        _op.on_gpu("Fp8Blocks", c, s)
-        need(c.dtype == torch.uint8 and c.dim() == 2 and s.dtype == torch.float32 and s.is_contiguous(),
-             "Fp8Blocks: uint8 codes [rows, cols] and contiguous float32 scales")
-        need(tuple(s.shape) == _scales_shape(c.shape[0], c.shape[1], self.blocks),
-             f"Fp8Blocks: scales {tuple(s.shape)} for codes {tuple(c.shape)}, expected {_scales_shape(c.shape[0], c.shape[1], self.blocks)}", InvalidShape)
-        if c.numel():
-            need((c.stride(1) == 1 or c.shape[1] == 1) and c.data_ptr() % 16 == 0, "Fp8Blocks: codes must be row-major and start on 16 bytes")
-            need(c.shape[0] == 1 or (c.stride(0) % 16 == 0 and c.stride(0) >= c.shape[1]), "Fp8Blocks: rows of codes must be a multiple of 16 bytes apart")
-
-    @property
-    def shape(self) -> Tuple[int, int]:
-        return tuple(self.codes.shape)
-
-    @property
-    def stride(self) -> int:
-        """Bytes from row to row.  A matrix of one row may be the start of longer memory: its stride is its own length."""
-        c = self.codes
-        return c.stride(0) if c.shape[0] > 1 and c.shape[1] else _padded(c.shape[1])
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, blocks: str):
+        if blocks not in _BLOCKS:
+            raise InvalidInput(f"Fp8Blocks: blocks must be one of {', '.join(_BLOCKS)}")
+        _op.on_gpu("Fp8Blocks", codes, scales)
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or scales.dtype != torch.float32 or not scales.is_contiguous():
+            raise InvalidInput("Fp8Blocks: uint8 codes [rows, cols] and contiguous float32 scales")
+        rows, cols = codes.shape
+        want = _scales_shape(rows, cols, blocks)
+        if scales.shape != want:
+            raise InvalidShape(f"Fp8Blocks: scales {tuple(scales.shape)} for codes {(rows, cols)}, expected {want}")
+        # a matrix of one row may be the start of longer memory: its stride is its own length
+        stride = codes.stride(0) if rows > 1 and cols else _padded(cols)
+        if rows and cols:
+            if (codes.stride(1) != 1 and cols != 1) or codes.data_ptr() % 16 != 0:
+                raise InvalidInput("Fp8Blocks: codes must be row-major and start on 16 bytes")
+            if stride % 16 != 0 or stride < cols:
+                raise InvalidInput("Fp8Blocks: rows of codes must be a multiple of 16 bytes apart")
+        self.codes, self.scales, self.blocks, self.shape, self.stride = codes, scales, blocks, (rows, cols), stride
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """code * scale as a new BF16 or F32 matrix."""
-        need(dtype in _op.DTYPE, "dequantize: BF16 or F32")
+        if dtype not in _op.DTYPE:
+            raise InvalidInput("dequantize: BF16 or F32")
         rows, cols = self.shape
         out = torch.empty(rows, cols, dtype=dtype, device=self.codes.device)
         _op.call("flame_fp8_dequant_2d", out.device, self.codes.data_ptr(), self.stride, self.scales.data_ptr(), _BLOCKS[self.blocks],
@@ -76,30 +73,31 @@ class Fp8Blocks:
         return out
 
 
-def _padded(cols: int) -> int:
-    return max(16, (cols + 15) // 16 * 16)
-
-
-def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x as a BF16 matrix with neighbouring columns, without a copy."""
-    need(x.dtype == torch.bfloat16 and x.dim() >= 1, f"{what}: BF16 tensors")
-    if x.dim() != 2:
-        need(x.is_contiguous(), f"{what}: a tensor of other than two dimensions must be contiguous")
-        x = x.view(_rows_of(x), x.shape[-1])
-    need(x.numel() == 0 or ((x.stride(1) == 1 or x.shape[1] == 1) and (x.shape[0] == 1 or x.stride(0) >= x.shape[1])),
-         f"{what}: the columns of a matrix must be neighbours, and its rows must not overlap")
-    return x
-
-
-def _rows_of(x: torch.Tensor) -> int:
+def _rows_of(shape) -> int:
     n = 1
-    for s in x.shape[:-1]:
+    for s in shape[:-1]:
         n *= s
     return n
 
 
-def _quantize(x, blocks: Optional[str], columns: bool):
-    rows, cols = x.shape
+def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int]:
+    """(rows, columns, elements from row to row) of a BF16 tensor read as a matrix of its last dimension."""
+    if x.dtype != torch.bfloat16 or x.dim() < 1:
+        raise InvalidInput(f"{what}: BF16 tensors of one dimension at least")
+    shape = x.shape
+    rows, cols = _rows_of(shape), shape[-1]
+    if x.is_contiguous():
+        return rows, cols, cols
+    if x.dim() != 2:
+        raise InvalidInput(f"{what}: a tensor of other than two dimensions must be contiguous")
+    if (x.stride(1) != 1 and cols != 1) or (rows != 1 and x.stride(0) < cols):
+        raise InvalidInput(f"{what}: the columns of a matrix must be neighbours, and its rows must not overlap")
+    return rows, cols, x.stride(0) if rows > 1 else cols
+
+
+def _quantize(x, what, blocks: Optional[str], columns: bool):
+    _op.on_gpu(what, x)
+    rows, cols, stride = _matrix(x, what)
     ld = _padded(cols)
 
     def make(kind):
@@ -108,7 +106,6 @@ def _quantize(x, blocks: Optional[str], columns: bool):
 
     c, s = make(blocks) if blocks else (None, None)
     cc, cs = make("columns") if columns else (None, None)
-    stride = x.stride(0) if rows > 1 else cols
     _op.call("flame_fp8_quant_2d", x.device, x.data_ptr(), rows, cols, stride, _op.ptr(c), _op.ptr(s), _BLOCKS[blocks] if blocks else 0,
              _op.ptr(cc), _op.ptr(cs), ld)
     out = []
@@ -121,16 +118,15 @@ def _quantize(x, blocks: Optional[str], columns: bool):
 
 def quantize_fp8(x: torch.Tensor, blocks: str = "rows") -> Fp8Blocks:
     """FP8 codes of a BF16 matrix (or of the rows of a contiguous tensor's last dimension)."""
-    _op.on_gpu("quantize_fp8", x)
-    need(blocks in _BLOCKS, f"quantize_fp8: blocks must be one of {', '.join(_BLOCKS)}")
-    x = _matrix(x, "quantize_fp8")
-    return _quantize(x, None, True)[0] if blocks == "columns" else _quantize(x, blocks, False)[0]
+    if blocks not in _BLOCKS:
+        raise InvalidInput(f"quantize_fp8: blocks must be one of {', '.join(_BLOCKS)}")
+    columns = blocks == "columns"
+    return _quantize(x, "quantize_fp8", None if columns else blocks, columns)[0]
 
 
 def quantize_fp8_both(x: torch.Tensor) -> Tuple[Fp8Blocks, Fp8Blocks]:
-    """``quantize_fp8(x, "rows")`` and ``quantize_fp8(x, "columns")`` from one read of x: what backward needs of an output gradient."""
-    _op.on_gpu("quantize_fp8_both", x)
-    rows, columns = _quantize(_matrix(x, "quantize_fp8_both"), "rows", True)
+    """``quantize_fp8(x, "rows")`` and ``quantize_fp8(x, "columns")`` from one read of x."""
+    rows, columns = _quantize(x, "quantize_fp8_both", "rows", True)
     return rows, columns
 
 
@@ -141,8 +137,10 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, transpose_b: bool = False, dtype: 
     * a "rows" [M, K], b "tiles" [K, N]:                                 a b
     * a "columns" [K, M], b "columns" [K, N]:                            a^T b
     """
-    need(isinstance(a, Fp8Blocks) and isinstance(b, Fp8Blocks), "fp8_matmul: Fp8Blocks operands")
-    need(dtype in _op.DTYPE, "fp8_matmul: the result is BF16 or F32")
+    if not (isinstance(a, Fp8Blocks) and isinstance(b, Fp8Blocks)):
+        raise InvalidInput("fp8_matmul: Fp8Blocks operands")
+    if dtype not in _op.DTYPE:
+        raise InvalidInput("fp8_matmul: the result is BF16 or F32")
     device = _op.on_gpu("fp8_matmul", a.codes, b.codes)
     kinds = (a.blocks, b.blocks, bool(transpose_b))
     if kinds in (("rows", "rows", True), ("rows", "tiles", True)):
@@ -154,38 +152,69 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, transpose_b: bool = False, dtype: 
     else:
         raise Unsupported(f"fp8_matmul: no product of {a.blocks} and {b.blocks}{' transposed' if transpose_b else ''}: "
                           "the blocks must run along the contraction")
-    need(k == kb, f"fp8_matmul: shapes {a.shape} and {b.shape} do not fit", InvalidShape)
+    if k != kb:
+        raise InvalidShape(f"fp8_matmul: shapes {a.shape} and {b.shape} do not fit")
     c = torch.empty(m, n, dtype=dtype, device=device)
     _op.call("flame_fp8_product", device, a.codes.data_ptr(), a.stride, a.scales.data_ptr(), _BLOCKS[a.blocks], b.codes.data_ptr(), b.stride,
              b.scales.data_ptr(), _BLOCKS[b.blocks], int(bool(transpose_b)), c.data_ptr(), n, _op.DTYPE[dtype], m, n, k)
     return c
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(m: int, n: int, k: int, backward: int) -> int:
+    return max(_op.function("flame_fp8_linear_workspace_bytes")(m, n, k, backward), 16)
+
+
+def _forward(x, codes: Optional[Fp8Blocks], weight, frozen: Optional[Fp8Blocks]):
+    """(y, codes of the weight, their scales): one call of the library; a BF16 weight is quantised in it."""
+    device = x.device
+    m, k, x_stride = _matrix(x, "fp8_linear")
+    if frozen is not None:
+        n, blocks, w_codes, w_scales, ld, w_stride = frozen.shape[0], _BLOCKS[frozen.blocks], frozen.codes, frozen.scales, frozen.stride, 0
+    else:
+        n, _, w_stride = _matrix(weight, "fp8_linear")
+        blocks, ld = 3, _padded(k)
+        w_codes = torch.empty(n, ld, dtype=torch.uint8, device=device)
+        w_scales = torch.empty(_blocks_of(n), _blocks_of(k), dtype=torch.float32, device=device)
+    y = torch.empty(x.shape[:-1] + (n,), dtype=torch.bfloat16, device=device)
+    if codes is None:
+        size = _workspace_bytes(m, n, k, 0)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        given = (None, 0, None)
+    else:
+        ws, size, given = None, 0, (codes.codes.data_ptr(), codes.stride, codes.scales.data_ptr())
+    _op.call("flame_fp8_linear", device, x.data_ptr(), x_stride, *given, _op.ptr(weight), w_stride, w_codes.data_ptr(), ld, w_scales.data_ptr(),
+             blocks, y.data_ptr(), m, n, k, _op.ptr(ws), size)
+    return y, w_codes, w_scales
+
+
 class _Linear(torch.autograd.Function):
     """y = x w^T.  Saved for backward: x where the weight is trained (BF16, so that a pool can offload it), and the weight's codes."""
 
     @staticmethod
-    def forward(ctx, x, weight, x_codes, x_scales, w_codes, w_scales, w_blocks):
-        m = _matrix(x, "fp8_linear")
-        qx = Fp8Blocks(x_codes, x_scales, "rows") if x_codes is not None else _quantize(m, "rows", False)[0]
-        qw = Fp8Blocks(w_codes, w_scales, w_blocks) if w_codes is not None else _quantize(_matrix(weight, "fp8_linear"), "tiles", False)[0]
-        y = fp8_matmul(qx, qw, transpose_b=True)
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None,
-                              *((qw.codes, qw.scales) if ctx.needs_input_grad[0] else (None, None)))
-        ctx.shapes = (x.shape, qw.shape)
-        return y.view(*x.shape[:-1], qw.shape[0])
+    def forward(ctx, x, weight, codes, frozen):
+        y, w_codes, w_scales = _forward(x, codes, weight, frozen)
+        want_dx = ctx.needs_input_grad[0]
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w_codes if want_dx else None, w_scales if want_dx else None)
+        ctx.ld = frozen.stride if frozen is not None else w_codes.shape[1]
+        ctx.x_shape, ctx.n = x.shape, y.shape[-1]
+        return y
 
-    @staticmethod
-    @once_differentiable
+    @_op.first_order
     def backward(ctx, dy):
         x, w_codes, w_scales = ctx.saved_tensors
-        x_shape, (n, k) = ctx.shapes
-        dy = dy.contiguous().view(_rows_of(dy), n)
         want_dx, want_dw = ctx.needs_input_grad[:2]
-        q = _quantize(dy, "rows" if want_dx else None, want_dw)
-        dx = fp8_matmul(q[0], Fp8Blocks(w_codes, w_scales, "tiles")).view(x_shape) if want_dx else None
-        dw = fp8_matmul(q[-1], _quantize(_matrix(x, "fp8_linear"), None, True)[0]) if want_dw else None
-        return dx, dw, None, None, None, None, None
+        shape, n = ctx.x_shape, ctx.n
+        device = dy.device
+        dy = dy.contiguous()
+        m, k = _rows_of(shape), shape[-1]
+        dx = torch.empty(shape, dtype=torch.bfloat16, device=device) if want_dx else None
+        dw = torch.empty(n, k, dtype=torch.bfloat16, device=device) if want_dw else None
+        size = _workspace_bytes(m, n, k, 1)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        _op.call("flame_fp8_linear_backward", device, dy.data_ptr(), n, _op.ptr(x), _matrix(x, "fp8_linear")[2] if want_dw else 0,
+                 _op.ptr(w_codes), ctx.ld, _op.ptr(w_scales), _op.ptr(dx), _op.ptr(dw), m, n, k, ws.data_ptr(), size)
+        return dx, dw, None, None
 
 
 def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], *, codes: Optional[Fp8Blocks] = None) -> torch.Tensor:
@@ -193,19 +222,21 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], *, codes
 
     ``weight`` as ``Fp8Blocks`` is frozen ("tiles", or "rows" where x needs no gradient); as a BF16 tensor it is quantised in the call and
     receives a gradient.  ``codes``: the "rows" codes of x where a producer has written them already (``group_norm_fp8``)."""
-    frozen = isinstance(weight, Fp8Blocks)
-    w = weight.codes if frozen else weight
+    frozen = weight if isinstance(weight, Fp8Blocks) else None
+    w = weight if frozen is None else frozen.codes
     _op.on_gpu("fp8_linear", x, w, codes.codes if codes is not None else None)
-    if not frozen:
-        need(weight.dtype == torch.bfloat16, "fp8_linear: the weight is a BF16 matrix or Fp8Blocks")
-    need(w.dim() == 2, "fp8_linear: the weight is a matrix [N, K]")
-    need(x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] == w.shape[1],
-         f"fp8_linear: x {tuple(x.shape)} and weight {tuple(w.shape)} do not fit", InvalidShape)
-    if frozen:
-        need(weight.blocks != "columns", "fp8_linear: the blocks of a weight are tiles or rows", Unsupported)
-        need(weight.blocks == "tiles" or not (torch.is_grad_enabled() and x.requires_grad),
-             "fp8_linear: a weight with rows of blocks has no input gradient; quantise it to tiles", Unsupported)
-    if codes is not None:
-        need(codes.blocks == "rows" and codes.shape == (_rows_of(x), x.shape[-1]), "fp8_linear: codes must be the rows of x", InvalidShape)
-    return _Linear.apply(x, None if frozen else weight, codes.codes if codes is not None else None, codes.scales if codes is not None else None,
-                         weight.codes if frozen else None, weight.scales if frozen else None, weight.blocks if frozen else None)
+    if frozen is None and (weight.dtype != torch.bfloat16 or weight.dim() != 2):
+        raise InvalidInput("fp8_linear: the weight is a BF16 matrix [N, K] or Fp8Blocks")
+    if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise InvalidShape(f"fp8_linear: x {x.dtype} {tuple(x.shape)} and weight {tuple(w.shape)} do not fit")
+    if codes is not None and (codes.blocks != "rows" or codes.shape != (_rows_of(x.shape), x.shape[-1])):
+        raise InvalidShape("fp8_linear: codes must be the rows of x")
+    record = _op.recorded(x, None if frozen is not None else weight)
+    if frozen is not None and frozen.blocks != "tiles":
+        if frozen.blocks == "columns":
+            raise Unsupported("fp8_linear: the blocks of a weight are tiles or rows")
+        if record:
+            raise Unsupported("fp8_linear: a weight with rows of blocks has no input gradient; quantise it to tiles")
+    if not record:
+        return _forward(x, codes, None if frozen is not None else weight, frozen)[0]
+    return _Linear.apply(x, None if frozen is not None else weight, codes, frozen)
