@@ -208,13 +208,13 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 }
 
 // ---- product ------------------------------------------------------------------------
-// One pass over the contraction in blocks of 128.  Roles of a thread block (20 warps):
-//   warps 0-15  epilogue: per block of the contraction they read the tensor cores' sums from tensor memory (32 rows x a quarter of the
-//               columns a warp, a thread is a row) and add them to fp32 registers with the block's scales;
-//   warp 16     copies tiles of both operands to shared memory (TMA, 128-byte swizzle, out-of-range elements are zeros);
-//   warps 17, 18 issue tcgen05.mma kind::f8f6f4, four of them (32 deep each) for a block of 128; each has an accumulator of its own and
+// One pass over the contraction in blocks of 128.  Roles of a thread block (12 warps):
+//   warps 0-7   epilogue: per block of the contraction they read the tensor cores' sums from tensor memory (32 rows x half of the
+//               columns a warp) and add them to fp32 registers with the block's scales;
+//   warp 8      copies tiles of both operands to shared memory (TMA, 128-byte swizzle, out-of-range elements are zeros);
+//   warps 9, 10 issue tcgen05.mma kind::f8f6f4, four of them (32 deep each) for a block of 128; each has an accumulator of its own and
 //               takes every other block, so that one's waits pass while the other's products run;
-//   warp 19     copies the blocks' scales to a ring in shared memory (asynchronous 4-byte copies, three blocks ahead).
+//   warp 11     copies the blocks' scales to a ring in shared memory (asynchronous 4-byte copies, three blocks ahead).
 // Operands lie in shared memory as they lie in global memory: along the contraction (K-major) or along the rows of C (MN-major,
 // the weight of the input gradient and both operands of the weight gradient), which the matrix descriptor says; nothing is
 // transposed.  A block's sum is scaled by one fused multiply-add a number, which is why each block needs an accumulator of its own
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 //
 // Every wait gives up after two seconds: the kernel then counts the fault (flame_fp8_product_faults), leaves its copies time to land
 // and returns its tensor memory.
-constexpr int kEpiWarps = 16;
+constexpr int kEpiWarps = 8;
 constexpr int kProductThreads = 32 * (kEpiWarps + 4);
 constexpr int kTileM = 128;                     // rows of a thread block
 constexpr int kStages = 6;
@@ -246,6 +246,7 @@ struct ProductArgs {
   uint32_t sa_stride, sb_stride;   // floats between rows of the scale arrays
   uint32_t tiles_m, tiles_n, blocks_k;
   uint32_t wide;                   // rows of C start on 32 bytes
+  uint32_t wide_sa, wide_sb;       // scales that lie along M or N: rows of them start on 16 bytes
 };
 
 struct ProductSmem {
@@ -332,18 +333,52 @@ __device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool live)
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4u : 0u) : "memory");
 }
 
-// The wait belongs to the same statement: nothing else tells the compiler that the registers are not there before it.
-__device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-               "tcgen05.wait::ld.sync.aligned;"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-                 "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-               : "r"(addr) : "memory");
+// 16 numbers of each lane, there when tmem_wait() has returned.  With a scale for 128 columns a thread takes 16 columns of one row.  With
+// a scale for each column it takes the layout of 16 x 8 fragments, columns 2 (lane % 4), + 1 of rows lane / 4, + 8 in each of four
+// fragments: a thread then needs the scales of a quarter of the columns, and reading them for every lane took as long as the products
+// (128 bytes a cycle come from shared memory, whether or not the lanes ask for the same).
+template <bool kFragments>
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
+  if constexpr (kFragments)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+  else
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+}
+// The loads issued so far are done.  What uses them is volatile like this and like the loads, so that the three stay in order.
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+// acc += {lo, hi} * s, two numbers at a time
+__device__ __forceinline__ void add_scaled(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
+  asm volatile("{ .reg .b64 x; mov.b64 x, {%1, %2}; fma.rn.f32x2 %0, x, %3, %0; }" : "+l"(acc) : "r"(lo), "r"(hi), "l"(s));
+}
+// The eight pairs of four fragments: acc += (pair * scales of its columns) * scale of its row.  The products of four pairs come
+// before the sums, so that none waits for the one before it.
+__device__ __forceinline__ void add_scaled_fragments(uint64_t* acc, const uint32_t (&x)[16], const uint64_t (&t)[4], uint64_t s_up, uint64_t s_down) {
+#pragma unroll
+  for (int f = 0; f < 4; f += 2)
+    asm volatile("{ .reg .b64 a, b, c, d; mov.b64 a, {%4, %5}; mov.b64 b, {%6, %7}; mov.b64 c, {%8, %9}; mov.b64 d, {%10, %11};\n\t"
+                 "mul.rn.f32x2 a, a, %12; mul.rn.f32x2 b, b, %12; mul.rn.f32x2 c, c, %13; mul.rn.f32x2 d, d, %13;\n\t"
+                 "fma.rn.f32x2 %0, a, %14, %0; fma.rn.f32x2 %1, b, %15, %1; fma.rn.f32x2 %2, c, %14, %2; fma.rn.f32x2 %3, d, %15, %3; }"
+                 : "+l"(acc[2 * f]), "+l"(acc[2 * f + 1]), "+l"(acc[2 * f + 2]), "+l"(acc[2 * f + 3])
+                 : "r"(x[4 * f]), "r"(x[4 * f + 1]), "r"(x[4 * f + 2]), "r"(x[4 * f + 3]), "r"(x[4 * f + 4]), "r"(x[4 * f + 5]), "r"(x[4 * f + 6]), "r"(x[4 * f + 7]),
+                   "l"(t[f]), "l"(t[f + 1]), "l"(s_up), "l"(s_down));
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void copy16(uint32_t dst, const float* src, uint32_t bytes) {   // the first `bytes` of 16, then zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync_all() {
@@ -385,7 +420,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   using S = ProductSmem;
   constexpr int kN = kPair ? 256 : 128;                          // columns of the tile
   constexpr int kRows = kPair ? 256 : 128;                       // rows of the tile
-  constexpr int kCols = kN / 4;                                  // columns of an epilogue warp
+  constexpr int kCols = kN / (kEpiWarps / 4);                                  // columns of an epilogue warp
   constexpr uint32_t kTmemCols = 2 * kN;
   // D fp32, A and B e4m3, major-ness, N / 8, M / 16
   constexpr uint32_t kIdesc = (1u << 4) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) | ((uint32_t)(kN / 8) << 17) | ((uint32_t)(kRows / 16) << 24);
@@ -431,10 +466,10 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const uint32_t tmem = *tmem_slot;
   pdl_prologue();
 
-  // The epilogue's sums need more registers than an equal share: 640 threads start with 96 each, 61,440 together; four warps go down
-  // to 32 and sixteen up to 112, 61,440 again.
+  // The epilogue's sums need more registers than an equal share: 384 threads start with 168 each, 64,512 together; four warps go down
+  // to 88 and eight up to 208, 64,512 again.
   if (warp < kEpiWarps) {
-    if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t quarter = warp & 3, col_off = (warp >> 2) * kCols;
     const uint32_t row = quarter * 32 + lane;
     const uint32_t release = at_rank(acc_empty(0), kPair ? 0 : rank);
@@ -445,35 +480,50 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       const uint32_t m0 = tm * kRows + row_off + quarter * 32;
       const uint32_t n0 = tn * kN + col_off;
       const bool live = m0 < p.M && n0 < p.N;
-      float acc[kCols];
+      uint64_t acc2[kCols / 2];
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < kCols / 2; ++i) acc2[i] = 0ull;
       for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t b = it & 1;
         ok = ok && bar_wait(acc_full(b), (it >> 1) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
         __syncwarp();
         tmem_fence_after();
         if (live) {
-          const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + it % kSlots * S::kScales);
           const uint32_t src = tmem + b * kN + col_off + (quarter << 21);   // lane 32 * quarter in the upper 16 bits
-          const float sa = kBvec ? sc[row] : sc[row] * sc[kTileM + col_off / kBlock];
+          uint32_t v[2][16];
+          // piece k: 16 columns of the thread's row, or 32 columns of the thread's four fragments in 16 of the warp's rows
+          auto piece = [&](int k) { return kBvec ? src + k / 2 * 32 + ((uint32_t)(k % 2) << 20) : src + k * 16; };
+          tmem_load16<kBvec>(v[0], piece(0));
+          const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + it % kSlots * S::kScales);
+          uint64_t sa2[kBvec ? 4 : 1];
+          if constexpr (kBvec) {
 #pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
-            uint32_t v[32];
-            tmem_load32(v, src + c);
-            if (c + 32 == kCols) {       // all is in registers: the accumulator is free for the block after the next
+            for (int i = 0; i < 4; ++i) { const uint32_t w = __float_as_uint(sc[quarter * 32 + i * 8 + lane / 4]); sa2[i] = pack2(w, w); }
+          } else {
+            const uint32_t w = __float_as_uint(sc[row] * sc[kTileM + col_off / kBlock]);
+            sa2[0] = pack2(w, w);
+          }
+          uint64_t sb[4];
+#pragma unroll
+          for (int k = 0; k < kCols / 16; ++k) {
+            uint32_t(&x)[16] = v[k % 2];
+            tmem_wait();
+            if (k + 1 < kCols / 16) {
+              tmem_load16<kBvec>(v[k % 2 ^ 1], piece(k + 1));
+            } else {       // all is in registers: the accumulator is free for the block after the next
               tmem_fence_before();
               __syncwarp();
               if (lane == 0) bar_arrive_cluster(release + 8 * b);
             }
+            if constexpr (kBvec) {
+              if (k % 2 == 0) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-              if (kBvec) w = *reinterpret_cast<const float4*>(sc + kTileM + col_off + c + i);
-              acc[c + i] = fmaf(kBvec ? __uint_as_float(v[i]) * w.x : __uint_as_float(v[i]), sa, acc[c + i]);
-              acc[c + i + 1] = fmaf(kBvec ? __uint_as_float(v[i + 1]) * w.y : __uint_as_float(v[i + 1]), sa, acc[c + i + 1]);
-              acc[c + i + 2] = fmaf(kBvec ? __uint_as_float(v[i + 2]) * w.z : __uint_as_float(v[i + 2]), sa, acc[c + i + 2]);
-              acc[c + i + 3] = fmaf(kBvec ? __uint_as_float(v[i + 3]) * w.w : __uint_as_float(v[i + 3]), sa, acc[c + i + 3]);
+                for (int f = 0; f < 4; ++f) sb[f] = *reinterpret_cast<const uint64_t*>(sc + kTileM + col_off + k / 2 * 32 + f * 8 + lane % 4 * 2);
+              }
+              add_scaled_fragments(acc2 + 8 * k, x, sb, sa2[k % 2 * 2], sa2[k % 2 * 2 + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) add_scaled(acc2[8 * k + i], x[2 * i], x[2 * i + 1], sa2[0]);
             }
           }
         } else if (lane == 0) {
@@ -486,37 +536,76 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const uint32_t rows = p.M - m0 < 32 ? p.M - m0 : 32;
         T* out = static_cast<T*>(p.c) + (size_t)m0 * p.c_stride + n0;
         uint8_t* st = smem + S::kOffStaging + warp * kStagingBytes;
+        const uint8_t* my_row = st + lane * kStagePitch;
 #pragma unroll
         for (int c = 0; c < kCols; c += kPer) {
+          if (n0 + c >= p.N) break;
+          const bool wide = p.wide && n0 + c + kPer <= p.N;
           uint32_t w[8];
+          if constexpr (kBvec) {
+            // fragments: two neighbouring columns of four rows
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = to_word<T>(acc + c + i * kPer / 8);
-          if (n0 + c >= p.N) {
-          } else if (p.wide && n0 + c + kPer <= p.N) {
+            for (int f = 0; f < kPer / 8; ++f)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int nb = c / 8 + f;          // fragment column of the warp, rows i * 8 + lane / 4
+                const float2 u = unpack2(acc2[(nb / 4 * 2 + i / 2) * 8 + nb % 4 * 2 + i % 2]);
+                uint8_t* at = st + (i * 8 + lane / 4) * kStagePitch + f * 8 * sizeof(T) + lane % 4 * 2 * sizeof(T);
+                const float pair[2] = {u.x, u.y};
+                *reinterpret_cast<uint32_t*>(at) = to_word<T>(pair);
+                if (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(at + 4) = __float_as_uint(u.y);
+              }
+            __syncwarp();
+            if (wide) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint32_t*>(my_row + 4 * i);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 u = unpack2(acc2[sizeof(T) == 2 ? c / 2 + i : (c + i) / 2]);
+              const float pair[2] = {sizeof(T) == 2 || i % 2 == 0 ? u.x : u.y, u.y};
+              w[i] = to_word<T>(pair);
+            }
+            if (!wide) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(st + lane * kStagePitch + 4 * i) = w[i];
+              __syncwarp();
+            }
+          }
+          if (wide) {
             // a whole sector of a row from each lane
             if (lane < rows)
               asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + (size_t)lane * p.c_stride + c), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
                            "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
           } else {
-            // rows that start anywhere: through shared memory, so that neighbouring lanes write neighbouring columns
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(st + lane * kStagePitch + 4 * i) = w[i];
-            __syncwarp();
+            // rows that start anywhere: neighbouring lanes write neighbouring columns
             const uint32_t cols = p.N - (n0 + c) < (uint32_t)kPer ? p.N - (n0 + c) : kPer, j = lane % kPer;
             if (j < cols)
               for (uint32_t r = lane / kPer; r < rows; r += 32 / kPer) out[(size_t)r * p.c_stride + c + j] = reinterpret_cast<const T*>(st + r * kStagePitch)[j];
-            __syncwarp();
           }
+          __syncwarp();
         }
       } else if (live) {
         // this block's share of the tile, over the pipeline's buffers: every copy has landed and every product has been read
-        float* mine = reinterpret_cast<float*>(smem) + (size_t)row * (kN + 4) + col_off;
+        float* mine = reinterpret_cast<float*>(smem) + (size_t)(quarter * 32) * (kN + 4) + col_off;
+        if constexpr (kBvec) {
 #pragma unroll
-        for (int i = 0; i < kCols; i += 4) *reinterpret_cast<float4*>(mine + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          for (int k = 0; k < kCols / 16; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float2*>(mine + (k % 2 * 16 + i % 2 * 8 + lane / 4) * (kN + 4) + k / 2 * 32 + i / 2 * 8 + lane % 4 * 2) = unpack2(acc2[8 * k + i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kCols / 2; i += 2) {
+            const float2 u = unpack2(acc2[i]), v = unpack2(acc2[i + 1]);
+            *reinterpret_cast<float4*>(mine + lane * (kN + 4) + 2 * i) = make_float4(u.x, u.y, v.x, v.y);
+          }
+        }
       }
     }
   } else {
-    if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == kEpiWarps) {
       if (lane == 0) {
         uint32_t it = 0;
@@ -563,25 +652,40 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       const float *pa = p.sa, *pb = p.sb;
       // from one row (column) of the tile to the 32nd after it, and from one block of the contraction to the next
       const size_t a32 = kAmn ? 32 : 32 * (size_t)p.sa_stride, b32 = kBmn ? 32 : 32 * (size_t)p.sb_stride;
+      const bool wide_a = kAmn && p.wide_sa, wide_b = kBvec && kBmn && p.wide_sb;
       auto copy_next = [&]() {
         if (kb_copy == kb1 && t_copy < tiles) {      // a new tile: this lane's first row and column of scales
           uint32_t tm, tn;
           tile_at(p, t_copy, tm, tn);
           t_copy += workers;
           kb_copy = kb0;
-          const uint32_t m = tm * kRows + row_off + lane, n = kBvec ? tn * kN + lane : tn * (kN / kBlock) + lane;
+          // the lane's first row (and column) of scales: every 32nd, or where they are neighbours in memory four together
+          const uint32_t la = wide_a ? 4 * lane : lane, lb = wide_b ? 4 * lane : lane;
+          const uint32_t m = tm * kRows + row_off + la, n = kBvec ? tn * kN + lb : tn * (kN / kBlock) + lb;
           const uint32_t n_end = kBvec ? p.N : (p.N + kBlock - 1) / kBlock;
-          a_left = m < p.M ? p.M - m : 0;            // the lane's rows are live while 32 * i < a_left
+          a_left = m < p.M ? p.M - m : 0;
           b_left = n < n_end ? n_end - n : 0;
           pa = p.sa + (a_left == 0 ? 0 : kAmn ? (size_t)kb0 * p.sa_stride + m : (size_t)m * p.sa_stride + kb0);
           pb = p.sb + (b_left == 0 ? 0 : kBmn ? (size_t)kb0 * p.sb_stride + n : (size_t)n * p.sb_stride + kb0);
         }
         if (kb_copy < kb1) {
+          if (wide_a) {
+            copy16(slot_at + lane * 16, pa, a_left < 4 ? a_left * 4 : 16);
+          } else {
 #pragma unroll
-          for (uint32_t i = 0; i < kTileM / 32; ++i) copy4(slot_at + (i * 32 + lane) * 4, i * 32 < a_left ? pa + i * a32 : p.sa, i * 32 < a_left);
+            for (uint32_t i = 0; i < kTileM / 32; ++i) copy4(slot_at + (i * 32 + lane) * 4, i * 32 < a_left ? pa + i * a32 : p.sa, i * 32 < a_left);
+          }
           if constexpr (kBvec) {
+            if (wide_b) {
 #pragma unroll
-            for (uint32_t i = 0; i < kN / 32; ++i) copy4(slot_at + (kTileM + i * 32 + lane) * 4, i * 32 < b_left ? pb + i * b32 : p.sb, i * 32 < b_left);
+              for (uint32_t i = 0; i < kN / 128; ++i) {
+                const uint32_t left = b_left > i * 128 ? b_left - i * 128 : 0;
+                copy16(slot_at + (kTileM + i * 128) * 4 + lane * 16, left ? pb + i * 128 : p.sb, left < 4 ? left * 4 : 16);
+              }
+            } else {
+#pragma unroll
+              for (uint32_t i = 0; i < kN / 32; ++i) copy4(slot_at + (kTileM + i * 32 + lane) * 4, i * 32 < b_left ? pb + i * b32 : p.sb, i * 32 < b_left);
+            }
           } else if (lane < kN / kBlock) {
             copy4(slot_at + (kTileM + lane) * 4, b_left ? pb : p.sb, b_left != 0);
           }
@@ -720,6 +824,8 @@ cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stre
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   p.blocks_k = (p.K + kBlock - 1) / kBlock;
   p.wide = (reinterpret_cast<uintptr_t>(p.c) & 31u) == 0 && (p.c_stride * sizeof(T)) % 32 == 0;
+  p.wide_sa = kAmn && (reinterpret_cast<uintptr_t>(p.sa) & 15u) == 0 && p.sa_stride % 4 == 0;
+  p.wide_sb = kBmn && kBvec && (reinterpret_cast<uintptr_t>(p.sb) & 15u) == 0 && p.sb_stride % 4 == 0;
   const uint32_t pairs = (uint32_t)sms / 2;
   p.tiles_m = (p.M + 255) / 256;
   p.tiles_n = (p.N + 255) / 256;
