@@ -11,41 +11,47 @@
 
 namespace flame_b200 {
 
-struct Fp8Scale {
-  float scale, inv;
-  bool divide;
-};
-
-__device__ __forceinline__ Fp8Scale fp8_scale_of(float amax) {
-  Fp8Scale s;
-  s.scale = __fdiv_rn(amax, 448.0f);
-  s.inv = s.scale == 0.0f ? 0.0f : __frcp_rn(s.scale);   // also where amax / 448 underflows to 0 (amax under 2^-141): codes of zero
-  s.divide = s.inv > 3.0e38f;
-  return s;
+// max(|a|, |b|) of two packed BF16 pairs in one instruction; the sign bits of the result mean nothing.  A NaN operand is ignored.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// The larger of a packed pair of magnitudes as a binary32 number; NaN counts as zero.
+__device__ __forceinline__ float larger_of(uint32_t pair) {
+  return fmaxf(fmaxf(__uint_as_float((pair << 16) & 0x7FFF0000u), __uint_as_float(pair & 0x7FFF0000u)), 0.0f);
 }
 
-__device__ __forceinline__ float fp8_scaled(float x, const Fp8Scale& s) {
-  if (s.divide) return __fdiv_rn(x, s.scale);
-  return __fmul_rn(x, s.inv);
-}
+__device__ __forceinline__ float fp8_scale_of(float amax) { return __fdiv_rn(amax, 448.0f); }
+// The factor of the elements.  Infinite where they have to be divided by the scale; 0 for a scale of 0 (also where amax / 448
+// underflows, amax under 2^-141).
+__device__ __forceinline__ float fp8_factor_of(float scale) { return scale == 0.0f ? 0.0f : __frcp_rn(scale); }
+__device__ __forceinline__ bool fp8_divides(float factor) { return factor > 3.0e38f; }
 
 __device__ __forceinline__ uint32_t fp8_encode2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-
-// Eight elements of a block with absolute maximum amax.
-__device__ __forceinline__ uint2 fp8_encode8(const float (&x)[8], const Fp8Scale& s) {
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = fp8_encode2(fp8_scaled(x[2 * i], s), fp8_scaled(x[2 * i + 1], s));
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+__device__ __forceinline__ uint2 fp8_pack8(const float (&y)[8]) {
+  return make_uint2(fp8_encode2(y[0], y[1]) | (fp8_encode2(y[2], y[3]) << 16), fp8_encode2(y[4], y[5]) | (fp8_encode2(y[6], y[7]) << 16));
 }
-__device__ __forceinline__ uint2 fp8_encode8(const float (&x)[8], float amax, float& scale) {
-  const Fp8Scale s = fp8_scale_of(amax);
-  scale = s.scale;
-  return fp8_encode8(x, s);
+// Eight elements of one block.
+__device__ __forceinline__ uint2 fp8_encode8(const float (&x)[8], float scale, float factor) {
+  float y[8];
+  if (fp8_divides(factor)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[i], factor);
+  }
+  return fp8_pack8(y);
+}
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&f)[8]) {   // eight BF16 numbers
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
 }
 
 }  // namespace flame_b200

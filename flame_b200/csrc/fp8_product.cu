@@ -46,121 +46,118 @@ struct QuantJob {
 // Up to two matrices in a launch: a layer's input and weight, or its output gradient and input.
 struct QuantJobs { QuantJob job[2]; };
 
-__global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(const __grid_constant__ QuantJobs jobs) {
+__global__ void __launch_bounds__(kQuantThreads, 4) fp8_quant_kernel(const __grid_constant__ QuantJobs jobs) {
   pdl_prologue();
-  __shared__ float part[8][kBlock];
+  __shared__ uint32_t part[8][kBlock / 2];       // packed maxima of two columns
+  __shared__ __align__(16) float factors[kBlock];
+  __shared__ __align__(16) float scales[kBlock];
   const bool second = blockIdx.x >= jobs.job[0].tiles;
   const QuantJob& a = jobs.job[second];
   const uint32_t tile = blockIdx.x - (second ? jobs.job[0].tiles : 0);
-  const uint32_t tm = tile / a.tiles_across, tn = tile % a.tiles_across;
+  const uint32_t tm = tile / a.tiles_across, tn = tile - tm * a.tiles_across;
   const uint32_t t = threadIdx.x, lr = t >> 4, lc = t & 15;
-  const uint32_t col = tn * kBlock + lc * 8;
-  const bool wide = a.mode & kQuantWide;
+  const uint32_t row0 = tm * kBlock + lr, col = tn * kBlock + lc * 8;
   uint4 raw[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t row = tm * kBlock + lr + 16 * j;
-    raw[j] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < a.rows && col < a.cols) {
-      const __nv_bfloat16* src = a.x + (size_t)row * a.x_stride + col;
-      if (wide) {
-        raw[j] = *reinterpret_cast<const uint4*>(src);
-      } else {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
+  for (int j = 0; j < 8; ++j) raw[j] = make_uint4(0u, 0u, 0u, 0u);
+  if (col < a.cols) {
+    const __nv_bfloat16* src = a.x + (size_t)row0 * a.x_stride + col;
+    if (a.mode & kQuantWide) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (col + i < a.cols) w[i / 2] |= (uint32_t)__bfloat16_as_ushort(src[i]) << (16 * (i & 1));
-        raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int j = 0; j < 8; ++j)
+        if (row0 + 16 * j < a.rows) raw[j] = __ldcs(reinterpret_cast<const uint4*>(src + (size_t)(16 * j) * a.x_stride));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (row0 + 16 * j < a.rows) {
+          uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < a.cols) w[i / 2] |= (uint32_t)__bfloat16_as_ushort(src[(size_t)(16 * j) * a.x_stride + i]) << (16 * (i & 1));
+          raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
   }
-  auto unpack = [&](int j, float (&f)[8]) {
-    const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-  };
-  auto put = [&](uint8_t* codes, int j, const uint2& c) {
-    const uint32_t row = tm * kBlock + lr + 16 * j;
-    if (row < a.rows && col < a.cols) *reinterpret_cast<uint2*>(codes + (size_t)row * a.code_stride + col) = c;   // the row's padding gets zeros
+  auto put = [&](uint8_t* codes, int j, const uint2& c) {      // a row's padding gets zeros
+    if (row0 + 16 * j < a.rows && col < a.cols) *reinterpret_cast<uint2*>(codes + (size_t)(row0 + 16 * j) * a.code_stride + col) = c;
   };
   if (a.mode & kQuantRows) {
+    // 16 lanes hold a row.  Each lane takes the maximum of one of its eight rows to a scale and a factor, and the others ask it.
+    float mine = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float f[8], m = 0.0f;
-      unpack(j, f);
+      uint32_t m = max_abs2(max_abs2(raw[j].x, raw[j].y), max_abs2(raw[j].z, raw[j].w));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+      for (int d = 8; d > 0; d >>= 1) m = max_abs2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+      if ((lc & 7) == (uint32_t)j) mine = larger_of(m);
+    }
+    const float scale = fp8_scale_of(mine), factor = fp8_factor_of(scale);
+    if (lc < 8 && row0 + 16 * lc < a.rows) a.row_scales[(size_t)(row0 + 16 * lc) * a.tiles_across + tn] = scale;
 #pragma unroll
-      for (int d = 8; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-      float s;
-      put(a.row_codes, j, fp8_encode8(f, m, s));
-      const uint32_t row = tm * kBlock + lr + 16 * j;
-      if (lc == 0 && row < a.rows) a.row_scales[(size_t)row * a.tiles_across + tn] = s;
+    for (int j = 0; j < 8; ++j) {
+      const float fj = __shfl_sync(0xFFFFFFFFu, factor, j, 16), sj = __shfl_sync(0xFFFFFFFFu, scale, j, 16);
+      float f[8];
+      unpack8(raw[j], f);
+      put(a.row_codes, j, fp8_encode8(f, sj, fj));
     }
   }
-  if (a.mode & kQuantTiles) {
-    float tmax = 0.0f;
+  if (a.mode & (kQuantTiles | kQuantColumns)) {
+    uint32_t c[4] = {0u, 0u, 0u, 0u};     // packed maxima of this thread's eight columns over its eight rows, and its neighbour's
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f[8];
-      unpack(j, f);
+    for (int j = 0; j < 8; ++j) { c[0] = max_abs2(c[0], raw[j].x); c[1] = max_abs2(c[1], raw[j].y); c[2] = max_abs2(c[2], raw[j].z); c[3] = max_abs2(c[3], raw[j].w); }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) tmax = fmaxf(tmax, fabsf(f[i]));
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xFFFFFFFFu, tmax, d));
-    if ((t & 31) == 0) part[0][t >> 5] = tmax;
+    for (int i = 0; i < 4; ++i) c[i] = max_abs2(c[i], __shfl_xor_sync(0xFFFFFFFFu, c[i], 16));
+    if ((t & 16) == 0) *reinterpret_cast<uint4*>(&part[t >> 5][lc * 4]) = make_uint4(c[0], c[1], c[2], c[3]);
     __syncthreads();
+    if (t < 32) {      // a lane joins four columns
+      uint32_t u = part[0][2 * t], v = part[0][2 * t + 1];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) tmax = fmaxf(tmax, part[0][k]);
-    const Fp8Scale s = fp8_scale_of(tmax);
+      for (int k = 1; k < 8; ++k) { u = max_abs2(u, part[k][2 * t]); v = max_abs2(v, part[k][2 * t + 1]); }
+      float m[4];
+      if (a.mode & kQuantTiles) {
+        uint32_t w = max_abs2(u, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f[8];
-      unpack(j, f);
-      put(a.row_codes, j, fp8_encode8(f, s));
-    }
-    if (t == 0) a.row_scales[(size_t)tm * a.tiles_across + tn] = s.scale;
-  }
-  if (a.mode & kQuantColumns) {
-    float cmax[8];
+        for (int d = 16; d > 0; d >>= 1) w = max_abs2(w, __shfl_xor_sync(0xFFFFFFFFu, w, d));
+        m[0] = m[1] = m[2] = m[3] = larger_of(w);
+      } else {
+        m[0] = fmaxf(__uint_as_float((u << 16) & 0x7FFF0000u), 0.0f);      // NaN counts as zero
+        m[1] = fmaxf(__uint_as_float(u & 0x7FFF0000u), 0.0f);
+        m[2] = fmaxf(__uint_as_float((v << 16) & 0x7FFF0000u), 0.0f);
+        m[3] = fmaxf(__uint_as_float(v & 0x7FFF0000u), 0.0f);
+      }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cmax[i] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f[8];
-      unpack(j, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) cmax[i] = fmaxf(cmax[i], fabsf(f[i]));
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) cmax[i] = fmaxf(cmax[i], __shfl_xor_sync(0xFFFFFFFFu, cmax[i], 16));
-    if ((t & 16) == 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) part[t >> 5][lc * 8 + i] = cmax[i];
+      for (int i = 0; i < 4; ++i) { scales[4 * t + i] = fp8_scale_of(m[i]); factors[4 * t + i] = fp8_factor_of(scales[4 * t + i]); }
     }
     __syncthreads();
-    Fp8Scale s[8];
+    if (a.mode & kQuantTiles) {
+      const float scale = scales[0], factor = factors[0];
+      if (t == 0) a.row_scales[(size_t)tm * a.tiles_across + tn] = scale;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float m = part[0][lc * 8 + i];
+      for (int j = 0; j < 8; ++j) {
+        float f[8];
+        unpack8(raw[j], f);
+        put(a.row_codes, j, fp8_encode8(f, scale, factor));
+      }
+    } else {
+      if (t < kBlock && tn * kBlock + t < a.cols) a.col_scales[(size_t)tm * a.cols + tn * kBlock + t] = scales[t];
+      const float4 f0 = *reinterpret_cast<const float4*>(factors + lc * 8), f1 = *reinterpret_cast<const float4*>(factors + lc * 8 + 4);
+      const float fc[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+      bool divides = false;
 #pragma unroll
-      for (int k = 1; k < 8; ++k) m = fmaxf(m, part[k][lc * 8 + i]);
-      s[i] = fp8_scale_of(m);
-    }
-    if (lr == 0) {
+      for (int i = 0; i < 8; ++i) divides |= fp8_divides(fc[i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < a.cols) a.col_scales[(size_t)tm * a.cols + col + i] = s[i].scale;
-    }
+      for (int j = 0; j < 8; ++j) {
+        float f[8];
+        unpack8(raw[j], f);
+        if (divides) {
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) f[i] = fp8_divides(factors[lc * 8 + i]) ? __fdiv_rn(f[i], scales[lc * 8 + i]) : __fmul_rn(f[i], factors[lc * 8 + i]);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float f[8];
-      unpack(j, f);
-      uint32_t h[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = fp8_encode2(fp8_scaled(f[2 * i], s[2 * i]), fp8_scaled(f[2 * i + 1], s[2 * i + 1]));
-      put(a.col_codes, j, make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16)));
+          for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], fc[i]);
+        }
+        put(a.col_codes, j, fp8_pack8(f));
+      }
     }
   }
 }

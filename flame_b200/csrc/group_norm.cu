@@ -218,7 +218,8 @@ __device__ __forceinline__ uint2 encode_row_block(const float (&y)[8], float& sc
   for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));   // a NaN is ignored
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-  return fp8_encode8(y, amax, scale);
+  scale = fp8_scale_of(amax);
+  return fp8_encode8(y, scale, fp8_factor_of(scale));
 }
 
 template <int V, bool kCodes>
