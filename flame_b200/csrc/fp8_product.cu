@@ -209,13 +209,15 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 //   warps 0-7   epilogue: per block of the contraction they read the tensor cores' sums from tensor memory (32 rows x half of the
 //               columns a warp) and add them to fp32 registers with the block's scales;
 //   warp 8      copies tiles of both operands to shared memory (TMA, 128-byte swizzle, out-of-range elements are zeros);
-//   warps 9, 10 issue tcgen05.mma kind::f8f6f4, four of them (32 deep each) for a block of 128; each has an accumulator of its own and
-//               takes every other block, so that one's waits pass while the other's products run;
+//   warps 9, 10 issue tcgen05.mma kind::f8f6f4, four of them (32 deep each) for a block of 128; each takes every other block, so that
+//               one's waits pass while the other's products run;
 //   warp 11     copies the blocks' scales to a ring in shared memory (asynchronous 4-byte copies, three blocks ahead).
 // Operands lie in shared memory as they lie in global memory: along the contraction (K-major) or along the rows of C (MN-major,
 // the weight of the input gradient and both operands of the weight gradient), which the matrix descriptor says; nothing is
 // transposed.  A block's sum is scaled by one fused multiply-add a number, which is why each block needs an accumulator of its own
-// in tensor memory: two take turns, so that the tensor cores work on one while the other is read.
+// in tensor memory: they take turns, so that the tensor cores work on one while another is read.  The way from a product's end over
+// the epilogue to the accumulator's next use takes some 1,000 cycles, a block's product 256 to 512: four accumulators of 128 columns
+// hide it, two of 256 (all that tensor memory holds) nearly do.
 //
 // Two forms.  kPair, for many tiles: the two SMs of a pair work on one tile of 256 x 256 (cta_group::2), each holds half of either
 // operand, the leader issues the products for both.  Without it a block has a tile of 128 x 128, and where tiles are few (serving,
@@ -228,7 +230,7 @@ constexpr int kEpiWarps = 8;
 constexpr int kProductThreads = 32 * (kEpiWarps + 4);
 constexpr int kTileM = 128;                     // rows of a thread block
 constexpr int kStages = 6;
-constexpr int kSlots = 8;                       // blocks of scales in shared memory
+constexpr int kScaleBytes = 12 * 1024;          // the ring of scales: 8 blocks of a pair's tile, 12 of a single block's
 constexpr int kStagePitch = 36;                 // bytes from row to row of a warp's output staging: 32 and 4 against bank conflicts
 constexpr int kStagingBytes = 32 * kStagePitch;
 
@@ -248,9 +250,8 @@ struct ProductArgs {
 
 struct ProductSmem {
   static constexpr int kOperand = kTileM * kBlock, kStage = 2 * kOperand;   // 128 x 128 bytes of either operand
-  static constexpr int kScales = (kTileM + 256) * 4;                        // of one block of the contraction
   static constexpr int kOffScales = kStages * kStage;
-  static constexpr int kOffStaging = kOffScales + kSlots * kScales;
+  static constexpr int kOffStaging = kOffScales + kScaleBytes;
   static constexpr int kOffBars = kOffStaging + kEpiWarps * kStagingBytes;
   static constexpr int kBytes = kOffBars + 512 + 1024;                      // and room to start on 1024 bytes
 };
@@ -418,7 +419,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   constexpr int kN = kPair ? 256 : 128;                          // columns of the tile
   constexpr int kRows = kPair ? 256 : 128;                       // rows of the tile
   constexpr int kCols = kN / (kEpiWarps / 4);                                  // columns of an epilogue warp
-  constexpr uint32_t kTmemCols = 2 * kN;
+  constexpr uint32_t kTmemCols = 512, kAccs = kTmemCols / kN;
+  constexpr uint32_t kScales = (kTileM + kN) * 4, kSlots = kScaleBytes / kScales;   // scales of one block of the contraction
   // D fp32, A and B e4m3, major-ness, N / 8, M / 16
   constexpr uint32_t kIdesc = (1u << 4) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) | ((uint32_t)(kN / 8) << 17) | ((uint32_t)(kRows / 16) << 24);
   extern __shared__ uint8_t smem_raw[];
@@ -428,8 +430,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   auto full = [&](uint32_t s) { return bars + 8 * s; };
   auto empty = [&](uint32_t s) { return bars + 8 * (kStages + s); };
   auto acc_full = [&](uint32_t b) { return bars + 8 * (2 * kStages + b); };
-  auto acc_empty = [&](uint32_t b) { return bars + 8 * (2 * kStages + 2 + b); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffBars + 8 * (2 * kStages + 4));
+  auto acc_empty = [&](uint32_t b) { return bars + 8 * (2 * kStages + 4 + b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffBars + 8 * (2 * kStages + 8));
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t group = cluster_size(), rank = cluster_rank();  // a pair, or the blocks that share a tile's contraction
@@ -443,7 +445,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kStages; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
     // an accumulator is full when the products are done and the block's scales are there
-    for (uint32_t b = 0; b < 2; ++b) { bar_init(acc_full(b), 2); bar_init(acc_empty(b), kPair ? 2 * kEpiWarps : kEpiWarps); }
+    for (uint32_t b = 0; b < kAccs; ++b) { bar_init(acc_full(b), 2); bar_init(acc_empty(b), kPair ? 2 * kEpiWarps : kEpiWarps); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -481,8 +483,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) acc2[i] = 0ull;
       for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-        const uint32_t b = it & 1;
-        ok = ok && bar_wait(acc_full(b), (it >> 1) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
+        const uint32_t b = it % kAccs;
+        ok = ok && bar_wait(acc_full(b), (it / kAccs) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
         __syncwarp();
         tmem_fence_after();
         if (live) {
@@ -491,7 +493,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           // piece k: 16 columns of the thread's row, or 32 columns of the thread's four fragments in 16 of the warp's rows
           auto piece = [&](int k) { return kBvec ? src + k / 2 * 32 + ((uint32_t)(k % 2) << 20) : src + k * 16; };
           tmem_load16<kBvec>(v[0], piece(0));
-          const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + it % kSlots * S::kScales);
+          const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + it % kSlots * kScales);
           uint64_t sa2[kBvec ? 4 : 1];
           if constexpr (kBvec) {
 #pragma unroll
@@ -507,7 +509,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             tmem_wait();
             if (k + 1 < kCols / 16) {
               tmem_load16<kBvec>(v[k % 2 ^ 1], piece(k + 1));
-            } else {       // all is in registers: the accumulator is free for the block after the next
+            } else {       // all is in registers: the accumulator is free for a later block
               tmem_fence_before();
               __syncwarp();
               if (lane == 0) bar_arrive_cluster(release + 8 * b);
@@ -625,11 +627,10 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       }
     } else if (warp <= kEpiWarps + 2) {
       if (lane == 0 && (!kPair || rank == 0)) {
-        const uint32_t b = warp - (kEpiWarps + 1);     // the accumulator; this warp's blocks are b, b + 2, ...
         const uint32_t mine = tiles > worker ? (tiles - worker + workers - 1) / workers * (kb1 - kb0) : 0;   // of all the block's tiles
-        for (uint32_t it = b; it < mine; it += 2) {
-          const uint32_t s = it % kStages;
-          if (!(ok = ok && bar_wait(full(s), (it / kStages) & 1) && bar_wait(acc_empty(b), ((it >> 1) & 1) ^ 1))) continue;
+        for (uint32_t it = warp - (kEpiWarps + 1); it < mine; it += 2) {
+          const uint32_t s = it % kStages, b = it % kAccs;
+          if (!(ok = ok && bar_wait(full(s), (it / kStages) & 1) && bar_wait(acc_empty(b), ((it / kAccs) & 1) ^ 1))) continue;
           tmem_fence_after();
           const uint32_t sa = base + s * S::kStage, sb = sa + S::kOperand;
           // 32 deep a step: 32 bytes along a K-major row, 32 rows of 128 bytes of an MN-major tile
@@ -641,10 +642,11 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
       }
     } else {
-      // Copies run kAhead blocks ahead.  When block i - 2 has its products, every warp of the epilogue has given block i - 4's accumulator
-      // back, which it does after its last use of block i - 5's scales: their place in the ring is free for block i + 3's.
-      constexpr uint32_t kAhead = 3;
-      static_assert(kSlots == kAhead + 5, "the argument above");
+      // Copies run kAhead blocks ahead.  When block i - kAccs has its products, every warp of the epilogue has given the accumulator of
+      // block i - 2 kAccs back, which it does after its last use of the scales of the block before that: their place in the ring is
+      // free for block i + kSlots - 2 kAccs - 1's.
+      constexpr uint32_t kAhead = kSlots - 2 * kAccs - 1;
+      static_assert(kAhead == 3, "8 places for two accumulators, 12 for four");
       uint32_t t_copy = worker, kb_copy = kb1, slot_at = base + S::kOffScales, a_left = 0, b_left = 0;
       const float *pa = p.sa, *pb = p.sb;
       // from one row (column) of the tile to the 32nd after it, and from one block of the contraction to the next
@@ -690,15 +692,15 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           if (b_left) pb += kBmn ? p.sb_stride : 1;
           ++kb_copy;
         }
-        slot_at = slot_at + S::kScales == base + S::kOffScales + kSlots * S::kScales ? base + S::kOffScales : slot_at + S::kScales;
+        slot_at = slot_at + kScales == base + S::kOffScales + kSlots * kScales ? base + S::kOffScales : slot_at + kScales;
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       for (uint32_t i = 0; i < kAhead; ++i) copy_next();
       uint32_t it = 0;
       for (uint32_t t = worker; t < tiles; t += workers)
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t b = it & 1;
-          if (it >= 2) ok = ok && bar_wait(acc_full(b), ((it >> 1) & 1) ^ 1);
+          const uint32_t b = it % kAccs;
+          if (it >= kAccs) ok = ok && bar_wait(acc_full(b), ((it / kAccs) & 1) ^ 1);
           __syncwarp();
           copy_next();
           asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");   // block `it` has landed
@@ -823,15 +825,20 @@ cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stre
   p.wide = (reinterpret_cast<uintptr_t>(p.c) & 31u) == 0 && (p.c_stride * sizeof(T)) % 32 == 0;
   p.wide_sa = kAmn && (reinterpret_cast<uintptr_t>(p.sa) & 15u) == 0 && p.sa_stride % 4 == 0;
   p.wide_sb = kBmn && kBvec && (reinterpret_cast<uintptr_t>(p.sb) & 15u) == 0 && p.sb_stride % 4 == 0;
-  const uint32_t pairs = (uint32_t)sms / 2;
-  p.tiles_m = (p.M + 255) / 256;
-  p.tiles_n = (p.N + 255) / 256;
-  if ((uint64_t)p.tiles_m * p.tiles_n >= pairs) return launch_tiles<true, kAmn, kBmn, kBvec, T>(o, p, 2, 2 * pairs, stream);
+  // Which form: a round of pairs (256 x 256 tiles, one for two SMs) took 1.0 where a round of single blocks (128 x 128) took 0.635,
+  // measured at 4096^3, 2048^3 and 2304^3 (18.9 and 12.0 us a round at K = 4096); 128 blocks that share the contraction four
+  // at a time (one token, 2048 x 2048) 5.2 us, two at a time 6.0, none 7.5, eight 9.3: clusters of eight wait for a place.
+  const uint64_t pairs = (uint64_t)sms / 2, rounds_of_pairs = ((uint64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) + pairs - 1) / pairs;
   p.tiles_m = (p.M + 127) / 128;
   p.tiles_n = (p.N + 127) / 128;
-  const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+  const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n, rounds = (tiles + sms - 1) / sms;
   uint32_t splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= (uint64_t)sms && splits * 2 <= p.blocks_k) splits *= 2;
+  while (splits < 4 && tiles * splits * 2 <= (uint64_t)sms && splits * 2 <= p.blocks_k) splits *= 2;
+  if (splits == 1 && rounds_of_pairs * 1000 <= rounds * 635) {
+    p.tiles_m = (p.M + 255) / 256;
+    p.tiles_n = (p.N + 255) / 256;
+    return launch_tiles<true, kAmn, kBmn, kBvec, T>(o, p, 2, (uint32_t)(2 * pairs), stream);
+  }
   const uint32_t blocks = splits > 1 ? (uint32_t)tiles * splits : (uint32_t)(tiles < (uint64_t)sms ? tiles : (uint64_t)sms);
   return launch_tiles<false, kAmn, kBmn, kBvec, T>(o, p, splits, blocks, stream);
 }
