@@ -244,6 +244,7 @@ struct ProductArgs {
   uint32_t M, N, K;
   uint32_t sa_stride, sb_stride;   // floats between rows of the scale arrays
   uint32_t tiles_m, tiles_n, blocks_k;
+  uint32_t rows_a;                 // rows of A that a copy brings: fewer than 128 where C has fewer, a multiple of 8
   uint32_t wide;                   // rows of C start on 32 bytes
   uint32_t wide_sa, wide_sb;       // scales that lie along M or N: rows of them start on 16 bytes
 };
@@ -616,7 +617,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             const uint32_t s = it % kStages;
             if (!(ok = ok && bar_wait(empty(s), ((it / kStages) & 1) ^ 1))) continue;
             // the leader's barrier counts the bytes of both blocks
-            if (!kPair || rank == 0) bar_expect(full(s), kPair ? 2 * S::kStage : S::kStage);
+            if (!kPair || rank == 0) bar_expect(full(s), kPair ? 2 * S::kStage : S::kOperand + (kAmn ? S::kOperand : p.rows_a * kBlock));
             const uint32_t bar = kPair ? at_rank(full(s), 0) : full(s);
             const uint32_t sa = base + s * S::kStage, sb = sa + S::kOperand;
             const int32_t k = (int32_t)(kb * kBlock);
@@ -765,12 +766,12 @@ EncodeTiled encode_tiled() {
   }();
   return f;
 }
-// rows x cols bytes, `stride` bytes from row to row, copied as 128 x 128
-bool byte_matrix(CUtensorMap* map, const uint8_t* p, uint64_t rows, uint64_t cols, uint64_t stride) {
+// rows x cols bytes, `stride` bytes from row to row, copied as 128 columns x `high` rows
+bool byte_matrix(CUtensorMap* map, const uint8_t* p, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t high) {
   const EncodeTiled f = encode_tiled();
   if (!f) return false;
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride};
-  const cuuint32_t box[2] = {kBlock, kBlock}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {kBlock, high}, one[2] = {1, 1};
   return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -784,7 +785,8 @@ struct Operands {
 template <bool kPair, bool kAmn, bool kBmn, bool kBvec, typename T>
 cudaError_t launch_tiles(const Operands& o, const ProductArgs& p, uint32_t group, uint32_t blocks, cudaStream_t stream) {
   CUtensorMap map_a, map_b;
-  const bool ok = byte_matrix(&map_a, o.a, kAmn ? p.K : p.M, kAmn ? p.M : p.K, o.a_stride) && byte_matrix(&map_b, o.b, kBmn ? p.K : p.N, kBmn ? p.N : p.K, o.b_stride);
+  const bool ok = byte_matrix(&map_a, o.a, kAmn ? p.K : p.M, kAmn ? p.M : p.K, o.a_stride, kAmn ? kBlock : p.rows_a) &&
+                  byte_matrix(&map_b, o.b, kBmn ? p.K : p.N, kBmn ? p.N : p.K, o.b_stride, kBlock);
   if (!ok) return cudaErrorNotSupported;
   auto kern = fp8_product_kernel<kPair, kAmn, kBmn, kBvec, T>;
   static std::atomic<uint64_t> allowed{0};     // a bit for each device on which the kernel may use this much shared memory
@@ -823,6 +825,9 @@ cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stre
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   p.blocks_k = (p.K + kBlock - 1) / kBlock;
   p.wide = (reinterpret_cast<uintptr_t>(p.c) & 31u) == 0 && (p.c_stride * sizeof(T)) % 32 == 0;
+  // Rows of C that do not exist: what their rows of A hold in shared memory reaches no other row of C and is not stored, so a copy
+  // leaves them out (one token against 8192 x 8192: 18.3 -> 14.4 us; out-of-range rows of a copy are written as zeros and take time).
+  p.rows_a = p.M < (uint32_t)kTileM ? (p.M + 7) / 8 * 8 : kTileM;
   p.wide_sa = kAmn && (reinterpret_cast<uintptr_t>(p.sa) & 15u) == 0 && p.sa_stride % 4 == 0;
   p.wide_sb = kBmn && kBvec && (reinterpret_cast<uintptr_t>(p.sb) & 15u) == 0 && p.sb_stride % 4 == 0;
   // Which form: a round of pairs (256 x 256 tiles, one for two SMs) took 1.0 where a round of single blocks (128 x 128) took 0.635,
@@ -837,6 +842,7 @@ cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stre
   if (splits == 1 && rounds_of_pairs * 1000 <= rounds * 635) {
     p.tiles_m = (p.M + 255) / 256;
     p.tiles_n = (p.N + 255) / 256;
+    p.rows_a = kTileM;
     return launch_tiles<true, kAmn, kBmn, kBvec, T>(o, p, 2, (uint32_t)(2 * pairs), stream);
   }
   const uint32_t blocks = splits > 1 ? (uint32_t)tiles * splits : (uint32_t)(tiles < (uint64_t)sms ? tiles : (uint64_t)sms);
