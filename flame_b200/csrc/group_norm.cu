@@ -7,12 +7,13 @@
 //
 // Two launches each way: the first reduces, the second applies.  A thread owns V neighbouring channels and walks down the
 // positions of its chunk, so that a warp reads whole lines of the channels-last rows, and per-channel sums stay in registers.
-// Sums are kept about a shift, the channel's first element in the sample: x - shift is of the size of the spread and not of the
-// mean, so that sums of squares lose nothing when the mean is large against the spread.  A thread block turns its channel sums
-// into (count, mean, sum of squares about the mean) of each group and writes those; the second launch joins the chunks' triples
-// in a fixed order (T. Chan, G. Golub, R. LeVeque, 1983).  No atomics: the same inputs give the same bits.
+// The forward sums are kept about a shift, the group's first element in the sample: x - shift is of the size of the spread and not of
+// the mean, so that sums of squares lose nothing when the mean is large against the spread.  A cluster of thread blocks adds its sums
+// up through distributed shared memory, which leaves the second launch an eighth of them to read.  Everything is added in a fixed
+// order, without atomics: the same inputs give the same bits.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -26,6 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr uint32_t kCluster = 8;
 
 struct NormArgs {
   const __nv_bfloat16* x;
@@ -36,25 +38,37 @@ struct NormArgs {
   uint8_t* codes;                // forward, may be NULL: FP8 codes of y, a scale for 128 elements of a row
   float* code_scales;
   float* stats;                  // [B, G, 2]: mean, rstd
-  float* partial;                // forward: [B, parts, G, 3]; backward: [B, parts, G, 2]
-  float* channel_partial;        // backward: [B, chunks, C, 2]
+  float2* partial;               // [B, parts, G]: forward sums of x - shift and of its square, backward s1 and s2
+  float2* channel_partial;       // backward: [B, parts, C]: sums for dbias and dweight
   void* dweight;                 // backward, may be NULL
   void* dbias;
-  uint32_t B, C, G, cg;
+  uint32_t B, C, G, cg, by_cg;
   uint64_t L;
-  uint32_t chunks;               // per sample
+  uint32_t chunks;               // per sample and slab, a multiple of the cluster's blocks (the last ones may be empty)
+  uint32_t parts;                // clusters per sample: chunks / kCluster * slabs
   uint64_t rows_per_chunk;
   uint32_t slabs;                // channel slabs of one thread block's width
   uint32_t slab_vecs;            // V-wide channel vectors in a slab
   float eps;
   int silu, params_f32;
+  int stream;                    // x and y together are larger than the L2 cache
 };
 
 __device__ __forceinline__ float param(const void* p, int f32, uint32_t c, float none) {
   if (!p) return none;
   return f32 ? static_cast<const float*>(p)[c] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c]);
 }
-__device__ __forceinline__ float sigmoid(float h) { return __fdividef(1.0f, 1.0f + __expf(-h)); }
+// 1 / (1 + exp(-h)) on the special-function unit: a few units in the last place of binary32, far below the rounding to BF16.  The
+// flush-to-zero forms skip the scaling of sub-normal arguments, which 1 + exp(-h) and its reciprocal have no use for.
+__device__ __forceinline__ float sigmoid(float h) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h * -1.442695041f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+// The group of channel c: c / cg by a multiplication, exact for c and cg up to 65,536 (by_cg = ceil(2^32 / cg), 0 for cg = 1).
+// Eight divisions a thread took longer than the sums themselves at 64 x 64 positions.
+__device__ __forceinline__ uint32_t group_of(uint32_t c, uint32_t by_cg) { return by_cg ? __umulhi(c, by_cg) : c; }
 
 template <int V>
 struct Vec { __nv_bfloat16 v[V]; };
@@ -64,17 +78,84 @@ template <>
 struct alignas(4) Vec<2> { __nv_bfloat16 v[2]; };
 
 template <int V>
-__device__ __forceinline__ void load(const __nv_bfloat16* p, float (&f)[V]) {
-  const Vec<V> r = *reinterpret_cast<const Vec<V>*>(p);
+__device__ __forceinline__ void unpack(const Vec<V>& r, float (&f)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = __bfloat162float(r.v[i]);
 }
 template <int V>
-__device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[V]) {
+__device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[V], int stream) {
   Vec<V> r;
 #pragma unroll
   for (int i = 0; i < V; ++i) r.v[i] = __float2bfloat16_rn(f[i]);
+  if constexpr (V == 8) {
+    if (stream) { __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&r)); return; }
+  }
   *reinterpret_cast<Vec<V>*>(p) = r;
+}
+// Walks a thread down its rows: f(offset, vectors) for each, offset in elements from the thread's first row, kN tensors at a time;
+// kBack: from the last row to the first.  f(.., live = false) where another thread of the block still has a row and this one has none
+// (only with kWhole, for shuffles inside f).
+//
+// The rows ahead are on their way to shared memory as asynchronous copies, each thread's own in places of its own, so nothing waits
+// for another thread and nothing is held in registers: with one row in flight in registers the two passes over 1024 x 1024 x 128
+// took 72 and 174 us, with four, which left two blocks on an SM, 76 and 152.
+constexpr int kDepth = 8;
+template <int kN, int V, bool kBack, bool kWhole, typename F>
+__device__ __forceinline__ void walk(const __nv_bfloat16* const (&src)[kN], uint64_t rows, uint32_t lane_row, uint32_t row_step, uint32_t C, uint4* ring, F&& f) {
+  const uint32_t mine = rows > lane_row ? (uint32_t)((rows - lane_row + row_step - 1) / row_step) : 0;
+  const uint32_t most = kWhole ? (uint32_t)((rows + row_step - 1) / row_step) : mine;
+  const size_t step = (size_t)row_step * C;
+  if constexpr (V == 8) {
+    constexpr int kD = kDepth / kN;
+    auto place = [&](uint32_t n, int k) { return ring + ((n % kD) * kN + k) * kThreads + threadIdx.x; };
+    auto row_of = [&](uint32_t n) { return kBack ? most - 1 - n : n; };
+    auto issue = [&](uint32_t n) {
+      if (n < most && row_of(n) < mine) {
+#pragma unroll
+        for (int k = 0; k < kN; ++k)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(place(n, k))), "l"(src[k] + row_of(n) * step) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int n = 0; n < kD; ++n) issue(n);
+    for (uint32_t n = 0; n < most; ++n) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kD - 1) : "memory");
+      Vec<V> v[kN];
+      const bool live = row_of(n) < mine;
+      if (live) {
+#pragma unroll
+        for (int k = 0; k < kN; ++k) { const uint4 w = *place(n, k); v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
+      }
+      f(row_of(n) * step, v, live);
+      issue(n + kD);
+    }
+  } else {
+    for (uint32_t n = 0; n < most; ++n) {
+      const size_t at = (kBack ? most - 1 - n : n) * step;
+      Vec<V> v[kN];
+      const bool live = (kBack ? most - 1 - n : n) < mine;
+      if (live) {
+#pragma unroll
+        for (int k = 0; k < kN; ++k) v[k] = *reinterpret_cast<const Vec<V>*>(src[k] + at);
+      }
+      f(at, v, live);
+    }
+  }
+}
+
+// V neighbouring channels of weight or bias
+template <int V>
+__device__ __forceinline__ void params(const void* p, int f32, uint32_t c, float none, float (&out)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = none;
+  if (p && f32) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = static_cast<const float*>(p)[c + i];
+  } else if (p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c + i]);
+  }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -82,6 +163,8 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
 }
+
+__device__ __forceinline__ uint4* ring_of(float2* sh) { return reinterpret_cast<uint4*>(sh); }
 
 // Where a thread works: which channel vector of the slab, which rows of the chunk.
 template <int V>
@@ -102,6 +185,7 @@ struct Place {
     live = lane_row < row_step;
     c0 = (first + vec) * V;
     row0 = (uint64_t)chunk * a.rows_per_chunk;
+    if (row0 > a.L) row0 = a.L;
     row1 = row0 + a.rows_per_chunk < a.L ? row0 + a.rows_per_chunk : a.L;
   }
 };
@@ -127,88 +211,115 @@ __device__ __forceinline__ void join_rows(const Place<V>& p, const float (&s)[V]
   __syncthreads();
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Pairs in `count` places of every block's `sh`, added over the cluster's blocks in the order of their ranks; each block writes
+// its share of the sums.
+__device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, float2* out) {
+  cluster_sync_all();
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(sh));
+  for (uint32_t i = cluster_rank() + kCluster * threadIdx.x; i < count; i += kCluster * kThreads) {
+    float2 v[kCluster];
+#pragma unroll
+    for (uint32_t k = 0; k < kCluster; ++k) {
+      uint32_t peer;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + i * 8), "r"(k));
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[k].x), "=f"(v[k].y) : "r"(peer) : "memory");
+    }
+    float2 t = v[0];
+#pragma unroll
+    for (uint32_t k = 1; k < kCluster; ++k) { t.x += v[k].x; t.y += v[k].y; }
+    out[i] = t;
+  }
+  cluster_sync_all();      // nobody leaves or writes its sums while they are read
+}
+// The slab's channel sums, weighted, added up to the groups that the slab touches: a warp a group.
+template <typename F>
+__device__ __forceinline__ void join_channels(const NormArgs& a, uint32_t slab_c0, uint32_t width, float2* groups, F&& pair) {
+  const uint32_t lane = threadIdx.x & 31;
+  for (uint32_t g = threadIdx.x >> 5; g < a.G; g += kWarps) {
+    const uint32_t lo = g * a.cg > slab_c0 ? g * a.cg : slab_c0;
+    const uint32_t hi = (g + 1) * a.cg < slab_c0 + width ? (g + 1) * a.cg : slab_c0 + width;
+    float s = 0.0f, q = 0.0f;
+    for (uint32_t c = lo + lane; c < hi; c += 32) {
+      const float2 t = pair(c);
+      s += t.x;
+      q += t.y;
+    }
+    s = warp_sum(s);
+    q = warp_sum(q);
+    if (lane == 0) groups[g] = make_float2(s, q);
+  }
+}
+// The sums of every group of sample b from the parts: eight threads a group take every eighth part each, then join.
+template <typename F>
+__device__ __forceinline__ void join_parts(const NormArgs& a, uint32_t b, F&& done) {
+  for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / 8) {
+    const uint32_t g = g0 + threadIdx.x / 8, k = threadIdx.x % 8;
+    float s = 0.0f, q = 0.0f;
+    if (g < a.G) {
+      const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
+#pragma unroll 4
+      for (uint32_t i = k; i < a.parts; i += 8) {
+        const float2 t = in[(size_t)i * a.G];
+        s += t.x;
+        q += t.y;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+      q += __shfl_xor_sync(0xFFFFFFFFu, q, d);
+    }
+    if (g < a.G && k == 0) done(g, s, q);
+  }
+  __syncthreads();
+}
+
 template <int V>
-__global__ void __launch_bounds__(kThreads) group_stats_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ float2 sh[];
+  extern __shared__ __align__(16) float2 sh[];
   const Place<V> p(a);
   const __nv_bfloat16* xs = a.x + (size_t)p.b * a.L * a.C;
   float shift[V], s[V], q[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = q[i] = shift[i] = 0.0f;
   if (p.live) {
-    load<V>(xs + p.c0, shift);
-    for (uint64_t r = p.row0 + p.lane_row; r < p.row1; r += p.row_step) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) shift[i] = __bfloat162float(xs[group_of(p.c0 + i, a.by_cg) * a.cg]);
+    const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
+    walk<1, V, false, false>(src, p.row1 - p.row0, p.lane_row, p.row_step, a.C, ring_of(sh), [&](size_t, const Vec<V>(&v)[1], bool) {
       float f[V];
-      load<V>(xs + r * a.C + p.c0, f);
+      unpack<V>(v[0], f);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float d = f[i] - shift[i];
         s[i] += d;
         q[i] = fmaf(d, d, q[i]);
       }
-    }
+    });
   }
+  __syncthreads();      // the sums take the ring's place
   const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
   const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
   join_rows<V>(p, s, q, sh, width);
-  // a warp for each group: mean and sum of squares about it over the group's channels that lie in this slab
-  const float n = (float)(p.row1 - p.row0);
-  float* out = a.partial + ((size_t)(p.b * a.chunks + p.chunk) * a.slabs + p.slab) * a.G * 3;
-  const uint32_t lane = threadIdx.x & 31;
-  for (uint32_t g = threadIdx.x >> 5; g < a.G; g += kWarps) {
-    const uint32_t lo = g * a.cg > slab_c0 ? g * a.cg : slab_c0;
-    const uint32_t hi = (g + 1) * a.cg < slab_c0 + width ? (g + 1) * a.cg : slab_c0 + width;
-    float count = 0.0f, mean = 0.0f, m2 = 0.0f;
-    if (lo < hi && n > 0.0f) {
-      float sum = 0.0f;
-      for (uint32_t c = lo + lane; c < hi; c += 32) sum += __bfloat162float(xs[c]) + sh[c - slab_c0].x / n;
-      mean = warp_sum(sum) / (float)(hi - lo);
-      float acc = 0.0f;
-      for (uint32_t c = lo + lane; c < hi; c += 32) {
-        const float2 t = sh[c - slab_c0];
-        const float off = __bfloat162float(xs[c]) + t.x / n - mean;
-        acc += fmaxf(t.y - t.x * (t.x / n), 0.0f) + n * off * off;
-      }
-      m2 = warp_sum(acc);
-      count = n * (float)(hi - lo);
-    }
-    if (lane == 0) { out[g * 3] = count; out[g * 3 + 1] = mean; out[g * 3 + 2] = m2; }
-  }
+  float2* groups = sh + kThreads * V;
+  join_channels(a, slab_c0, width, groups, [&](uint32_t c) { return sh[c - slab_c0]; });
+  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G);
 }
 
-// (mean, rstd) of every group of sample b, from the parts' triples: eight threads a group join every eighth part each, then
-// their results, always in the same order.
-__device__ __forceinline__ void chan(float& n, float& mean, float& m2, float n2, float mean2, float m22) {
-  const float t = n + n2;
-  if (n2 <= 0.0f) return;
-  if (n <= 0.0f) { n = n2; mean = mean2; m2 = m22; return; }
-  const float d = mean2 - mean, f = n2 / t;
-  mean = fmaf(d, f, mean);
-  m2 += m22 + d * d * n * f;
-  n = t;
-}
+// (mean, rstd) of every group of sample b
 __device__ __forceinline__ void finish_stats(const NormArgs& a, uint32_t b, float2* stats) {
-  const uint32_t parts = a.chunks * a.slabs;
-  for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / 8) {
-    const uint32_t g = g0 + threadIdx.x / 8, k = threadIdx.x % 8;
-    float n = 0.0f, mean = 0.0f, m2 = 0.0f;
-    if (g < a.G) {
-      const float* in = a.partial + ((size_t)b * parts * a.G + g) * 3;
-      for (uint32_t i = k; i < parts; i += 8) {
-        const float* t = in + (size_t)i * a.G * 3;
-        chan(n, mean, m2, t[0], t[1], t[2]);
-      }
-    }
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) {
-      const float n2 = __shfl_xor_sync(0xFFFFFFFFu, n, d), e2 = __shfl_xor_sync(0xFFFFFFFFu, mean, d), v2 = __shfl_xor_sync(0xFFFFFFFFu, m2, d);
-      if (k & d) { float na = n2, ma = e2, va = v2; chan(na, ma, va, n, mean, m2); n = na; mean = ma; m2 = va; }
-      else chan(n, mean, m2, n2, e2, v2);
-    }
-    if (g < a.G && k == 0) stats[g] = make_float2(mean, rsqrtf(m2 / n + a.eps));
-  }
-  __syncthreads();
+  const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
+  join_parts(a, b, [&](uint32_t g, float s, float q) {
+    const float off = s * inv_n, var = fmaxf(q * inv_n - off * off, 0.0f);
+    // fmaxf would turn the NaN of a group with a NaN or an infinity into 0
+    stats[g] = make_float2(__bfloat162float(a.x[(size_t)b * a.L * a.C + g * a.cg]) + off, q == q && q < INFINITY ? rsqrtf(var + a.eps) : NAN);
+  });
 }
 
 // Codes of V = 8 channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
@@ -223,145 +334,122 @@ __device__ __forceinline__ uint2 encode_row_block(const float (&y)[8], float& sc
 }
 
 template <int V, bool kCodes>
-__global__ void __launch_bounds__(kThreads) group_apply_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ float2 sh[];
+  extern __shared__ __align__(16) float2 sh[];
   const Place<V> p(a);
   finish_stats(a, p.b, sh);
   if (p.chunk == 0 && p.slab == 0)
-    for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) {
-      a.stats[((size_t)p.b * a.G + g) * 2] = sh[g].x;
-      a.stats[((size_t)p.b * a.G + g) * 2 + 1] = sh[g].y;
-    }
+    for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) reinterpret_cast<float2*>(a.stats)[(size_t)p.b * a.G + g] = sh[g];
   float mean[V], scale[V], bias[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const uint32_t c = p.c0 + i;
-    mean[i] = scale[i] = bias[i] = 0.0f;
-    if (p.live) {
-      const float2 t = sh[c / a.cg];
+  for (int i = 0; i < V; ++i) mean[i] = scale[i] = bias[i] = 0.0f;
+  if (p.live) {
+    params<V>(a.weight, a.params_f32, p.c0, 1.0f, scale);
+    params<V>(a.bias, a.params_f32, p.c0, 0.0f, bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 t = sh[group_of(p.c0 + i, a.by_cg)];
       mean[i] = t.x;
-      scale[i] = t.y * param(a.weight, a.params_f32, c, 1.0f);
-      bias[i] = param(a.bias, a.params_f32, c, 0.0f);
+      scale[i] *= t.y;
     }
   }
-  const size_t base = (size_t)p.b * a.L * a.C;
-  // with codes, 16 neighbouring lanes share a row: C / 8 is a multiple of 16 and so is the slab's width, so they are all live or none is
-  for (uint64_t r0 = p.row0; r0 < p.row1; r0 += p.row_step) {
-    const uint64_t r = r0 + p.lane_row;
-    const bool in = p.live && r < p.row1;
-    if (!kCodes && !in) continue;
+  __syncthreads();      // the ring takes the statistics' place
+  // From the chunk's end to its start: what the first launch read last is still in L2.
+  // With codes, 16 neighbouring lanes share a row (C / 8 and the slab's width are multiples of 16): all of them are live or none is.
+  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
+  if (!kCodes && !p.live) return;
+  const __nv_bfloat16* const src[1] = {a.x + first};
+  walk<1, V, true, kCodes>(src, p.row1 - p.row0, p.live ? p.lane_row : 0xFFFFFFFFu, p.row_step, a.C, ring_of(sh), [&](size_t at, const Vec<V>(&v)[1], bool live) {
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = 0.0f;
-    const size_t at = base + r * a.C + p.c0;
-    if (in) load<V>(a.x + at, f);
+    if (live) unpack<V>(v[0], f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float h = fmaf(f[i] - mean[i], scale[i], bias[i]);
+      const float h = fmaf(f[i] - mean[i], scale[i], bias[i]);      // first the difference: a group of equal values gives exactly the bias
       f[i] = a.silu ? h * sigmoid(h) : h;
     }
-    if (in) store<V>(a.y + at, f);
+    if (live) store<V>(a.y + first + at, f, a.stream);
     if constexpr (kCodes) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = __bfloat162float(__float2bfloat16_rn(f[i]));   // the codes are those of the BF16 output
+      for (int i = 0; i < V; ++i) f[i] = live ? __bfloat162float(__float2bfloat16_rn(f[i])) : 0.0f;   // the codes are those of the BF16 output
       float s;
       const uint2 c = encode_row_block(f, s);
-      if (in) {
-        *reinterpret_cast<uint2*>(a.codes + at) = c;
-        if ((p.vec & 15) == 0) a.code_scales[at / 128] = s;
+      if (live) {
+        *reinterpret_cast<uint2*>(a.codes + first + at) = c;
+        if ((p.vec & 15) == 0) a.code_scales[(first + at) / 128] = s;
       }
     }
-  }
+  });
 }
 
-// dh = dy * act'(h) of V channels
-template <int V>
-__device__ __forceinline__ void grad_h(const float (&x)[V], const float (&dy)[V], const float (&mean)[V], const float (&rstd)[V],
-                                       const float (&w)[V], const float (&bias)[V], int silu, float (&xhat)[V], float (&dh)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    xhat[i] = (x[i] - mean[i]) * rstd[i];
-    dh[i] = dy[i];
-    if (silu) {
-      const float h = fmaf(xhat[i], w[i], bias[i]), g = sigmoid(h);
-      dh[i] *= g * fmaf(h, 1.0f - g, 1.0f);
-    }
-  }
+// dy * act'(h)
+__device__ __forceinline__ float grad_h(float h, float dy, int silu) {
+  if (!silu) return dy;
+  const float g = sigmoid(h);
+  return dy * (g * fmaf(h, 1.0f - g, 1.0f));
 }
 
 template <int V>
-__device__ __forceinline__ void channel_params(const NormArgs& a, const Place<V>& p, float (&mean)[V], float (&rstd)[V], float (&w)[V], float (&bias)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    mean[i] = rstd[i] = w[i] = bias[i] = 0.0f;
-    if (p.live) {
-      const uint32_t c = p.c0 + i;
-      const float* t = a.stats + ((size_t)p.b * a.G + c / a.cg) * 2;
-      mean[i] = t[0];
-      rstd[i] = t[1];
-      w[i] = param(a.weight, a.params_f32, c, 1.0f);
-      bias[i] = param(a.bias, a.params_f32, c, 0.0f);
-    }
-  }
-}
-
-template <int V>
-__global__ void __launch_bounds__(kThreads) group_grad_sums_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ float2 sh[];
+  extern __shared__ __align__(16) float2 sh[];
   const Place<V> p(a);
-  float mean[V], rstd[V], w[V], bias[V], s[V], q[V];
-  channel_params<V>(a, p, mean, rstd, w, bias);
+  const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
+  float mean[V], scale[V], bias[V], s[V], q[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = q[i] = 0.0f;
-  const size_t base = (size_t)p.b * a.L * a.C;
   if (p.live) {
-    for (uint64_t r = p.row0 + p.lane_row; r < p.row1; r += p.row_step) {
-      float x[V], dy[V], xhat[V], dh[V];
-      load<V>(a.x + base + r * a.C + p.c0, x);
-      load<V>(a.dy + base + r * a.C + p.c0, dy);
-      grad_h<V>(x, dy, mean, rstd, w, bias, a.silu, xhat, dh);
+    params<V>(a.weight, a.params_f32, p.c0, 1.0f, scale);
+    params<V>(a.bias, a.params_f32, p.c0, 0.0f, bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 t = stats[group_of(p.c0 + i, a.by_cg)];
+      mean[i] = t.x;
+      scale[i] *= t.y;
+    }
+    const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
+    const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
+    walk<2, V, false, false>(src, p.row1 - p.row0, p.lane_row, p.row_step, a.C, ring_of(sh), [&](size_t, const Vec<V>(&v)[2], bool) {
+      float x[V], dy[V];
+      unpack<V>(v[0], x);
+      unpack<V>(v[1], dy);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[i] += dh[i];
-        q[i] = fmaf(dh[i], xhat[i], q[i]);
+        const float d = x[i] - mean[i], dh = grad_h(fmaf(d, scale[i], bias[i]), dy[i], a.silu);
+        s[i] += dh;
+        q[i] = fmaf(dh, d, q[i]);      // times rstd at the end
       }
-    }
+    });
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] *= stats[group_of(p.c0 + i, a.by_cg)].y;
   }
+  __syncthreads();      // the sums take the ring's place
   const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
   const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
   join_rows<V>(p, s, q, sh, width);
-  float2* cp = reinterpret_cast<float2*>(a.channel_partial) + (size_t)(p.b * a.chunks + p.chunk) * a.C + slab_c0;
-  for (uint32_t c = threadIdx.x; c < width; c += kThreads) cp[c] = sh[c];
-  float* out = a.partial + ((size_t)(p.b * a.chunks + p.chunk) * a.slabs + p.slab) * a.G * 2;
-  const uint32_t lane = threadIdx.x & 31;
-  for (uint32_t g = threadIdx.x >> 5; g < a.G; g += kWarps) {
-    const uint32_t lo = g * a.cg > slab_c0 ? g * a.cg : slab_c0;
-    const uint32_t hi = (g + 1) * a.cg < slab_c0 + width ? (g + 1) * a.cg : slab_c0 + width;
-    float s1 = 0.0f, s2 = 0.0f;
-    for (uint32_t c = lo + lane; c < hi; c += 32) {
-      const float wc = param(a.weight, a.params_f32, c, 1.0f);
-      s1 = fmaf(wc, sh[c - slab_c0].x, s1);
-      s2 = fmaf(wc, sh[c - slab_c0].y, s2);
-    }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    if (lane == 0) { out[g * 2] = s1; out[g * 2 + 1] = s2; }
-  }
+  float2* groups = sh + kThreads * V;
+  join_channels(a, slab_c0, width, groups, [&](uint32_t c) {
+    const float w = param(a.weight, a.params_f32, c, 1.0f);
+    return make_float2(w * sh[c - slab_c0].x, w * sh[c - slab_c0].y);
+  });
+  const uint32_t first = p.chunk / kCluster;
+  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + first) * a.G);
+  join_cluster(sh, width, a.channel_partial + ((size_t)p.b * (a.chunks / kCluster) + first) * a.C + slab_c0);
 }
 
 // The first blocks apply; the blocks behind them add the channel sums up to dweight and dbias.
 template <int V>
-__global__ void __launch_bounds__(kThreads) group_grad_apply_kernel(const __grid_constant__ NormArgs a, uint32_t apply_blocks) {
+__global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __grid_constant__ NormArgs a, uint32_t apply_blocks) {
   pdl_prologue();
-  extern __shared__ float2 sh[];
+  extern __shared__ __align__(16) float2 sh[];
   if (blockIdx.x >= apply_blocks) {
     // a warp's 32 lanes take 32 neighbouring channels, the eight warps every eighth part
     __shared__ float2 part[kWarps][32];
     const uint32_t lane = threadIdx.x & 31, wp = threadIdx.x >> 5, c = (blockIdx.x - apply_blocks) * 32 + lane;
-    const float2* cp = reinterpret_cast<const float2*>(a.channel_partial);
-    const uint32_t parts = a.B * a.chunks;
+    const float2* cp = a.channel_partial;
+    const uint32_t parts = a.B * (a.chunks / kCluster);
     float2 t = make_float2(0.0f, 0.0f);
     if (c < a.C)
       for (uint32_t i = wp; i < parts; i += kWarps) {
@@ -384,48 +472,40 @@ __global__ void __launch_bounds__(kThreads) group_grad_apply_kernel(const __grid
     return;
   }
   const Place<V> p(a);
-  {
-    const uint32_t parts = a.chunks * a.slabs;
-    const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
-    for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / 8) {
-      const uint32_t g = g0 + threadIdx.x / 8, k = threadIdx.x % 8;
-      float s1 = 0.0f, s2 = 0.0f;
-      if (g < a.G) {
-        const float* in = a.partial + ((size_t)p.b * parts * a.G + g) * 2;
-        for (uint32_t i = k; i < parts; i += 8) {
-          s1 += in[(size_t)i * a.G * 2];
-          s2 += in[(size_t)i * a.G * 2 + 1];
-        }
-      }
+  const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
+  join_parts(a, p.b, [&](uint32_t g, float s, float q) { sh[g] = make_float2(s * inv_n, q * inv_n); });
+  // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
+  const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
+  float scale[V], offset[V], slope[V], rest[V];
+  if (p.live) {
+    params<V>(a.weight, a.params_f32, p.c0, 1.0f, scale);
+    params<V>(a.bias, a.params_f32, p.c0, 0.0f, offset);
 #pragma unroll
-      for (int d = 1; d < 8; d <<= 1) {
-        s1 += __shfl_xor_sync(0xFFFFFFFFu, s1, d);
-        s2 += __shfl_xor_sync(0xFFFFFFFFu, s2, d);
-      }
-      if (g < a.G && k == 0) sh[g] = make_float2(s1 * inv_n, s2 * inv_n);
+    for (int i = 0; i < V; ++i) {
+      const uint32_t g = group_of(p.c0 + i, a.by_cg);
+      const float2 t = stats[g], m = sh[g];
+      scale[i] *= t.y;
+      offset[i] = fmaf(-t.x, scale[i], offset[i]);
+      slope[i] = -t.y * t.y * m.y;
+      rest[i] = fmaf(-t.x, slope[i], -t.y * m.x);
     }
-    __syncthreads();
   }
-  float mean[V], rstd[V], w[V], bias[V], m1[V], m2[V];
-  channel_params<V>(a, p, mean, rstd, w, bias);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float2 t = p.live ? sh[(p.c0 + i) / a.cg] : make_float2(0.0f, 0.0f);
-    m1[i] = t.x;
-    m2[i] = t.y;
-  }
-  const size_t base = (size_t)p.b * a.L * a.C;
+  __syncthreads();      // the ring takes the sums' place
   if (!p.live) return;
-  for (uint64_t r = p.row0 + p.lane_row; r < p.row1; r += p.row_step) {
-    float x[V], dy[V], xhat[V], dh[V];
-    const size_t at = base + r * a.C + p.c0;
-    load<V>(a.x + at, x);
-    load<V>(a.dy + at, dy);
-    grad_h<V>(x, dy, mean, rstd, w, bias, a.silu, xhat, dh);
+  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
+  const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
+  // from the chunk's end, as in the forward pass
+  walk<2, V, true, false>(src, p.row1 - p.row0, p.lane_row, p.row_step, a.C, ring_of(sh), [&](size_t at, const Vec<V>(&v)[2], bool) {
+    float x[V], dy[V];
+    unpack<V>(v[0], x);
+    unpack<V>(v[1], dy);
 #pragma unroll
-    for (int i = 0; i < V; ++i) dh[i] = rstd[i] * (fmaf(w[i], dh[i], -m1[i]) - xhat[i] * m2[i]);
-    store<V>(a.y + at, dh);
-  }
+    for (int i = 0; i < V; ++i) {
+      const float dh = grad_h(fmaf(x[i], scale[i], offset[i]), dy[i], a.silu);
+      x[i] = fmaf(scale[i], dh, fmaf(slope[i], x[i], rest[i]));
+    }
+    store<V>(a.y + first + at, x, a.stream);
+  });
 }
 
 int sm_count_here() {
@@ -437,33 +517,34 @@ int sm_count_here() {
 // How a call is cut: the width of a thread's channel vector, slabs of channels, chunks of positions.
 struct Plan {
   int V;
-  uint32_t slab_vecs, slabs, chunks;
+  uint32_t slab_vecs, slabs, chunks, parts;
   uint64_t rows_per_chunk;
 };
-Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, int sms) {
+Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, bool backward, int sms) {
   Plan p;
   p.V = (C % 8 == 0 && aligned16) ? 8 : (C % 2 == 0 && aligned4) ? 2 : 1;
   const uint32_t nvec = C / p.V;
   p.slabs = (nvec + kThreads - 1) / kThreads;
   // with slabs, a width that is a multiple of 16 vectors: a block of 128 channels lies in one slab
   p.slab_vecs = p.slabs == 1 ? nvec : kThreads;
-  // about four thread blocks on each SM, and at least 16 rows of threads' worth of work in a chunk
-  const uint64_t want = ((uint64_t)sms * 4 + (uint64_t)B * p.slabs - 1) / ((uint64_t)B * p.slabs);
+  // all the thread blocks that fit on the SMs at a time, and a few rows for each thread
+  uint64_t want = (uint64_t)sms * (backward ? 3 : 4) / ((uint64_t)B * p.slabs);
+  if (want < 1) want = 1;
   const uint32_t row_step = kThreads / p.slab_vecs;
   uint64_t most = (L + (uint64_t)row_step * 4 - 1) / ((uint64_t)row_step * 4);
   if (most < 1) most = 1;
   uint64_t chunks = want < most ? want : most;
-  if (chunks < 1) chunks = 1;
   if (chunks > 1024) chunks = 1024;
+  chunks = chunks < kCluster ? kCluster : chunks / kCluster * kCluster;
   p.rows_per_chunk = (L + chunks - 1) / chunks;
-  if (p.rows_per_chunk < 1) p.rows_per_chunk = 1;
-  p.chunks = (uint32_t)((L + p.rows_per_chunk - 1) / p.rows_per_chunk);
-  if (p.chunks < 1) p.chunks = 1;
+  chunks = (L + p.rows_per_chunk - 1) / p.rows_per_chunk;
+  p.chunks = (uint32_t)((chunks + kCluster - 1) / kCluster * kCluster);
+  p.parts = p.chunks / kCluster * p.slabs;
   return p;
 }
-size_t partial_floats(const Plan& p, uint32_t B, uint32_t C, uint32_t G, bool backward) {
-  const size_t groups = (size_t)B * p.chunks * p.slabs * G * (backward ? 2 : 3);
-  return ((groups + 3) / 4 * 4) + (backward ? (size_t)B * p.chunks * C * 2 : 0);
+size_t group_pairs(const Plan& p, uint32_t B, uint32_t G) { return ((size_t)B * p.parts * G + 1) / 2 * 2; }   // whole 16 bytes
+size_t partial_pairs(const Plan& p, uint32_t B, uint32_t C, uint32_t G, bool backward) {
+  return group_pairs(p, B, G) + (backward ? (size_t)B * (p.chunks / kCluster) * C : 0);
 }
 bool al(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -484,6 +565,24 @@ int refuse(const char* who, const char* what) {
   return (int)cudaErrorInvalidValue;
 }
 
+template <typename K>
+cudaError_t launch_clusters(K kernel, unsigned grid, size_t smem, cudaStream_t stream, const NormArgs& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 template <typename F>
 cudaError_t by_width(int V, F&& f) {
   if (V == 8) return f(std::integral_constant<int, 8>());
@@ -502,10 +601,10 @@ size_t flame_group_norm_workspace_bytes(size_t B, size_t L, size_t C, size_t G, 
   if (check("flame_group_norm_workspace_bytes", B, L, C, G, 0, 0) != 0 || B == 0 || L == 0) return 0;
   size_t most = 0;   // whatever the alignment of the tensors turns out to be
   for (int k = 0; k < 3; ++k) {
-    const size_t f = partial_floats(plan((uint32_t)B, L, (uint32_t)C, k == 0, k <= 1, sm_count_here()), (uint32_t)B, (uint32_t)C, (uint32_t)G, backward != 0);
+    const size_t f = partial_pairs(plan((uint32_t)B, L, (uint32_t)C, k == 0, k <= 1, backward != 0, sm_count_here()), (uint32_t)B, (uint32_t)C, (uint32_t)G, backward != 0);
     most = f > most ? f : most;
   }
-  return most * sizeof(float);
+  return most * sizeof(float2);
 }
 
 int flame_group_norm(const void* x, const void* weight, const void* bias, void* y, void* codes, void* code_scales, void* stats,
@@ -520,20 +619,22 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   const bool al16 = al(x, 16) && al(y, 16);
   if (codes && (C % 128 != 0 || !al16 || !al(codes, 8) || !code_scales)) return refuse(who, "codes need channels % 128 == 0, 16-byte aligned tensors and a place for the scales");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
-  const Plan p = plan((uint32_t)B, L, (uint32_t)C, al16, al(x, 4) && al(y, 4), sm_count_here());
+  const Plan p = plan((uint32_t)B, L, (uint32_t)C, al16, al(x, 4) && al(y, 4), false, sm_count_here());
   NormArgs a = {};
   a.x = static_cast<const __nv_bfloat16*>(x); a.weight = weight; a.bias = bias; a.y = static_cast<__nv_bfloat16*>(y);
   a.codes = static_cast<uint8_t*>(codes); a.code_scales = static_cast<float*>(code_scales); a.stats = static_cast<float*>(stats);
-  a.partial = static_cast<float*>(workspace);
+  a.partial = static_cast<float2*>(workspace);
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
-  a.chunks = p.chunks; a.rows_per_chunk = p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
-  a.eps = eps; a.silu = activation == FLAME_ACTIVATION_SILU; a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
+  a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
+  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
+  a.eps = eps; a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
   const unsigned grid = (unsigned)(B * p.slabs * p.chunks);
-  const size_t sums = (size_t)kThreads * p.V * sizeof(float2), groups = G * sizeof(float2);
+  const size_t ring = p.V == 8 ? (size_t)kDepth * kThreads * 16 : 0, pairs = ((size_t)kThreads * p.V + G) * sizeof(float2), sums = pairs > ring ? pairs : ring;
+  const size_t groups = G * sizeof(float2) > ring ? G * sizeof(float2) : ring;
   cudaStream_t s = (cudaStream_t)stream;
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    cudaError_t e = launch_after(group_stats_kernel<V>, grid, kThreads, sums, s, a);
+    cudaError_t e = launch_clusters(group_stats_kernel<V>, grid, sums, s, a);
     if (e != cudaSuccess) return e;
     if constexpr (V == 8) {
       if (a.codes) return launch_after(group_apply_kernel<8, true>, grid, kThreads, groups, s, a);
@@ -558,22 +659,24 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   if (workspace_bytes < flame_group_norm_workspace_bytes(B, L, C, G, 1)) return refuse(who, "workspace too small");
   if (!al(x, 2) || !al(dy, 2) || !al(dx, 2) || !al(stats, 4) || !al(workspace, 16)) return refuse(who, "misaligned tensor");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
-  const Plan p = plan((uint32_t)B, L, (uint32_t)C, al(x, 16) && al(dy, 16) && al(dx, 16), al(x, 4) && al(dy, 4) && al(dx, 4), sm_count_here());
+  const Plan p = plan((uint32_t)B, L, (uint32_t)C, al(x, 16) && al(dy, 16) && al(dx, 16), al(x, 4) && al(dy, 4) && al(dx, 4), true, sm_count_here());
   NormArgs a = {};
   a.x = static_cast<const __nv_bfloat16*>(x); a.dy = static_cast<const __nv_bfloat16*>(dy); a.weight = weight; a.bias = bias;
   a.y = static_cast<__nv_bfloat16*>(dx); a.stats = const_cast<float*>(static_cast<const float*>(stats));
-  a.partial = static_cast<float*>(workspace);
-  a.channel_partial = a.partial + ((size_t)B * p.chunks * p.slabs * G * 2 + 3) / 4 * 4;
+  a.partial = static_cast<float2*>(workspace);
+  a.channel_partial = a.partial + group_pairs(p, (uint32_t)B, (uint32_t)G);
   a.dweight = dweight; a.dbias = dbias;
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
-  a.chunks = p.chunks; a.rows_per_chunk = p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
-  a.silu = activation == FLAME_ACTIVATION_SILU; a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
+  a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
+  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
+  a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
   const unsigned grid = (unsigned)(B * p.slabs * p.chunks);
   const unsigned more = (dweight || dbias) ? (unsigned)((C + 31) / 32) : 0;
-  const size_t sums = (size_t)kThreads * p.V * sizeof(float2), groups = G * sizeof(float2);
+  const size_t ring = p.V == 8 ? (size_t)kDepth * kThreads * 16 : 0, pairs = ((size_t)kThreads * p.V + G) * sizeof(float2), sums = pairs > ring ? pairs : ring;
+  const size_t groups = G * sizeof(float2) > ring ? G * sizeof(float2) : ring;
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    const cudaError_t e = launch_after(group_grad_sums_kernel<V>, grid, kThreads, sums, s, a);
+    const cudaError_t e = launch_clusters(group_grad_sums_kernel<V>, grid, sums, s, a);
     if (e != cudaSuccess) return e;
     return launch_after(group_grad_apply_kernel<V>, grid + more, kThreads, groups, s, a, (uint32_t)grid);
   });
