@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr uint32_t kCluster = 8;
+constexpr uint32_t kCluster = 4;
 
 struct NormArgs {
   const __nv_bfloat16* x;
@@ -46,7 +46,7 @@ struct NormArgs {
   uint64_t L;
   uint32_t chunks;               // per sample and slab, a multiple of the cluster's blocks (the last ones may be empty)
   uint32_t parts;                // clusters per sample: chunks / kCluster * slabs
-  uint64_t rows_per_chunk;
+  uint32_t rows_per_chunk;
   uint32_t slabs;                // channel slabs of one thread block's width
   uint32_t slab_vecs;            // V-wide channel vectors in a slab
   float eps;
@@ -92,64 +92,91 @@ __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[V], int
   }
   *reinterpret_cast<Vec<V>*>(p) = r;
 }
-// Walks a thread down its rows: f(offset, vectors) for each, offset in elements from the thread's first row, kN tensors at a time;
-// kBack: from the last row to the first.  f(.., live = false) where another thread of the block still has a row and this one has none
-// (only with kWhole, for shuffles inside f).
+// A thread's way down its rows, kN tensors at a time; kBack: from the last row to the first.  The constructor sends the first rows on
+// their way, run(f) calls f(offset, vectors, live) for each row, offset in elements from the thread's first row; with kWhole also,
+// with live = false, where another thread of the block has a row and this one has none (for shuffles inside f).
 //
 // The rows ahead are on their way to shared memory as asynchronous copies, each thread's own in places of its own, so nothing waits
 // for another thread and nothing is held in registers: with one row in flight in registers the two passes over 1024 x 1024 x 128
-// took 72 and 174 us, with four, which left two blocks on an SM, 76 and 152.
+// took 72 and 174 us, with four, which left two blocks on an SM, 76 and 152, this way 57 and 95.
 constexpr int kDepth = 8;
-template <int kN, int V, bool kBack, bool kWhole, typename F>
-__device__ __forceinline__ void walk(const __nv_bfloat16* const (&src)[kN], uint64_t rows, uint32_t lane_row, uint32_t row_step, uint32_t C, uint4* ring, F&& f) {
-  const uint32_t mine = rows > lane_row ? (uint32_t)((rows - lane_row + row_step - 1) / row_step) : 0;
-  const uint32_t most = kWhole ? (uint32_t)((rows + row_step - 1) / row_step) : mine;
-  const size_t step = (size_t)row_step * C;
-  if constexpr (V == 8) {
-    constexpr int kD = kDepth / kN;
-    auto place = [&](uint32_t n, int k) { return ring + ((n % kD) * kN + k) * kThreads + threadIdx.x; };
-    auto row_of = [&](uint32_t n) { return kBack ? most - 1 - n : n; };
-    auto issue = [&](uint32_t n) {
-      if (n < most && row_of(n) < mine) {
+constexpr size_t kRingBytes = (size_t)kDepth * kThreads * 16;
+template <int kN, int V, bool kBack, bool kWhole>
+struct Walk {
+  static constexpr int kD = kDepth / kN;      // rows on their way
+  const __nv_bfloat16* const (&src)[kN];
+  uint4* ring;
+  uint32_t mine, most, skip, in, sent;
+  ptrdiff_t step, first, next;
+
+  __device__ __forceinline__ void send() {
+    if (sent < most && (!kWhole || (kBack ? sent >= skip : sent < mine))) {
+      const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring + threadIdx.x);
 #pragma unroll
-        for (int k = 0; k < kN; ++k)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(place(n, k))), "l"(src[k] + row_of(n) * step) : "memory");
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int n = 0; n < kD; ++n) issue(n);
-    for (uint32_t n = 0; n < most; ++n) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kD - 1) : "memory");
-      Vec<V> v[kN];
-      const bool live = row_of(n) < mine;
-      if (live) {
-#pragma unroll
-        for (int k = 0; k < kN; ++k) { const uint4 w = *place(n, k); v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
-      }
-      f(row_of(n) * step, v, live);
-      issue(n + kD);
+      for (int k = 0; k < kN; ++k)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + (in * kN + k) * kThreads * 16), "l"(src[k] + next) : "memory");
     }
-  } else {
-    for (uint32_t n = 0; n < most; ++n) {
-      const size_t at = (kBack ? most - 1 - n : n) * step;
+    ++sent;
+    next += step;
+    in = in + 1 == kD ? 0 : in + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ Walk(const __nv_bfloat16* const (&s)[kN], uint32_t rows, uint32_t lane_row, uint32_t row_step, uint32_t C, uint4* r)
+      : src(s), ring(r), in(0), sent(0) {
+    mine = rows > lane_row ? (rows - lane_row + row_step - 1) / row_step : 0;
+    most = kWhole ? (rows + row_step - 1) / row_step : mine;
+    step = (kBack ? -1 : 1) * (ptrdiff_t)((size_t)row_step * C);
+    first = next = kBack ? -step * ((ptrdiff_t)most - 1) : 0;
+    skip = kBack ? most - mine : 0;      // rounds before this thread's first row, from the back
+    if constexpr (V == 8) {
+#pragma unroll
+      for (int n = 0; n < kD; ++n) send();
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(F&& f) {
+    ptrdiff_t at = first;
+    uint32_t out = 0;
+    for (uint32_t n = 0; n < most; ++n, at += step) {
       Vec<V> v[kN];
-      const bool live = (kBack ? most - 1 - n : n) < mine;
-      if (live) {
+      const bool live = !kWhole || (kBack ? n >= skip : n < mine);
+      if constexpr (V == 8) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kD - 1) : "memory");
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < kN; ++k) { const uint4 w = ring[(out * kN + k) * kThreads + threadIdx.x]; v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
+        }
+        out = out + 1 == kD ? 0 : out + 1;
+      } else if (live) {
 #pragma unroll
         for (int k = 0; k < kN; ++k) v[k] = *reinterpret_cast<const Vec<V>*>(src[k] + at);
       }
       f(at, v, live);
+      if constexpr (V == 8) send();
     }
   }
-}
+};
 
 // V neighbouring channels of weight or bias
 template <int V>
 __device__ __forceinline__ void params(const void* p, int f32, uint32_t c, float none, float (&out)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] = none;
-  if (p && f32) {
+  if (V == 8 && p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {      // c is a multiple of 8
+    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + c);
+    float4 lo, hi;
+    if (f32) {
+      lo = f[0];
+      hi = f[1];
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + c);
+      lo = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+      hi = make_float4(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xFFFF0000u), __uint_as_float(w.w << 16), __uint_as_float(w.w & 0xFFFF0000u));
+    }
+    const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = v[i];
+  } else if (p && f32) {
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = static_cast<const float*>(p)[c + i];
   } else if (p) {
@@ -164,39 +191,44 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ uint4* ring_of(float2* sh) { return reinterpret_cast<uint4*>(sh); }
+// Shared memory: the ring (vectors of eight channels only), then pairs of sums.
+template <int V>
+__device__ __forceinline__ float2* sums_of(uint4* ring) { return reinterpret_cast<float2*>(ring + (V == 8 ? kRingBytes / 16 : 0)); }
 
 // Where a thread works: which channel vector of the slab, which rows of the chunk.
 template <int V>
 struct Place {
   uint32_t b, chunk, slab, vec, lane_row, row_step, c0;
-  uint64_t row0, row1;
+  uint64_t row0;
+  uint32_t rows;
   bool live;
   __device__ __forceinline__ explicit Place(const NormArgs& a) {
-    chunk = blockIdx.x % a.chunks;
-    const uint32_t rest = blockIdx.x / a.chunks;
-    slab = rest % a.slabs;
-    b = rest / a.slabs;
+    chunk = blockIdx.x;
+    slab = blockIdx.y;
+    b = blockIdx.z;
     const uint32_t nvec = a.C / V, first = slab * a.slab_vecs;
     const uint32_t here = nvec - first < a.slab_vecs ? nvec - first : a.slab_vecs;
     row_step = kThreads / here;
-    vec = threadIdx.x % here;
     lane_row = threadIdx.x / here;
+    vec = threadIdx.x - lane_row * here;
     live = lane_row < row_step;
     c0 = (first + vec) * V;
     row0 = (uint64_t)chunk * a.rows_per_chunk;
     if (row0 > a.L) row0 = a.L;
-    row1 = row0 + a.rows_per_chunk < a.L ? row0 + a.rows_per_chunk : a.L;
+    rows = a.L - row0 < a.rows_per_chunk ? (uint32_t)(a.L - row0) : a.rows_per_chunk;
   }
 };
 
-// Per-channel pairs of a thread block, added over its rows of threads in a fixed order: out[c] for the slab's channels.
+// Per-channel pairs of a thread block, added over its rows of threads in a fixed order.  Channel c of the slab lies at
+// place_of(c): first every vector's first channel, then every second one, so that neighbouring lanes write neighbouring words.
+template <int V>
+__device__ __forceinline__ uint32_t place_of(uint32_t c, uint32_t width) { return c % V * (width / V) + c / V; }
 template <int V>
 __device__ __forceinline__ void join_rows(const Place<V>& p, const float (&s)[V], const float (&q)[V], float2* sh, uint32_t width) {
   // sh holds row_step x width pairs; width = channels of the slab
   if (p.live) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) sh[p.lane_row * width + p.vec * V + i] = make_float2(s[i], q[i]);
+    for (int i = 0; i < V; ++i) sh[p.lane_row * width + i * (width / V) + p.vec] = make_float2(s[i], q[i]);
   }
   __syncthreads();
   for (uint32_t c = threadIdx.x; c < width; c += kThreads) {
@@ -216,9 +248,10 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Pairs in `count` places of every block's `sh`, added over the cluster's blocks in the order of their ranks; each block writes
-// its share of the sums.
-__device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, float2* out) {
+// `count` pairs of every block's `sh`, pair i at place(i), added over the cluster's blocks in the order of their ranks; each block
+// writes its share of the sums.
+template <typename F>
+__device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, float2* out, F&& place) {
   cluster_sync_all();
   const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(sh));
   for (uint32_t i = cluster_rank() + kCluster * threadIdx.x; i < count; i += kCluster * kThreads) {
@@ -226,7 +259,7 @@ __device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, f
 #pragma unroll
     for (uint32_t k = 0; k < kCluster; ++k) {
       uint32_t peer;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + i * 8), "r"(k));
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + place(i) * 8), "r"(k));
       asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[k].x), "=f"(v[k].y) : "r"(peer) : "memory");
     }
     float2 t = v[0];
@@ -236,22 +269,22 @@ __device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, f
   }
   cluster_sync_all();      // nobody leaves or writes its sums while they are read
 }
-// The slab's channel sums, weighted, added up to the groups that the slab touches: a warp a group.
+// The slab's channel sums, weighted, added up to the groups that the slab touches: a thread a group, a warp where groups are wide.
 template <typename F>
 __device__ __forceinline__ void join_channels(const NormArgs& a, uint32_t slab_c0, uint32_t width, float2* groups, F&& pair) {
   const uint32_t lane = threadIdx.x & 31;
-  for (uint32_t g = threadIdx.x >> 5; g < a.G; g += kWarps) {
+  const bool warps = a.cg > 32;
+  for (uint32_t g = warps ? threadIdx.x >> 5 : threadIdx.x; g < a.G; g += warps ? kWarps : kThreads) {
     const uint32_t lo = g * a.cg > slab_c0 ? g * a.cg : slab_c0;
     const uint32_t hi = (g + 1) * a.cg < slab_c0 + width ? (g + 1) * a.cg : slab_c0 + width;
     float s = 0.0f, q = 0.0f;
-    for (uint32_t c = lo + lane; c < hi; c += 32) {
+    for (uint32_t c = warps ? lo + lane : lo; c < hi; c += warps ? 32 : 1) {
       const float2 t = pair(c);
       s += t.x;
       q += t.y;
     }
-    s = warp_sum(s);
-    q = warp_sum(q);
-    if (lane == 0) groups[g] = make_float2(s, q);
+    if (warps) { s = warp_sum(s); q = warp_sum(q); }
+    if (!warps || lane == 0) groups[g] = make_float2(s, q);
   }
 }
 // The sums of every group of sample b from the parts: eight threads a group take every eighth part each, then join.
@@ -282,34 +315,34 @@ __device__ __forceinline__ void join_parts(const NormArgs& a, uint32_t b, F&& do
 template <int V>
 __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ __align__(16) float2 sh[];
+  extern __shared__ uint4 ring[];
+  float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
   const __nv_bfloat16* xs = a.x + (size_t)p.b * a.L * a.C;
+  const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
+  Walk<1, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   float shift[V], s[V], q[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) s[i] = q[i] = shift[i] = 0.0f;
-  if (p.live) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) shift[i] = __bfloat162float(xs[group_of(p.c0 + i, a.by_cg) * a.cg]);
-    const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
-    walk<1, V, false, false>(src, p.row1 - p.row0, p.lane_row, p.row_step, a.C, ring_of(sh), [&](size_t, const Vec<V>(&v)[1], bool) {
-      float f[V];
-      unpack<V>(v[0], f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = f[i] - shift[i];
-        s[i] += d;
-        q[i] = fmaf(d, d, q[i]);
-      }
-    });
+  for (int i = 0; i < V; ++i) {
+    s[i] = q[i] = 0.0f;
+    shift[i] = p.live ? __bfloat162float(xs[group_of(p.c0 + i, a.by_cg) * a.cg]) : 0.0f;
   }
-  __syncthreads();      // the sums take the ring's place
+  way.run([&](ptrdiff_t, const Vec<V>(&v)[1], bool) {
+    float f[V];
+    unpack<V>(v[0], f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float d = f[i] - shift[i];
+      s[i] += d;
+      q[i] = fmaf(d, d, q[i]);
+    }
+  });
   const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
   const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
   join_rows<V>(p, s, q, sh, width);
   float2* groups = sh + kThreads * V;
-  join_channels(a, slab_c0, width, groups, [&](uint32_t c) { return sh[c - slab_c0]; });
-  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G);
+  join_channels(a, slab_c0, width, groups, [&](uint32_t c) { return sh[place_of<V>(c - slab_c0, width)]; });
+  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G, [](uint32_t i) { return i; });
 }
 
 // (mean, rstd) of every group of sample b
@@ -336,8 +369,14 @@ __device__ __forceinline__ uint2 encode_row_block(const float (&y)[8], float& sc
 template <int V, bool kCodes>
 __global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ __align__(16) float2 sh[];
+  extern __shared__ uint4 ring[];
+  float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
+  // From the chunk's end to its start: what the first launch read last is still in L2.
+  // With codes, 16 neighbouring lanes share a row (C / 8 and the slab's width are multiples of 16): all of them are live or none is.
+  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
+  const __nv_bfloat16* const src[1] = {a.x + first};
+  Walk<1, V, true, kCodes> way(src, kCodes || p.live ? p.rows : 0, p.live ? p.lane_row : 0xFFFFFFFFu, p.row_step, a.C, ring);
   finish_stats(a, p.b, sh);
   if (p.chunk == 0 && p.slab == 0)
     for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) reinterpret_cast<float2*>(a.stats)[(size_t)p.b * a.G + g] = sh[g];
@@ -354,13 +393,7 @@ __global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(c
       scale[i] *= t.y;
     }
   }
-  __syncthreads();      // the ring takes the statistics' place
-  // From the chunk's end to its start: what the first launch read last is still in L2.
-  // With codes, 16 neighbouring lanes share a row (C / 8 and the slab's width are multiples of 16): all of them are live or none is.
-  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
-  if (!kCodes && !p.live) return;
-  const __nv_bfloat16* const src[1] = {a.x + first};
-  walk<1, V, true, kCodes>(src, p.row1 - p.row0, p.live ? p.lane_row : 0xFFFFFFFFu, p.row_step, a.C, ring_of(sh), [&](size_t at, const Vec<V>(&v)[1], bool live) {
+  way.run([&](ptrdiff_t at, const Vec<V>(&v)[1], bool live) {
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = 0.0f;
@@ -394,9 +427,13 @@ __device__ __forceinline__ float grad_h(float h, float dy, int silu) {
 template <int V>
 __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ __align__(16) float2 sh[];
+  extern __shared__ uint4 ring[];
+  float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
+  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
+  const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
+  Walk<2, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   float mean[V], scale[V], bias[V], s[V], q[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = q[i] = 0.0f;
@@ -409,9 +446,7 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
       mean[i] = t.x;
       scale[i] *= t.y;
     }
-    const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
-    const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
-    walk<2, V, false, false>(src, p.row1 - p.row0, p.lane_row, p.row_step, a.C, ring_of(sh), [&](size_t, const Vec<V>(&v)[2], bool) {
+    way.run([&](ptrdiff_t, const Vec<V>(&v)[2], bool) {
       float x[V], dy[V];
       unpack<V>(v[0], x);
       unpack<V>(v[1], dy);
@@ -425,53 +460,61 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < V; ++i) q[i] *= stats[group_of(p.c0 + i, a.by_cg)].y;
   }
-  __syncthreads();      // the sums take the ring's place
   const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
   const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
   join_rows<V>(p, s, q, sh, width);
   float2* groups = sh + kThreads * V;
   join_channels(a, slab_c0, width, groups, [&](uint32_t c) {
     const float w = param(a.weight, a.params_f32, c, 1.0f);
-    return make_float2(w * sh[c - slab_c0].x, w * sh[c - slab_c0].y);
+    const float2 t = sh[place_of<V>(c - slab_c0, width)];
+    return make_float2(w * t.x, w * t.y);
   });
-  const uint32_t first = p.chunk / kCluster;
-  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + first) * a.G);
-  join_cluster(sh, width, a.channel_partial + ((size_t)p.b * (a.chunks / kCluster) + first) * a.C + slab_c0);
+  const uint32_t part = p.chunk / kCluster;
+  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + part) * a.G, [](uint32_t i) { return i; });
+  join_cluster(sh, width, a.channel_partial + ((size_t)p.b * (a.chunks / kCluster) + part) * a.C + slab_c0, [&](uint32_t c) { return place_of<V>(c, width); });
 }
 
-// The first blocks apply; the blocks behind them add the channel sums up to dweight and dbias.
+// The blocks of one more sample than there are add the channel sums up to dweight and dbias.
 template <int V>
-__global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __grid_constant__ NormArgs a, uint32_t apply_blocks) {
+__global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  extern __shared__ __align__(16) float2 sh[];
-  if (blockIdx.x >= apply_blocks) {
+  extern __shared__ uint4 ring[];
+  float2* sh = sums_of<V>(ring);
+  if (blockIdx.z == a.B) {
     // a warp's 32 lanes take 32 neighbouring channels, the eight warps every eighth part
     __shared__ float2 part[kWarps][32];
-    const uint32_t lane = threadIdx.x & 31, wp = threadIdx.x >> 5, c = (blockIdx.x - apply_blocks) * 32 + lane;
-    const float2* cp = a.channel_partial;
-    const uint32_t parts = a.B * (a.chunks / kCluster);
-    float2 t = make_float2(0.0f, 0.0f);
-    if (c < a.C)
-      for (uint32_t i = wp; i < parts; i += kWarps) {
-        const float2 u = cp[(size_t)i * a.C + c];
-        t.x += u.x;
-        t.y += u.y;
+    const uint32_t lane = threadIdx.x & 31, wp = threadIdx.x >> 5, parts = a.B * (a.chunks / kCluster);
+    for (uint32_t c0 = (blockIdx.y * gridDim.x + blockIdx.x) * 32; c0 < a.C; c0 += gridDim.x * gridDim.y * 32) {
+      const uint32_t c = c0 + lane;
+      float2 t = make_float2(0.0f, 0.0f);
+      if (c < a.C) {
+#pragma unroll 4
+        for (uint32_t i = wp; i < parts; i += kWarps) {
+          const float2 u = a.channel_partial[(size_t)i * a.C + c];
+          t.x += u.x;
+          t.y += u.y;
+        }
       }
-    part[wp][lane] = t;
-    __syncthreads();
-    if (wp == 0 && c < a.C) {
-      for (int k = 1; k < kWarps; ++k) { t.x += part[k][lane].x; t.y += part[k][lane].y; }
-      if (a.params_f32) {
-        if (a.dbias) static_cast<float*>(a.dbias)[c] = t.x;
-        if (a.dweight) static_cast<float*>(a.dweight)[c] = t.y;
-      } else {
-        if (a.dbias) static_cast<__nv_bfloat16*>(a.dbias)[c] = __float2bfloat16_rn(t.x);
-        if (a.dweight) static_cast<__nv_bfloat16*>(a.dweight)[c] = __float2bfloat16_rn(t.y);
+      part[wp][lane] = t;
+      __syncthreads();
+      if (wp == 0 && c < a.C) {
+        for (int k = 1; k < kWarps; ++k) { t.x += part[k][lane].x; t.y += part[k][lane].y; }
+        if (a.params_f32) {
+          if (a.dbias) static_cast<float*>(a.dbias)[c] = t.x;
+          if (a.dweight) static_cast<float*>(a.dweight)[c] = t.y;
+        } else {
+          if (a.dbias) static_cast<__nv_bfloat16*>(a.dbias)[c] = __float2bfloat16_rn(t.x);
+          if (a.dweight) static_cast<__nv_bfloat16*>(a.dweight)[c] = __float2bfloat16_rn(t.y);
+        }
       }
+      __syncthreads();
     }
     return;
   }
   const Place<V> p(a);
+  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
+  const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
+  Walk<2, V, true, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);      // from the chunk's end, as in the forward pass
   const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
   join_parts(a, p.b, [&](uint32_t g, float s, float q) { sh[g] = make_float2(s * inv_n, q * inv_n); });
   // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
@@ -490,12 +533,7 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
       rest[i] = fmaf(-t.x, slope[i], -t.y * m.x);
     }
   }
-  __syncthreads();      // the ring takes the sums' place
-  if (!p.live) return;
-  const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
-  const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
-  // from the chunk's end, as in the forward pass
-  walk<2, V, true, false>(src, p.row1 - p.row0, p.lane_row, p.row_step, a.C, ring_of(sh), [&](size_t at, const Vec<V>(&v)[2], bool) {
+  way.run([&](ptrdiff_t at, const Vec<V>(&v)[2], bool) {
     float x[V], dy[V];
     unpack<V>(v[0], x);
     unpack<V>(v[1], dy);
@@ -531,7 +569,7 @@ Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, boo
   uint64_t want = (uint64_t)sms * (backward ? 3 : 4) / ((uint64_t)B * p.slabs);
   if (want < 1) want = 1;
   const uint32_t row_step = kThreads / p.slab_vecs;
-  uint64_t most = (L + (uint64_t)row_step * 4 - 1) / ((uint64_t)row_step * 4);
+  uint64_t most = (L + (uint64_t)row_step * 8 - 1) / ((uint64_t)row_step * 8);
   if (most < 1) most = 1;
   uint64_t chunks = want < most ? want : most;
   if (chunks > 1024) chunks = 1024;
@@ -553,7 +591,7 @@ int check(const char* who, uint64_t B, uint64_t L, uint64_t C, uint64_t G, int a
   if (G == 0 || C == 0 || C % G != 0) what = "the channels must be a positive multiple of the groups";
   else if (C > 65536) what = "at most 65536 channels";
   else if (G > 4096) what = "at most 4096 groups";
-  else if (B > 65535 || L > 0x7FFFFFFFull) what = "at most 65535 samples of at most 2^31 - 1 positions";
+  else if (B > 65534 || L > 0x7FFFFFFFull) what = "at most 65534 samples of at most 2^31 - 1 positions";
   else if (activation != FLAME_ACTIVATION_NONE && activation != FLAME_ACTIVATION_SILU) what = "unknown activation";
   else if (param_dtype != FLAME_OFFLOAD_DTYPE_BF16 && param_dtype != FLAME_OFFLOAD_DTYPE_F32) what = "weight and bias must be BF16 or F32";
   if (!what) return 0;
@@ -566,20 +604,29 @@ int refuse(const char* who, const char* what) {
 }
 
 template <typename K>
-cudaError_t launch_clusters(K kernel, unsigned grid, size_t smem, cudaStream_t stream, const NormArgs& a) {
+cudaError_t launch(K kernel, dim3 grid, bool clusters, size_t smem, cudaStream_t stream, const NormArgs& a) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (clusters) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = kCluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = n;
+  if (smem > 46 * 1024)      // beside two kilobytes that are not dynamic
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
@@ -626,20 +673,19 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   a.partial = static_cast<float2*>(workspace);
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
   a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
-  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
+  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
   a.eps = eps; a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
-  const unsigned grid = (unsigned)(B * p.slabs * p.chunks);
-  const size_t ring = p.V == 8 ? (size_t)kDepth * kThreads * 16 : 0, pairs = ((size_t)kThreads * p.V + G) * sizeof(float2), sums = pairs > ring ? pairs : ring;
-  const size_t groups = G * sizeof(float2) > ring ? G * sizeof(float2) : ring;
+  const dim3 grid(p.chunks, p.slabs, (unsigned)B);
+  const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
   cudaStream_t s = (cudaStream_t)stream;
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    cudaError_t e = launch_clusters(group_stats_kernel<V>, grid, sums, s, a);
+    cudaError_t e = launch(group_stats_kernel<V>, grid, true, sums, s, a);
     if (e != cudaSuccess) return e;
     if constexpr (V == 8) {
-      if (a.codes) return launch_after(group_apply_kernel<8, true>, grid, kThreads, groups, s, a);
+      if (a.codes) return launch(group_apply_kernel<8, true>, grid, false, groups, s, a);
     }
-    return launch_after(group_apply_kernel<V, false>, grid, kThreads, groups, s, a);
+    return launch(group_apply_kernel<V, false>, grid, false, groups, s, a);
   });
 }
 
@@ -668,17 +714,16 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   a.dweight = dweight; a.dbias = dbias;
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
   a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
-  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
+  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
   a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
-  const unsigned grid = (unsigned)(B * p.slabs * p.chunks);
-  const unsigned more = (dweight || dbias) ? (unsigned)((C + 31) / 32) : 0;
-  const size_t ring = p.V == 8 ? (size_t)kDepth * kThreads * 16 : 0, pairs = ((size_t)kThreads * p.V + G) * sizeof(float2), sums = pairs > ring ? pairs : ring;
-  const size_t groups = G * sizeof(float2) > ring ? G * sizeof(float2) : ring;
+  const dim3 grid(p.chunks, p.slabs, (unsigned)B);
+  const dim3 more(p.chunks, p.slabs, (unsigned)B + (dweight || dbias ? 1 : 0));
+  const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    const cudaError_t e = launch_clusters(group_grad_sums_kernel<V>, grid, sums, s, a);
+    const cudaError_t e = launch(group_grad_sums_kernel<V>, grid, true, sums, s, a);
     if (e != cudaSuccess) return e;
-    return launch_after(group_grad_apply_kernel<V>, grid + more, kThreads, groups, s, a, (uint32_t)grid);
+    return launch(group_grad_apply_kernel<V>, more, false, groups, s, a);
   });
 }
 
