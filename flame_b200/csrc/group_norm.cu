@@ -58,13 +58,33 @@ __device__ __forceinline__ float param(const void* p, int f32, uint32_t c, float
   if (!p) return none;
   return f32 ? static_cast<const float*>(p)[c] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c]);
 }
-// 1 / (1 + exp(-h)) on the special-function unit: a few units in the last place of binary32, far below the rounding to BF16.  The
-// flush-to-zero forms skip the scaling of sub-normal arguments, which 1 + exp(-h) and its reciprocal have no use for.
-__device__ __forceinline__ float sigmoid(float h) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h * -1.442695041f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return r;
+// Two binary32 numbers in one register pair: additions and multiply-adds take one instruction for both.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() = default;
+  __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ float2 get() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+};
+__device__ __forceinline__ F2 add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 mul(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+
+// 1 / (1 + exp(-h)) of two numbers on the special-function unit, which is what bounds the kernels next to memory (16 results a cycle
+// and SM): two exponentials and one reciprocal, of the product, from which each takes its own.  The exponentials end at 2^60, so
+// that the product stays finite: under h = -41 the result stays at 2^-60.  A NaN counts as 60 there: it would make its neighbour NaN,
+// which may belong to another group, and comes back by the factor h that every use has.  Errors are a few units in the last place of binary32, far below the rounding to BF16.
+__device__ __forceinline__ F2 sigmoid(F2 h) {
+  const float2 t = mul(h, F2(-1.442695041f, -1.442695041f)).get();
+  float e0, e1, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(t.x, 60.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(t.y, 60.0f)));
+  const float2 a = add(F2(e0, e1), F2(1.0f, 1.0f)).get();
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a.x * a.y));
+  return mul(F2(r, r), F2(a.y, a.x));
 }
 // The group of channel c: c / cg by a multiplication, exact for c and cg up to 65,536 (by_cg = ceil(2^32 / cg), 0 for cg = 1).
 // Eight divisions a thread took longer than the sums themselves at 64 x 64 positions.
@@ -77,21 +97,40 @@ struct alignas(16) Vec<8> { __nv_bfloat16 v[8]; };
 template <>
 struct alignas(4) Vec<2> { __nv_bfloat16 v[2]; };
 
+// Pairs of neighbouring channels; with one channel the pair's other half is 0.
 template <int V>
-__device__ __forceinline__ void unpack(const Vec<V>& r, float (&f)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = __bfloat162float(r.v[i]);
-}
+constexpr int kPairs = (V + 1) / 2;
 template <int V>
-__device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[V], int stream) {
-  Vec<V> r;
+__device__ __forceinline__ void unpack(const Vec<V>& r, F2 (&f)[kPairs<V>]) {
+  if constexpr (V == 1) {
+    f[0] = F2(__bfloat162float(r.v[0]), 0.0f);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = __float2bfloat16_rn(f[i]);
-  if constexpr (V == 8) {
-    if (stream) { __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&r)); return; }
+    for (int i = 0; i < V / 2; ++i) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(&r)[i];
+      f[i] = F2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
   }
-  *reinterpret_cast<Vec<V>*>(p) = r;
 }
+__device__ __forceinline__ uint32_t to_bf16x2(F2 f) {
+  const float2 u = f.get();
+  uint32_t w;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(u.y), "f"(u.x));
+  return w;
+}
+template <int V>
+__device__ __forceinline__ void store(__nv_bfloat16* p, const F2 (&f)[kPairs<V>], int stream) {
+  if constexpr (V == 8) {
+    const uint4 w = make_uint4(to_bf16x2(f[0]), to_bf16x2(f[1]), to_bf16x2(f[2]), to_bf16x2(f[3]));
+    if (stream) __stcs(reinterpret_cast<uint4*>(p), w);
+    else *reinterpret_cast<uint4*>(p) = w;
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<uint32_t*>(p) = to_bf16x2(f[0]);
+  } else {
+    *p = __float2bfloat16_rn(f[0].get().x);
+  }
+}
+
 // A thread's way down its rows, kN tensors at a time; kBack: from the last row to the first.  The constructor sends the first rows on
 // their way, run(f) calls f(offset, vectors, live) for each row, offset in elements from the thread's first row; with kWhole also,
 // with live = false, where another thread of the block has a row and this one has none (for shuffles inside f).
@@ -103,56 +142,64 @@ constexpr int kDepth = 8;
 constexpr size_t kRingBytes = (size_t)kDepth * kThreads * 16;
 template <int kN, int V, bool kBack, bool kWhole>
 struct Walk {
-  static constexpr int kD = kDepth / kN;      // rows on their way
+  static constexpr int kD = V == 8 ? kDepth / kN : 1;      // rows on their way
   const __nv_bfloat16* const (&src)[kN];
   uint4* ring;
-  uint32_t mine, most, skip, in, sent;
+  uint32_t mine, most, skip, at_shared;
   ptrdiff_t step, first, next;
 
-  __device__ __forceinline__ void send() {
-    if (sent < most && (!kWhole || (kBack ? sent >= skip : sent < mine))) {
-      const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring + threadIdx.x);
+  // the row of round n, into place j of the ring
+  __device__ __forceinline__ void send(uint32_t n, int j) {
+    if (n < most && (!kWhole || (kBack ? n >= skip : n < mine))) {
 #pragma unroll
       for (int k = 0; k < kN; ++k)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + (in * kN + k) * kThreads * 16), "l"(src[k] + next) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at_shared + (j * kN + k) * kThreads * 16), "l"(src[k] + next) : "memory");
     }
-    ++sent;
     next += step;
-    in = in + 1 == kD ? 0 : in + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  __device__ __forceinline__ Walk(const __nv_bfloat16* const (&s)[kN], uint32_t rows, uint32_t lane_row, uint32_t row_step, uint32_t C, uint4* r)
-      : src(s), ring(r), in(0), sent(0) {
+  __device__ __forceinline__ Walk(const __nv_bfloat16* const (&s)[kN], uint32_t rows, uint32_t lane_row, uint32_t row_step, uint32_t C, uint4* r) : src(s), ring(r) {
     mine = rows > lane_row ? (rows - lane_row + row_step - 1) / row_step : 0;
     most = kWhole ? (rows + row_step - 1) / row_step : mine;
     step = (kBack ? -1 : 1) * (ptrdiff_t)((size_t)row_step * C);
     first = next = kBack ? -step * ((ptrdiff_t)most - 1) : 0;
     skip = kBack ? most - mine : 0;      // rounds before this thread's first row, from the back
+    at_shared = (uint32_t)__cvta_generic_to_shared(ring + threadIdx.x);
     if constexpr (V == 8) {
 #pragma unroll
-      for (int n = 0; n < kD; ++n) send();
+      for (int j = 0; j < kD; ++j) send(j, j);
     }
   }
   template <typename F>
   __device__ __forceinline__ void run(F&& f) {
     ptrdiff_t at = first;
-    uint32_t out = 0;
-    for (uint32_t n = 0; n < most; ++n, at += step) {
-      Vec<V> v[kN];
-      const bool live = !kWhole || (kBack ? n >= skip : n < mine);
-      if constexpr (V == 8) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kD - 1) : "memory");
+    if constexpr (V == 8) {
+      for (uint32_t n0 = 0; n0 < most; n0 += kD) {
+#pragma unroll
+        for (int j = 0; j < kD; ++j) {      // a turn of the ring
+          if (n0 + j >= most) break;
+          asm volatile("cp.async.wait_group %0;" ::"n"(kD - 1) : "memory");
+          Vec<V> v[kN];
+          const bool live = !kWhole || (kBack ? n0 + j >= skip : n0 + j < mine);
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < kN; ++k) { const uint4 w = ring[(j * kN + k) * kThreads + threadIdx.x]; v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
+          }
+          f(at, v, live);
+          at += step;
+          send(n0 + j + kD, j);
+        }
+      }
+    } else {
+      for (uint32_t n = 0; n < most; ++n, at += step) {
+        Vec<V> v[kN];
+        const bool live = !kWhole || (kBack ? n >= skip : n < mine);
         if (live) {
 #pragma unroll
-          for (int k = 0; k < kN; ++k) { const uint4 w = ring[(out * kN + k) * kThreads + threadIdx.x]; v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
+          for (int k = 0; k < kN; ++k) v[k] = *reinterpret_cast<const Vec<V>*>(src[k] + at);
         }
-        out = out + 1 == kD ? 0 : out + 1;
-      } else if (live) {
-#pragma unroll
-        for (int k = 0; k < kN; ++k) v[k] = *reinterpret_cast<const Vec<V>*>(src[k] + at);
+        f(at, v, live);
       }
-      f(at, v, live);
-      if constexpr (V == 8) send();
     }
   }
 };
@@ -224,11 +271,14 @@ struct Place {
 template <int V>
 __device__ __forceinline__ uint32_t place_of(uint32_t c, uint32_t width) { return c % V * (width / V) + c / V; }
 template <int V>
-__device__ __forceinline__ void join_rows(const Place<V>& p, const float (&s)[V], const float (&q)[V], float2* sh, uint32_t width) {
+__device__ __forceinline__ void join_rows(const Place<V>& p, const F2 (&s)[kPairs<V>], const F2 (&q)[kPairs<V>], float2* sh, uint32_t width) {
   // sh holds row_step x width pairs; width = channels of the slab
   if (p.live) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) sh[p.lane_row * width + i * (width / V) + p.vec] = make_float2(s[i], q[i]);
+    for (int i = 0; i < V; ++i) {
+      const float2 si = s[i / 2].get(), qi = q[i / 2].get();
+      sh[p.lane_row * width + i * (width / V) + p.vec] = i % 2 ? make_float2(si.y, qi.y) : make_float2(si.x, qi.x);
+    }
   }
   __syncthreads();
   for (uint32_t c = threadIdx.x; c < width; c += kThreads) {
@@ -321,20 +371,25 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
   const __nv_bfloat16* xs = a.x + (size_t)p.b * a.L * a.C;
   const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
   Walk<1, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
-  float shift[V], s[V], q[V];
+  F2 shift[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the shift's negative
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    s[i] = q[i] = 0.0f;
-    shift[i] = p.live ? __bfloat162float(xs[group_of(p.c0 + i, a.by_cg) * a.cg]) : 0.0f;
+  for (int i = 0; i < kPairs<V>; ++i) {
+    s[i] = q[i] = F2(0.0f, 0.0f);
+    float2 t = make_float2(0.0f, 0.0f);
+    if (p.live) {
+      t.x = -__bfloat162float(xs[group_of(p.c0 + 2 * i, a.by_cg) * a.cg]);
+      if (V > 1) t.y = -__bfloat162float(xs[group_of(p.c0 + 2 * i + 1, a.by_cg) * a.cg]);
+    }
+    shift[i] = F2(t.x, t.y);
   }
   way.run([&](ptrdiff_t, const Vec<V>(&v)[1], bool) {
-    float f[V];
+    F2 f[kPairs<V>];
     unpack<V>(v[0], f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float d = f[i] - shift[i];
-      s[i] += d;
-      q[i] = fmaf(d, d, q[i]);
+    for (int i = 0; i < kPairs<V>; ++i) {
+      const F2 d = add(f[i], shift[i]);
+      s[i] = add(s[i], d);
+      q[i] = fma(d, d, q[i]);
     }
   });
   const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
@@ -355,15 +410,33 @@ __device__ __forceinline__ void finish_stats(const NormArgs& a, uint32_t b, floa
   });
 }
 
-// Codes of V = 8 channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
-__device__ __forceinline__ uint2 encode_row_block(const float (&y)[8], float& scale) {
-  float amax = 0.0f;
+// Codes of eight channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
+__device__ __forceinline__ uint2 encode_row_block(const uint4& raw, float& scale) {
+  uint32_t m = max_abs2(max_abs2(raw.x, raw.y), max_abs2(raw.z, raw.w));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));   // a NaN is ignored
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-  scale = fp8_scale_of(amax);
+  for (int d = 8; d > 0; d >>= 1) m = max_abs2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  scale = fp8_scale_of(larger_of(m));
+  float y[8];
+  unpack8(raw, y);
   return fp8_encode8(y, scale, fp8_factor_of(scale));
+}
+
+// Bias of a thread's channels, and whatever f makes of the weight and the group's statistics of each.
+template <int V, typename F>
+__device__ __forceinline__ void load_params(const NormArgs& a, const Place<V>& p, F2 (&bias)[kPairs<V>], F&& f, const float2* stats, F2 (&u)[kPairs<V>], F2 (&v)[kPairs<V>]) {
+  float w[2 * kPairs<V>] = {}, b[2 * kPairs<V>] = {}, fu[2 * kPairs<V>] = {}, fv[2 * kPairs<V>] = {};
+  if (p.live) {
+    params<V>(a.weight, a.params_f32, p.c0, 1.0f, reinterpret_cast<float(&)[V]>(w));
+    params<V>(a.bias, a.params_f32, p.c0, 0.0f, reinterpret_cast<float(&)[V]>(b));
+#pragma unroll
+    for (int i = 0; i < V; ++i) f(i, w[i], stats[group_of(p.c0 + i, a.by_cg)], fu[i], fv[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    bias[i] = F2(b[2 * i], b[2 * i + 1]);
+    u[i] = F2(fu[2 * i], fu[2 * i + 1]);
+    v[i] = F2(fv[2 * i], fv[2 * i + 1]);
+  }
 }
 
 template <int V, bool kCodes>
@@ -380,35 +453,24 @@ __global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(c
   finish_stats(a, p.b, sh);
   if (p.chunk == 0 && p.slab == 0)
     for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) reinterpret_cast<float2*>(a.stats)[(size_t)p.b * a.G + g] = sh[g];
-  float mean[V], scale[V], bias[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) mean[i] = scale[i] = bias[i] = 0.0f;
-  if (p.live) {
-    params<V>(a.weight, a.params_f32, p.c0, 1.0f, scale);
-    params<V>(a.bias, a.params_f32, p.c0, 0.0f, bias);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 t = sh[group_of(p.c0 + i, a.by_cg)];
-      mean[i] = t.x;
-      scale[i] *= t.y;
-    }
-  }
+  F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>];      // the mean's negative
+  load_params<V>(a, p, bias, [&](int i, float w, float2 t, float& m, float& s) { m = -t.x; s = t.y * w; }, sh, mean, scale);
   way.run([&](ptrdiff_t at, const Vec<V>(&v)[1], bool live) {
-    float f[V];
+    F2 f[kPairs<V>];
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = 0.0f;
+    for (int i = 0; i < kPairs<V>; ++i) f[i] = F2(0.0f, 0.0f);
     if (live) unpack<V>(v[0], f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float h = fmaf(f[i] - mean[i], scale[i], bias[i]);      // first the difference: a group of equal values gives exactly the bias
-      f[i] = a.silu ? h * sigmoid(h) : h;
+    for (int i = 0; i < kPairs<V>; ++i) {
+      const F2 h = fma(add(f[i], mean[i]), scale[i], bias[i]);      // first the difference: a group of equal values gives exactly the bias
+      f[i] = a.silu ? mul(h, sigmoid(h)) : h;
     }
     if (live) store<V>(a.y + first + at, f, a.stream);
     if constexpr (kCodes) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = live ? __bfloat162float(__float2bfloat16_rn(f[i])) : 0.0f;   // the codes are those of the BF16 output
+      // the codes are those of the BF16 output
+      const uint4 raw = live ? make_uint4(to_bf16x2(f[0]), to_bf16x2(f[1]), to_bf16x2(f[2]), to_bf16x2(f[3])) : make_uint4(0u, 0u, 0u, 0u);
       float s;
-      const uint2 c = encode_row_block(f, s);
+      const uint2 c = encode_row_block(raw, s);
       if (live) {
         *reinterpret_cast<uint2*>(a.codes + first + at) = c;
         if ((p.vec & 15) == 0) a.code_scales[(first + at) / 128] = s;
@@ -418,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(c
 }
 
 // dy * act'(h)
-__device__ __forceinline__ float grad_h(float h, float dy, int silu) {
+__device__ __forceinline__ F2 grad_h(F2 h, F2 dy, int silu) {
   if (!silu) return dy;
-  const float g = sigmoid(h);
-  return dy * (g * fmaf(h, 1.0f - g, 1.0f));
+  const F2 g = sigmoid(h), one(1.0f, 1.0f), minus(-1.0f, -1.0f);
+  return mul(dy, mul(g, fma(h, fma(g, minus, one), one)));
 }
 
 template <int V>
@@ -434,31 +496,25 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
   const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
   const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
   Walk<2, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
-  float mean[V], scale[V], bias[V], s[V], q[V];
+  F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the mean's negative
+  load_params<V>(a, p, bias, [&](int, float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, stats, mean, scale);
 #pragma unroll
-  for (int i = 0; i < V; ++i) s[i] = q[i] = 0.0f;
-  if (p.live) {
-    params<V>(a.weight, a.params_f32, p.c0, 1.0f, scale);
-    params<V>(a.bias, a.params_f32, p.c0, 0.0f, bias);
+  for (int i = 0; i < kPairs<V>; ++i) s[i] = q[i] = F2(0.0f, 0.0f);
+  way.run([&](ptrdiff_t, const Vec<V>(&v)[2], bool) {
+    F2 x[kPairs<V>], dy[kPairs<V>];
+    unpack<V>(v[0], x);
+    unpack<V>(v[1], dy);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 t = stats[group_of(p.c0 + i, a.by_cg)];
-      mean[i] = t.x;
-      scale[i] *= t.y;
+    for (int i = 0; i < kPairs<V>; ++i) {
+      const F2 d = add(x[i], mean[i]), dh = grad_h(fma(d, scale[i], bias[i]), dy[i], a.silu);
+      s[i] = add(s[i], dh);
+      q[i] = fma(dh, d, q[i]);      // times rstd at the end
     }
-    way.run([&](ptrdiff_t, const Vec<V>(&v)[2], bool) {
-      float x[V], dy[V];
-      unpack<V>(v[0], x);
-      unpack<V>(v[1], dy);
+  });
+  if (p.live) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = x[i] - mean[i], dh = grad_h(fmaf(d, scale[i], bias[i]), dy[i], a.silu);
-        s[i] += dh;
-        q[i] = fmaf(dh, d, q[i]);      // times rstd at the end
-      }
-    });
-#pragma unroll
-    for (int i = 0; i < V; ++i) q[i] *= stats[group_of(p.c0 + i, a.by_cg)].y;
+    for (int i = 0; i < kPairs<V>; ++i)
+      q[i] = mul(q[i], F2(stats[group_of(p.c0 + 2 * i, a.by_cg)].y, V > 1 ? stats[group_of(p.c0 + 2 * i + 1, a.by_cg)].y : 0.0f));
   }
   const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
   const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
@@ -519,28 +575,31 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
   join_parts(a, p.b, [&](uint32_t g, float s, float q) { sh[g] = make_float2(s * inv_n, q * inv_n); });
   // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
-  float scale[V], offset[V], slope[V], rest[V];
-  if (p.live) {
-    params<V>(a.weight, a.params_f32, p.c0, 1.0f, scale);
-    params<V>(a.bias, a.params_f32, p.c0, 0.0f, offset);
+  F2 scale[kPairs<V>], offset[kPairs<V>], slope[kPairs<V>], rest[kPairs<V>], mean[kPairs<V>];
+  load_params<V>(a, p, offset, [&](int, float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, stats, mean, scale);
+  if (!p.live) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint32_t g = group_of(p.c0 + i, a.by_cg);
+  for (int i = 0; i < kPairs<V>; ++i) {
+    offset[i] = fma(mean[i], scale[i], offset[i]);
+    float sl[2] = {}, re[2] = {};
+#pragma unroll
+    for (int k = 0; k < 2 && 2 * i + k < V; ++k) {
+      const uint32_t g = group_of(p.c0 + 2 * i + k, a.by_cg);
       const float2 t = stats[g], m = sh[g];
-      scale[i] *= t.y;
-      offset[i] = fmaf(-t.x, scale[i], offset[i]);
-      slope[i] = -t.y * t.y * m.y;
-      rest[i] = fmaf(-t.x, slope[i], -t.y * m.x);
+      sl[k] = -t.y * t.y * m.y;
+      re[k] = fmaf(-t.x, sl[k], -t.y * m.x);
     }
+    slope[i] = F2(sl[0], sl[1]);
+    rest[i] = F2(re[0], re[1]);
   }
   way.run([&](ptrdiff_t at, const Vec<V>(&v)[2], bool) {
-    float x[V], dy[V];
+    F2 x[kPairs<V>], dy[kPairs<V>];
     unpack<V>(v[0], x);
     unpack<V>(v[1], dy);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float dh = grad_h(fmaf(x[i], scale[i], offset[i]), dy[i], a.silu);
-      x[i] = fmaf(scale[i], dh, fmaf(slope[i], x[i], rest[i]));
+    for (int i = 0; i < kPairs<V>; ++i) {
+      const F2 dh = grad_h(fma(x[i], scale[i], offset[i]), dy[i], a.silu);
+      x[i] = fma(scale[i], dh, fma(slope[i], x[i], rest[i]));
     }
     store<V>(a.y + first + at, x, a.stream);
   });
