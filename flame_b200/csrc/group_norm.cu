@@ -9,8 +9,9 @@
 // positions of its chunk, so that a warp reads whole lines of the channels-last rows, and per-channel sums stay in registers.
 // The forward sums are kept about a shift, the group's first element in the sample: x - shift is of the size of the spread and not of
 // the mean, so that sums of squares lose nothing when the mean is large against the spread.  A cluster of thread blocks adds its sums
-// up through distributed shared memory, which leaves the second launch an eighth of them to read.  Everything is added in a fixed
-// order, without atomics: the same inputs give the same bits.
+// up through distributed shared memory, which leaves the second launch a quarter of them to read; where there are many, a launch
+// of one block a sample adds them up in between.  Everything is added in a fixed order, without atomics: the same inputs give the
+// same bits.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -40,6 +41,7 @@ struct NormArgs {
   float* stats;                  // [B, G, 2]: mean, rstd
   float2* partial;               // [B, parts, G]: forward sums of x - shift and of its square, backward s1 and s2
   float2* channel_partial;       // backward: [B, parts, C]: sums for dbias and dweight
+  float2* finished;              // NULL, or [B, G]: what the launch between the two made of the parts
   void* dweight;                 // backward, may be NULL
   void* dbias;
   uint32_t B, C, G, cg, by_cg;
@@ -61,7 +63,7 @@ __device__ __forceinline__ float param(const void* p, int f32, uint32_t c, float
 // Two binary32 numbers in one register pair: additions and multiply-adds take one instruction for both.
 struct F2 {
   uint64_t v;
-  __device__ __forceinline__ F2() = default;
+  F2() = default;
   __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
   __device__ __forceinline__ float2 get() const {
     float2 r;
@@ -249,8 +251,9 @@ struct Place {
   uint64_t row0;
   uint32_t rows;
   bool live;
-  __device__ __forceinline__ explicit Place(const NormArgs& a) {
-    chunk = blockIdx.x;
+  // back: the last chunk first, which the launch before has read last
+  __device__ __forceinline__ explicit Place(const NormArgs& a, bool back = false) {
+    chunk = back ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
     slab = blockIdx.y;
     b = blockIdx.z;
     const uint32_t nvec = a.C / V, first = slab * a.slab_vecs;
@@ -400,14 +403,41 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
   join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G, [](uint32_t i) { return i; });
 }
 
-// (mean, rstd) of every group of sample b
-__device__ __forceinline__ void finish_stats(const NormArgs& a, uint32_t b, float2* stats) {
+// What the second launch needs of a group's sums: mean and rstd, or backward the means of s1 and s2.
+template <bool kBackward>
+__device__ __forceinline__ float2 finish(const NormArgs& a, uint32_t b, uint32_t g, float s, float q) {
   const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
-  join_parts(a, b, [&](uint32_t g, float s, float q) {
-    const float off = s * inv_n, var = fmaxf(q * inv_n - off * off, 0.0f);
-    // fmaxf would turn the NaN of a group with a NaN or an infinity into 0
-    stats[g] = make_float2(__bfloat162float(a.x[(size_t)b * a.L * a.C + g * a.cg]) + off, q == q && q < INFINITY ? rsqrtf(var + a.eps) : NAN);
-  });
+  if (kBackward) return make_float2(s * inv_n, q * inv_n);
+  const float off = s * inv_n, var = fmaxf(q * inv_n - off * off, 0.0f);
+  // fmaxf would turn the NaN of a group with a NaN or an infinity into 0
+  return make_float2(__bfloat162float(a.x[(size_t)b * a.L * a.C + g * a.cg]) + off, q == q && q < INFINITY ? rsqrtf(var + a.eps) : NAN);
+}
+template <bool kBackward>
+__device__ __forceinline__ void finish_all(const NormArgs& a, uint32_t b, float2* out) {
+  if (a.finished) {
+    for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) out[g] = a.finished[(size_t)b * a.G + g];
+    __syncthreads();
+  } else {
+    join_parts(a, b, [&](uint32_t g, float s, float q) { out[g] = finish<kBackward>(a, b, g, s, q); });
+  }
+}
+// A warp for each group of sample blockIdx.y.
+template <bool kBackward>
+__global__ void __launch_bounds__(kThreads) group_finish_kernel(const __grid_constant__ NormArgs a) {
+  pdl_prologue();
+  const uint32_t g = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y;
+  if (g >= a.G) return;
+  const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
+  float s = 0.0f, q = 0.0f;
+#pragma unroll 4
+  for (uint32_t i = lane; i < a.parts; i += 32) {
+    const float2 t = in[(size_t)i * a.G];
+    s += t.x;
+    q += t.y;
+  }
+  s = warp_sum(s);
+  q = warp_sum(q);
+  if (lane == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, b, g, s, q);
 }
 
 // Codes of eight channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
@@ -444,14 +474,14 @@ __global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(c
   pdl_prologue();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
-  const Place<V> p(a);
+  const Place<V> p(a, true);
   // From the chunk's end to its start: what the first launch read last is still in L2.
   // With codes, 16 neighbouring lanes share a row (C / 8 and the slab's width are multiples of 16): all of them are live or none is.
   const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
   const __nv_bfloat16* const src[1] = {a.x + first};
   Walk<1, V, true, kCodes> way(src, kCodes || p.live ? p.rows : 0, p.live ? p.lane_row : 0xFFFFFFFFu, p.row_step, a.C, ring);
-  finish_stats(a, p.b, sh);
-  if (p.chunk == 0 && p.slab == 0)
+  finish_all<false>(a, p.b, sh);
+  if (p.chunk == 0 && p.slab == 0 && a.finished == nullptr)
     for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) reinterpret_cast<float2*>(a.stats)[(size_t)p.b * a.G + g] = sh[g];
   F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>];      // the mean's negative
   load_params<V>(a, p, bias, [&](int i, float w, float2 t, float& m, float& s) { m = -t.x; s = t.y * w; }, sh, mean, scale);
@@ -567,12 +597,11 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
     }
     return;
   }
-  const Place<V> p(a);
+  const Place<V> p(a, true);
   const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
   const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
   Walk<2, V, true, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);      // from the chunk's end, as in the forward pass
-  const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
-  join_parts(a, p.b, [&](uint32_t g, float s, float q) { sh[g] = make_float2(s * inv_n, q * inv_n); });
+  finish_all<true>(a, p.b, sh);
   // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
   F2 scale[kPairs<V>], offset[kPairs<V>], slope[kPairs<V>], rest[kPairs<V>], mean[kPairs<V>];
@@ -624,14 +653,15 @@ Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, boo
   p.slabs = (nvec + kThreads - 1) / kThreads;
   // with slabs, a width that is a multiple of 16 vectors: a block of 128 channels lies in one slab
   p.slab_vecs = p.slabs == 1 ? nvec : kThreads;
-  // all the thread blocks that fit on the SMs at a time, and a few rows for each thread
-  uint64_t want = (uint64_t)sms * (backward ? 3 : 4) / ((uint64_t)B * p.slabs);
-  if (want < 1) want = 1;
+  // All the thread blocks that fit on the SMs at a time, with eight rows a thread at least.  Where each would have over 64, four times
+  // as many: SMs differ in speed, and with one block for each place the slowest is waited for (1024 x 1024 x 128).
+  const uint64_t places = (uint64_t)sms * (backward ? 3 : 4), samples = (uint64_t)B * p.slabs;
+  uint64_t want = places / samples > 1 ? places / samples : 1;
   const uint32_t row_step = kThreads / p.slab_vecs;
-  uint64_t most = (L + (uint64_t)row_step * 8 - 1) / ((uint64_t)row_step * 8);
-  if (most < 1) most = 1;
+  if (L / (want * row_step) > 64) want = 4 * places / samples > 1 ? 4 * places / samples : 1;
+  const uint64_t most = (L + (uint64_t)row_step * 8 - 1) / ((uint64_t)row_step * 8);
   uint64_t chunks = want < most ? want : most;
-  if (chunks > 1024) chunks = 1024;
+  if (chunks > 4096) chunks = 4096;
   chunks = chunks < kCluster ? kCluster : chunks / kCluster * kCluster;
   p.rows_per_chunk = (L + chunks - 1) / chunks;
   chunks = (L + p.rows_per_chunk - 1) / p.rows_per_chunk;
@@ -639,9 +669,11 @@ Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, boo
   p.parts = p.chunks / kCluster * p.slabs;
   return p;
 }
+// Over 64 parts the blocks of the second launch would spend longer on adding them up than a launch takes.
+bool finishes(const Plan& p) { return p.parts > 64; }
 size_t group_pairs(const Plan& p, uint32_t B, uint32_t G) { return ((size_t)B * p.parts * G + 1) / 2 * 2; }   // whole 16 bytes
 size_t partial_pairs(const Plan& p, uint32_t B, uint32_t C, uint32_t G, bool backward) {
-  return group_pairs(p, B, G) + (backward ? (size_t)B * (p.chunks / kCluster) * C : 0);
+  return group_pairs(p, B, G) + (backward ? (size_t)B * (p.chunks / kCluster) * C : 0) + (finishes(p) && backward ? (size_t)B * G : 0);
 }
 bool al(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -730,6 +762,7 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   a.x = static_cast<const __nv_bfloat16*>(x); a.weight = weight; a.bias = bias; a.y = static_cast<__nv_bfloat16*>(y);
   a.codes = static_cast<uint8_t*>(codes); a.code_scales = static_cast<float*>(code_scales); a.stats = static_cast<float*>(stats);
   a.partial = static_cast<float2*>(workspace);
+  if (finishes(p)) a.finished = reinterpret_cast<float2*>(a.stats);
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
   a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
   a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
@@ -740,6 +773,8 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
     cudaError_t e = launch(group_stats_kernel<V>, grid, true, sums, s, a);
+    if (e != cudaSuccess) return e;
+    if (a.finished) e = launch(group_finish_kernel<false>, dim3((a.G + kWarps - 1) / kWarps, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
     if constexpr (V == 8) {
       if (a.codes) return launch(group_apply_kernel<8, true>, grid, false, groups, s, a);
@@ -770,6 +805,7 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   a.y = static_cast<__nv_bfloat16*>(dx); a.stats = const_cast<float*>(static_cast<const float*>(stats));
   a.partial = static_cast<float2*>(workspace);
   a.channel_partial = a.partial + group_pairs(p, (uint32_t)B, (uint32_t)G);
+  if (finishes(p)) a.finished = a.channel_partial + (size_t)B * (p.chunks / kCluster) * C;
   a.dweight = dweight; a.dbias = dbias;
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
   a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
@@ -780,7 +816,9 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    const cudaError_t e = launch(group_grad_sums_kernel<V>, grid, true, sums, s, a);
+    cudaError_t e = launch(group_grad_sums_kernel<V>, grid, true, sums, s, a);
+    if (e != cudaSuccess) return e;
+    if (a.finished) e = launch(group_finish_kernel<true>, dim3((a.G + kWarps - 1) / kWarps, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
     return launch(group_grad_apply_kernel<V>, more, false, groups, s, a);
   });
