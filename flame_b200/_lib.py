@@ -158,7 +158,7 @@ SIGNATURES = {
     "flame_fp8_product": (_i, [_vp, _sz, _vp, _i, _vp, _sz, _vp, _i, _i, _vp, _sz, _i, _sz, _sz, _sz, _vp]),
     "flame_fp8_linear_workspace_bytes": (_sz, [_sz, _sz, _sz, _i]),
     "flame_fp8_linear": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _i, _vp, _sz, _sz, _sz, _vp, _sz, _vp]),
-    "flame_fp8_linear_backward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp]),
+    "flame_fp8_linear_backward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp]),
     "flame_fp8_product_faults": (_i, [C.POINTER(_u)]),
     "flame_group_norm_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _i]),
     "flame_group_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _f, _i, _i, _vp, _sz, _vp]),

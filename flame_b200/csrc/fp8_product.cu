@@ -43,17 +43,17 @@ struct QuantJob {
   uint32_t tiles;
   uint32_t mode;
 };
-// Up to two matrices in a launch: a layer's input and weight, or its output gradient and input.
-struct QuantJobs { QuantJob job[2]; };
+// Up to three matrices in a launch: a layer's output gradient, input and weight.
+struct QuantJobs { QuantJob job[3]; };
 
 __global__ void __launch_bounds__(kQuantThreads, 4) fp8_quant_kernel(const __grid_constant__ QuantJobs jobs) {
   pdl_prologue();
   __shared__ uint32_t part[8][kBlock / 2];       // packed maxima of two columns
   __shared__ __align__(16) float factors[kBlock];
   __shared__ __align__(16) float scales[kBlock];
-  const bool second = blockIdx.x >= jobs.job[0].tiles;
-  const QuantJob& a = jobs.job[second];
-  const uint32_t tile = blockIdx.x - (second ? jobs.job[0].tiles : 0);
+  uint32_t tile = blockIdx.x, which = 0;
+  while (which < 2 && tile >= jobs.job[which].tiles) tile -= jobs.job[which++].tiles;
+  const QuantJob& a = jobs.job[which];
   const uint32_t tm = tile / a.tiles_across, tn = tile - tm * a.tiles_across;
   const uint32_t t = threadIdx.x, lr = t >> 4, lc = t & 15;
   const uint32_t row0 = tm * kBlock + lr, col = tn * kBlock + lc * 8;
@@ -865,7 +865,8 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 uint64_t blocks_of(uint64_t n) { return (n + kBlock - 1) / kBlock; }
 // codes and, on the next 256 bytes, scales
 size_t codes_bytes(size_t rows, size_t cols, uint32_t mode) {
-  return up256(rows * up16(cols)) + up256((mode == kQuantColumns ? blocks_of(rows) * cols : rows * blocks_of(cols)) * sizeof(float));
+  const size_t scales = mode == kQuantColumns ? blocks_of(rows) * cols : mode == kQuantTiles ? blocks_of(rows) * blocks_of(cols) : rows * blocks_of(cols);
+  return up256(rows * up16(cols)) + up256(scales * sizeof(float));
 }
 
 // What is wrong with a BF16 matrix as a source of codes; NULL: nothing.
@@ -887,11 +888,16 @@ QuantJob quant_job(const void* x, size_t rows, size_t cols, size_t x_stride, uin
   a.mode = mode | (al(x, 16) && x_stride % 8 == 0 && cols % 8 == 0 ? kQuantWide : 0u);
   return a;
 }
-cudaError_t launch_quant(const QuantJob& a, const QuantJob& b, cudaStream_t stream) {
-  QuantJobs jobs;
-  jobs.job[0] = a;
-  jobs.job[1] = b;
-  return launch_after(fp8_quant_kernel, a.tiles + b.tiles, kQuantThreads, 0, stream, jobs);
+cudaError_t launch_quant(const QuantJobs& jobs, cudaStream_t stream) {
+  const uint64_t tiles = (uint64_t)jobs.job[0].tiles + jobs.job[1].tiles + jobs.job[2].tiles;
+  return tiles == 0 ? cudaSuccess : launch_after(fp8_quant_kernel, (unsigned)tiles, kQuantThreads, 0, stream, jobs);
+}
+// Where a matrix's codes and scales lie in a workspace; moves `at` on.
+struct Place { uint8_t *codes, *scales; };
+Place take(uint8_t*& at, size_t rows, size_t cols, uint32_t mode) {
+  const Place p = {at, at + up256(rows * up16(cols))};
+  at += codes_bytes(rows, cols, mode);
+  return p;
 }
 
 enum class Product { kNtTiles, kNtRows, kNnTiles, kTnColumns };
@@ -936,7 +942,9 @@ int flame_fp8_quant_2d(const void* x, size_t rows, size_t cols, size_t x_stride,
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
   const QuantJob a = quant_job(x, rows, cols, x_stride, (tile ? kQuantTiles : 0u) | (row ? kQuantRows : 0u) | (col ? kQuantColumns : 0u), codes, scales,
                                column_codes, column_scales, code_stride);
-  return (int)launch_quant(a, QuantJob{}, (cudaStream_t)stream);
+  QuantJobs jobs = {};
+  jobs.job[0] = a;
+  return (int)launch_quant(jobs, (cudaStream_t)stream);
 }
 
 int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scales, int blocks, void* out, int out_dtype, size_t rows,
@@ -982,73 +990,91 @@ int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales
   return (int)product(kind, a_codes, a_stride, a_scales, b_codes, b_stride, b_scales, c, c_stride, c_dtype == FLAME_OFFLOAD_DTYPE_F32, M, N, K, (cudaStream_t)stream);
 }
 
-size_t flame_fp8_linear_workspace_bytes(size_t M, size_t N, size_t K, int backward) {
+size_t flame_fp8_linear_workspace_bytes(size_t M, size_t N, size_t K, int flags) {
   if (M > kMostSize || N > kMostSize || K > kMostSize) return 0;
-  return backward ? codes_bytes(M, N, kQuantRows) + codes_bytes(M, N, kQuantColumns) + codes_bytes(M, K, kQuantColumns) : codes_bytes(M, K, kQuantRows);
+  const size_t w = (flags & FLAME_FP8_LINEAR_BF16_WEIGHT) ? codes_bytes(N, K, kQuantTiles) : 0;
+  if (!(flags & FLAME_FP8_LINEAR_BACKWARD)) return codes_bytes(M, K, kQuantRows) + w;
+  return codes_bytes(M, N, kQuantRows) + codes_bytes(M, N, kQuantColumns) + codes_bytes(M, K, kQuantColumns) + w;
 }
 
 int flame_fp8_linear(const void* x, size_t x_stride, const void* x_codes, size_t x_code_stride, const void* x_scales, const void* w,
-                     size_t w_stride, void* w_codes, size_t w_code_stride, void* w_scales, int w_blocks, void* y, size_t M, size_t N,
-                     size_t K, void* workspace, size_t workspace_bytes, void* stream) {
+                     size_t w_stride, const void* w_codes, size_t w_code_stride, const void* w_scales, int w_blocks, void* y, size_t M,
+                     size_t N, size_t K, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "flame_fp8_linear";
-  if (w_blocks != FLAME_FP8_BLOCKS_TILES && (w_blocks != FLAME_FP8_BLOCKS_ROWS || w)) return refuse(who, "the blocks of a weight are tiles, or rows where it is given as codes");
-  if (!x_codes)
-    if (const char* what = quant_source(x, M, K, x_stride)) return refuse(who, what);
-  if (w)
-    if (const char* what = quant_source(w, N, K, w_stride)) return refuse(who, what);
+  if (!w && w_blocks != FLAME_FP8_BLOCKS_TILES && w_blocks != FLAME_FP8_BLOCKS_ROWS) return refuse(who, "the blocks of a weight are tiles or rows");
+  if (const char* what = x_codes ? nullptr : quant_source(x, M, K, x_stride)) return refuse(who, what);
+  if (const char* what = w ? quant_source(w, N, K, w_stride) : nullptr) return refuse(who, what);
   if (M > kMostSize || N > kMostSize || K > kMostSize) return refuse(who, "matrix too large");
-  if (w_code_stride < K || w_code_stride % 16 != 0 || (x_codes && (x_code_stride < K || x_code_stride % 16 != 0))) return refuse(who, "a code stride is smaller than the row, or no multiple of 16");
-  if (N == 0 || (M == 0 && !w)) return 0;
-  if ((M > 0 && !y) || (K > 0 && (!w_codes || !w_scales)) || (x_codes && !x_scales)) return refuse(who, "null tensor");
+  if ((!w && (w_code_stride < K || w_code_stride % 16 != 0)) || (x_codes && (x_code_stride < K || x_code_stride % 16 != 0)))
+    return refuse(who, "a code stride is smaller than the row, or no multiple of 16");
+  if (N == 0 || M == 0) return 0;
+  if (!y || (x_codes && !x_scales) || (K > 0 && !w && (!w_codes || !w_scales))) return refuse(who, "null tensor");
   if (!al(y, 2) || !al(w_codes, 16) || !al(w_scales, 4) || !al(x_codes, 16) || !al(x_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  if (!x_codes && M > 0 && K > 0 && (!workspace || !al(workspace, 256) || workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, 0)))
+  if (K > 0 && (!x_codes || w) && (!workspace || !al(workspace, 256) || workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, w ? FLAME_FP8_LINEAR_BF16_WEIGHT : 0)))
     return refuse(who, "workspace too small, or not on 256 bytes");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
   cudaStream_t s = (cudaStream_t)stream;
-  QuantJob jobs[2] = {};
-  int n = 0;
-  if (!x_codes && M > 0 && K > 0) {
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  QuantJobs jobs = {};
+  if (!x_codes && K > 0) {
+    const Place q = take(at, M, K, kQuantRows);
     x_code_stride = up16(K);
-    x_codes = workspace;
-    x_scales = static_cast<uint8_t*>(workspace) + up256(M * x_code_stride);
-    jobs[n++] = quant_job(x, M, K, x_stride, kQuantRows, const_cast<void*>(x_codes), const_cast<void*>(x_scales), nullptr, nullptr, x_code_stride);
+    x_codes = q.codes;
+    x_scales = q.scales;
+    jobs.job[0] = quant_job(x, M, K, x_stride, kQuantRows, q.codes, q.scales, nullptr, nullptr, x_code_stride);
   }
-  if (w && K > 0) jobs[n++] = quant_job(w, N, K, w_stride, kQuantTiles, w_codes, w_scales, nullptr, nullptr, w_code_stride);
-  if (n > 0)
-    if (const cudaError_t e = launch_quant(jobs[0], jobs[1], s)) return (int)e;
-  if (M == 0) return 0;
-  return (int)product(w_blocks == FLAME_FP8_BLOCKS_TILES ? Product::kNtTiles : Product::kNtRows, x_codes, x_code_stride, x_scales, w_codes, w_code_stride, w_scales, y, N,
-                      false, M, N, K, s);
+  if (w && K > 0) {
+    const Place q = take(at, N, K, kQuantTiles);
+    w_code_stride = up16(K);
+    w_codes = q.codes;
+    w_scales = q.scales;
+    jobs.job[1] = quant_job(w, N, K, w_stride, kQuantTiles, q.codes, q.scales, nullptr, nullptr, w_code_stride);
+  }
+  if (const cudaError_t e = launch_quant(jobs, s)) return (int)e;
+  return (int)product(w || w_blocks == FLAME_FP8_BLOCKS_TILES ? Product::kNtTiles : Product::kNtRows, x_codes, x_code_stride, x_scales, w_codes, w_code_stride, w_scales,
+                      y, N, false, M, N, K, s);
 }
 
-int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, size_t x_stride, const void* w_codes, size_t w_code_stride,
-                              const void* w_scales, void* dx, void* dw, size_t M, size_t N, size_t K, void* workspace,
+int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, size_t x_stride, const void* w, size_t w_stride, const void* w_codes,
+                              size_t w_code_stride, const void* w_scales, void* dx, void* dw, size_t M, size_t N, size_t K, void* workspace,
                               size_t workspace_bytes, void* stream) {
   const char* who = "flame_fp8_linear_backward";
   if (const char* what = quant_source(dy, M, N, dy_stride)) return refuse(who, what);
-  if (dw)
-    if (const char* what = quant_source(x, M, K, x_stride)) return refuse(who, what);
+  if (const char* what = dw ? quant_source(x, M, K, x_stride) : nullptr) return refuse(who, what);
+  if (const char* what = dx && w ? quant_source(w, N, K, w_stride) : nullptr) return refuse(who, what);
   if (K > kMostSize) return refuse(who, "matrix too large");
-  if (dx && (w_code_stride < K || w_code_stride % 16 != 0)) return refuse(who, "a code stride is smaller than the row, or no multiple of 16");
+  if (dx && !w && (w_code_stride < K || w_code_stride % 16 != 0)) return refuse(who, "a code stride is smaller than the row, or no multiple of 16");
   if ((!dx && !dw) || K == 0) return 0;
-  if (dx && M > 0 && N > 0 && (!w_codes || !w_scales)) return refuse(who, "null tensor");
+  const bool any = M > 0 && N > 0;
+  if (any && dx && !w && (!w_codes || !w_scales)) return refuse(who, "null tensor");
   if (!al(dx, 2) || !al(dw, 2) || !al(w_codes, 16) || !al(w_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  if (M > 0 && N > 0 && (!workspace || !al(workspace, 256) || workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, 1)))
+  if (any && (!workspace || !al(workspace, 256) ||
+              workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, FLAME_FP8_LINEAR_BACKWARD | (w ? FLAME_FP8_LINEAR_BF16_WEIGHT : 0))))
     return refuse(who, "workspace too small, or not on 256 bytes");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
   cudaStream_t s = (cudaStream_t)stream;
   const size_t ldn = up16(N), ldk = up16(K);
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  uint8_t *rows = at, *cols = at + codes_bytes(M, N, kQuantRows), *xcols = cols + codes_bytes(M, N, kQuantColumns);
-  uint8_t *row_scales = rows + up256(M * ldn), *col_scales = cols + up256(M * ldn), *xcol_scales = xcols + up256(M * ldk);
-  if (M > 0 && N > 0) {
-    const QuantJob a = quant_job(dy, M, N, dy_stride, (dx ? kQuantRows : 0u) | (dw ? kQuantColumns : 0u), rows, row_scales, cols, col_scales, ldn);
-    const QuantJob b = dw ? quant_job(x, M, K, x_stride, kQuantColumns, nullptr, nullptr, xcols, xcol_scales, ldk) : QuantJob{};
-    if (const cudaError_t e = launch_quant(a, b, s)) return (int)e;
+  Place rows = {}, cols = {}, xcols = {};
+  if (any) {
+    rows = take(at, M, N, kQuantRows);
+    cols = take(at, M, N, kQuantColumns);
+    xcols = take(at, M, K, kQuantColumns);
+    QuantJobs jobs = {};
+    jobs.job[0] = quant_job(dy, M, N, dy_stride, (dx ? kQuantRows : 0u) | (dw ? kQuantColumns : 0u), rows.codes, rows.scales, cols.codes, cols.scales, ldn);
+    if (dw) jobs.job[1] = quant_job(x, M, K, x_stride, kQuantColumns, nullptr, nullptr, xcols.codes, xcols.scales, ldk);
+    if (dx && w) {
+      const Place q = take(at, N, K, kQuantTiles);
+      jobs.job[2] = quant_job(w, N, K, w_stride, kQuantTiles, q.codes, q.scales, nullptr, nullptr, ldk);
+      w_codes = q.codes;
+      w_code_stride = ldk;
+      w_scales = q.scales;
+    }
+    if (const cudaError_t e = launch_quant(jobs, s)) return (int)e;
   }
   if (dx && M > 0)
-    if (const cudaError_t e = product(Product::kNnTiles, rows, ldn, row_scales, w_codes, w_code_stride, w_scales, dx, K, false, M, K, N, s)) return (int)e;
-  if (dw && N > 0) return (int)product(Product::kTnColumns, cols, ldn, col_scales, xcols, ldk, xcol_scales, dw, K, false, N, K, M, s);
+    if (const cudaError_t e = product(Product::kNnTiles, rows.codes, ldn, rows.scales, w_codes, w_code_stride, w_scales, dx, K, false, M, K, N, s)) return (int)e;
+  if (dw && N > 0) return (int)product(Product::kTnColumns, cols.codes, ldn, cols.scales, xcols.codes, ldk, xcols.scales, dw, K, false, N, K, M, s);
   return 0;
 }
 

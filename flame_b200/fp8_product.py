@@ -161,48 +161,48 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, transpose_b: bool = False, dtype: 
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(m: int, n: int, k: int, backward: int) -> int:
-    return max(_op.function("flame_fp8_linear_workspace_bytes")(m, n, k, backward), 16)
+def _workspace_bytes(m: int, n: int, k: int, flags: int) -> int:
+    return max(_op.function("flame_fp8_linear_workspace_bytes")(m, n, k, flags), 16)
 
 
-def _forward(x, codes: Optional[Fp8Blocks], weight, frozen: Optional[Fp8Blocks]):
-    """(y, codes of the weight, their scales): one call of the library; a BF16 weight is quantised in it."""
+def _weight_args(weight, frozen: Optional[Fp8Blocks]):
+    """(N, the library's arguments for the weight): BF16, or codes that somebody keeps."""
+    if frozen is not None:
+        return frozen.shape[0], (None, 0, frozen.codes.data_ptr(), frozen.stride, frozen.scales.data_ptr())
+    n, _, stride = _matrix(weight, "fp8_linear")
+    return n, (weight.data_ptr(), stride, None, 0, None)
+
+
+def _forward(x, codes: Optional[Fp8Blocks], weight, frozen: Optional[Fp8Blocks]) -> torch.Tensor:
     device = x.device
     m, k, x_stride = _matrix(x, "fp8_linear")
-    if frozen is not None:
-        n, blocks, w_codes, w_scales, ld, w_stride = frozen.shape[0], _BLOCKS[frozen.blocks], frozen.codes, frozen.scales, frozen.stride, 0
-    else:
-        n, _, w_stride = _matrix(weight, "fp8_linear")
-        blocks, ld = 3, _padded(k)
-        w_codes = torch.empty(n, ld, dtype=torch.uint8, device=device)
-        w_scales = torch.empty(_blocks_of(n), _blocks_of(k), dtype=torch.float32, device=device)
+    n, w_args = _weight_args(weight, frozen)
     y = torch.empty(x.shape[:-1] + (n,), dtype=torch.bfloat16, device=device)
-    if codes is None:
-        size = _workspace_bytes(m, n, k, 0)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-        given = (None, 0, None)
-    else:
-        ws, size, given = None, 0, (codes.codes.data_ptr(), codes.stride, codes.scales.data_ptr())
-    _op.call("flame_fp8_linear", device, x.data_ptr(), x_stride, *given, _op.ptr(weight), w_stride, w_codes.data_ptr(), ld, w_scales.data_ptr(),
-             blocks, y.data_ptr(), m, n, k, _op.ptr(ws), size)
-    return y, w_codes, w_scales
+    size = _workspace_bytes(m, n, k, 0 if frozen is not None else 2)      # FLAME_FP8_LINEAR_BF16_WEIGHT
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    given = (None, 0, None) if codes is None else (codes.codes.data_ptr(), codes.stride, codes.scales.data_ptr())
+    _op.call("flame_fp8_linear", device, x.data_ptr(), x_stride, *given, *w_args, 3 if frozen is None else _BLOCKS[frozen.blocks], y.data_ptr(), m, n, k,
+             ws.data_ptr(), size)
+    return y
 
 
 class _Linear(torch.autograd.Function):
-    """y = x w^T.  Saved for backward: x where the weight is trained (BF16, so that a pool can offload it), and the weight's codes."""
+    """y = x w^T.  Saved for backward: x where the weight is trained (BF16, so that a pool can offload it) and the weight itself.  Its codes
+    are made again: keeping them would hold half as much memory again as the weights do, for a few per cent of a step's time."""
 
     @staticmethod
     def forward(ctx, x, weight, codes, frozen):
-        y, w_codes, w_scales = _forward(x, codes, weight, frozen)
-        want_dx = ctx.needs_input_grad[0]
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w_codes if want_dx else None, w_scales if want_dx else None)
-        ctx.ld = frozen.stride if frozen is not None else w_codes.shape[1]
+        y = _forward(x, codes, weight, frozen)
+        want_dx, want_dw = ctx.needs_input_grad[:2]
+        kept = (frozen.codes, frozen.scales) if frozen is not None else (weight, None)
+        ctx.save_for_backward(x if want_dw else None, *(kept if want_dx else (None, None)))
+        ctx.frozen = frozen is not None
         ctx.x_shape, ctx.n = x.shape, y.shape[-1]
         return y
 
     @_op.first_order
     def backward(ctx, dy):
-        x, w_codes, w_scales = ctx.saved_tensors
+        x, w, w_scales = ctx.saved_tensors
         want_dx, want_dw = ctx.needs_input_grad[:2]
         shape, n = ctx.x_shape, ctx.n
         device = dy.device
@@ -210,10 +210,13 @@ class _Linear(torch.autograd.Function):
         m, k = _rows_of(shape), shape[-1]
         dx = torch.empty(shape, dtype=torch.bfloat16, device=device) if want_dx else None
         dw = torch.empty(n, k, dtype=torch.bfloat16, device=device) if want_dw else None
-        size = _workspace_bytes(m, n, k, 1)
+        w_args = (None, 0, None, 0, None)
+        if want_dx:
+            w_args = _weight_args(w, Fp8Blocks(w, w_scales, "tiles") if ctx.frozen else None)[1]
+        size = _workspace_bytes(m, n, k, 1 if ctx.frozen else 3)
         ws = torch.empty(size, dtype=torch.uint8, device=device)
-        _op.call("flame_fp8_linear_backward", device, dy.data_ptr(), n, _op.ptr(x), _matrix(x, "fp8_linear")[2] if want_dw else 0,
-                 _op.ptr(w_codes), ctx.ld, _op.ptr(w_scales), _op.ptr(dx), _op.ptr(dw), m, n, k, ws.data_ptr(), size)
+        _op.call("flame_fp8_linear_backward", device, dy.data_ptr(), n, _op.ptr(x), _matrix(x, "fp8_linear")[2] if want_dw else 0, *w_args,
+                 _op.ptr(dx), _op.ptr(dw), m, n, k, ws.data_ptr(), size)
         return dx, dw, None, None
 
 
@@ -238,5 +241,5 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], *, codes
         if record:
             raise Unsupported("fp8_linear: a weight with rows of blocks has no input gradient; quantise it to tiles")
     if not record:
-        return _forward(x, codes, None if frozen is not None else weight, frozen)[0]
+        return _forward(x, codes, None if frozen is not None else weight, frozen)
     return _Linear.apply(x, None if frozen is not None else weight, codes, frozen)

@@ -571,17 +571,18 @@ int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales
                       const void* b_scales, int b_blocks, int b_transposed, void* c, size_t c_stride, int c_dtype, size_t M,
                       size_t N, size_t K, void* stream);
 /* The linear layer made of them: y [M, N] = x w^T, BF16 and contiguous, x [M, K] with x_stride elements from row to row.
- * x_codes (NULL: x is quantised into the workspace) are x's ROWS blocks.  w (NULL: w_codes / w_scales are given, TILES or ROWS) is
- * the BF16 weight [N, K], whose TILES blocks are written to w_codes / w_scales, for backward: dx [M, K], dw [N, K] (NULL = not
- * wanted) from dy [M, N], w's TILES blocks and x.  dy has ROWS blocks for dx and COLUMNS for dw, from one read; x COLUMNS.
- * workspace: flame_fp8_linear_workspace_bytes, on 256 bytes, free again when the call's work is done. */
-size_t flame_fp8_linear_workspace_bytes(size_t M, size_t N, size_t K, int backward);
+ * x_codes (NULL: x is quantised in the call) are x's ROWS blocks.  The weight [N, K] is BF16 (w, quantised to TILES in the call) or
+ * codes (w NULL; TILES or ROWS).  backward: dx [M, K], dw [N, K] (NULL = not wanted) from dy [M, N], the weight (for dx; TILES) and x
+ * (for dw).  dy has ROWS blocks for dx and COLUMNS for dw, from one read; x COLUMNS.
+ * workspace: flame_fp8_linear_workspace_bytes (flags as below), on 256 bytes, free again when the call's work is done. */
+enum { FLAME_FP8_LINEAR_BACKWARD = 1, FLAME_FP8_LINEAR_BF16_WEIGHT = 2 };
+size_t flame_fp8_linear_workspace_bytes(size_t M, size_t N, size_t K, int flags);
 int flame_fp8_linear(const void* x_bf16, size_t x_stride, const void* x_codes, size_t x_code_stride, const void* x_scales, const void* w_bf16,
-                     size_t w_stride, void* w_codes, size_t w_code_stride, void* w_scales, int w_blocks, void* y_bf16, size_t M, size_t N,
-                     size_t K, void* workspace, size_t workspace_bytes, void* stream);
-int flame_fp8_linear_backward(const void* dy_bf16, size_t dy_stride, const void* x_bf16, size_t x_stride, const void* w_codes,
-                              size_t w_code_stride, const void* w_scales, void* dx_bf16, void* dw_bf16, size_t M, size_t N, size_t K,
-                              void* workspace, size_t workspace_bytes, void* stream);
+                     size_t w_stride, const void* w_codes, size_t w_code_stride, const void* w_scales, int w_blocks, void* y_bf16, size_t M,
+                     size_t N, size_t K, void* workspace, size_t workspace_bytes, void* stream);
+int flame_fp8_linear_backward(const void* dy_bf16, size_t dy_stride, const void* x_bf16, size_t x_stride, const void* w_bf16, size_t w_stride,
+                              const void* w_codes, size_t w_code_stride, const void* w_scales, void* dx_bf16, void* dw_bf16, size_t M,
+                              size_t N, size_t K, void* workspace, size_t workspace_bytes, void* stream);
 /* How often a wait inside a product's kernel on the current device gave up after two seconds since the library was loaded, in
  * which case that product's result is wrong.  0 unless something else is broken.  Waits for the device. */
 int flame_fp8_product_faults(unsigned int* count);

@@ -58,6 +58,27 @@ def test_product_entry():
     assert lib.flame_fp8_product(None, 64, None, 1, None, 64, None, 3, 1, None, 16, 0, 0, 16, 64, None) == 0
 
 
+def test_linear_entries():
+    lib = _lib.lib()
+    assert lib.flame_fp8_linear_workspace_bytes(1 << 40, 1, 1, 0) == 0
+    size = lib.flame_fp8_linear_workspace_bytes(8, 16, 64, 2)
+    ok = [FAKE, 64, None, 0, None, FAKE, 64, None, 0, None, 0, FAKE, 8, 16, 64, FAKE, size, None]
+    for at, value, text in ((0, None, "null"), (1, 63, "stride"), (6, 60, "stride"), (11, None, "null"), (11, FAKE + 1, "misaligned"), (15, FAKE + 16, "workspace"), (16, size - 1, "workspace"),
+                            (12, 1 << 40, "too large"), (2, FAKE, "stride")):
+        bad = list(ok)
+        bad[at] = value
+        refused(text, "flame_fp8_linear", *bad)
+    refused("tiles or rows", "flame_fp8_linear", FAKE, 64, None, 0, None, None, 0, FAKE, 64, FAKE, 2, FAKE, 8, 16, 64, FAKE, size, None)
+    refused("null", "flame_fp8_linear", FAKE, 64, None, 0, None, None, 0, FAKE, 64, None, 3, FAKE, 8, 16, 64, FAKE, size, None)
+    size = lib.flame_fp8_linear_workspace_bytes(8, 16, 64, 3)
+    ok = [FAKE, 16, FAKE, 64, FAKE, 64, None, 0, None, FAKE, FAKE, 8, 16, 64, FAKE, size, None]
+    for at, value, text in ((0, None, "null"), (1, 15, "stride"), (2, None, "null"), (3, 63, "stride"), (5, 63, "stride"), (9, FAKE + 1, "misaligned"), (15, size - 1, "workspace")):
+        bad = list(ok)
+        bad[at] = value
+        refused(text, "flame_fp8_linear_backward", *bad)
+    assert lib.flame_fp8_linear(None, 64, None, 0, None, None, 0, None, 64, None, 3, None, 0, 16, 64, None, 0, None) == 0
+
+
 def test_group_norm_entries():
     lib = _lib.lib()
     assert lib.flame_group_norm_workspace_bytes(2, 10, 64, 7, 0) == 0 and "multiple" in _lib.last_error()
