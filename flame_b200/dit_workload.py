@@ -20,6 +20,8 @@ import torch.nn.functional as F
 
 from . import checkpoint as ckpt
 from . import fused_producers
+from .dropout import dropout
+from .fp8_product import fp8_linear
 from .activation_offload import ActivationOffloadPool, OffloadCompression
 from .policy import Block, Decision, plan_blocks, probe
 
@@ -29,6 +31,12 @@ TOKENS = IMG_TOKENS + TXT_TOKENS
 # True: RMSNorm and SwiGLU run as this library's kernels, which also emit the codes of the tensor the block saves
 # while a block is being offloaded (flame_b200/fused_producers.py); False: PyTorch ops, compress launches read the tensors.
 FUSED_PRODUCERS = False
+# True: the qkv, proj and gate-up products run in FP8 with a scale for each block of 128 (flame_b200/fp8_product.py), forward and
+# backward; what they save is the BF16 input, as before.
+FP8_LINEARS = False
+# Dropout before the two residual sums of a block (flame_b200/dropout.py): nothing is saved for it, and a recomputed block draws the
+# same mask.  The caller changes the seed from step to step.
+DROPOUT_P, DROPOUT_SEED = 0.0, 0
 
 
 def rope_tables(device):
@@ -119,8 +127,9 @@ class SwiGLUDownFn(torch.autograd.Function):
 class DiTBlock(nn.Module):
     """Saves, per block, exactly: norm1 output, rotated Q/K and V, attention output, norm2 output, gate+up."""
 
-    def __init__(self):
+    def __init__(self, index: int = 0):
         super().__init__()
+        self.index = index
         self.norm1_w = nn.Parameter(torch.ones(HIDDEN))
         self.qkv = nn.Linear(HIDDEN, 3 * HIDDEN, bias=False)
         self.proj = nn.Linear(HIDDEN, HIDDEN, bias=False)
@@ -128,21 +137,30 @@ class DiTBlock(nn.Module):
         self.gate_up = nn.Linear(HIDDEN, 2 * MLP_HIDDEN, bias=False)
         self.down = nn.Linear(MLP_HIDDEN, HIDDEN, bias=False)
 
+    @staticmethod
+    def _product(layer, x):
+        return fp8_linear(x, layer.weight) if FP8_LINEARS else layer(x)
+
+    def _residual(self, x, h, place):
+        if DROPOUT_P:
+            return dropout(h, DROPOUT_P, seed=DROPOUT_SEED, offset=2 * self.index + place, residual=x)
+        return x + h
+
     def forward(self, x, cos, sin):
         b, t, _ = x.shape
-        qkv = self.qkv(RMSNormFn.apply(x, self.norm1_w, 1e-6)).view(b, t, 3, HEADS, HEAD_DIM)
+        qkv = self._product(self.qkv, RMSNormFn.apply(x, self.norm1_w, 1e-6)).view(b, t, 3, HEADS, HEAD_DIM)
         q = RoPEFn.apply(qkv[:, :, 0], cos, sin)          # [B,T,H,D], contiguous
         k = RoPEFn.apply(qkv[:, :, 1], cos, sin)
         v = qkv[:, :, 2].contiguous()
         a = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))  # views over [B,T,H,D]
-        x = x + self.proj(a.transpose(1, 2).reshape(b, t, HIDDEN))
-        return x + SwiGLUDownFn.apply(self.gate_up(RMSNormFn.apply(x, self.norm2_w, 1e-6)), self.down.weight)
+        x = self._residual(x, self._product(self.proj, a.transpose(1, 2).reshape(b, t, HIDDEN)), 0)
+        return self._residual(x, SwiGLUDownFn.apply(self._product(self.gate_up, RMSNormFn.apply(x, self.norm2_w, 1e-6)), self.down.weight), 1)
 
 
 class DiT(nn.Module):
     def __init__(self, blocks: int = 20):
         super().__init__()
-        self.blocks = nn.ModuleList(DiTBlock() for _ in range(blocks))
+        self.blocks = nn.ModuleList(DiTBlock(i) for i in range(blocks))
         self.decisions = None  # per block: Decision, or None = plain autograd
 
     def forward(self, x, cos, sin):
