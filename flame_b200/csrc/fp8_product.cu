@@ -180,9 +180,11 @@ template <typename T>
 __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant__ DequantArgs a) {
   pdl_prologue();
   const uint32_t across = (a.cols + 7) / 8;   // eight elements a thread
-  const size_t total = (size_t)a.rows * across;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-    const uint32_t row = (uint32_t)(i / across), c0 = (uint32_t)(i - (size_t)row * across) * 8;
+  const bool wide = a.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
+  const uint32_t rows_at_once = gridDim.x * 256 / across;      // a thread keeps its columns and walks down the rows, where it can
+  const uint32_t t = blockIdx.x * 256 + threadIdx.x, c0 = t % across * 8;
+  if (t / across >= rows_at_once) return;
+  for (uint32_t row = t / across; row < a.rows; row += rows_at_once) {
     const uint8_t* src = a.codes + (size_t)row * a.code_stride + c0;
     uint2 w = make_uint2(0u, 0u);
     if (c0 + 8 <= a.cols) {
@@ -193,14 +195,29 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
         if (c0 + k < a.cols) (k < 4 ? w.x : w.y) |= (uint32_t)src[k] << (8 * (k & 3));
     }
     const float* s = a.scales + (size_t)(row / a.down) * a.scales_across;
-    T* out = static_cast<T*>(a.out) + (size_t)row * a.cols + c0;
+    float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (c0 + k < a.cols) {
-        const float v = fp8_decode(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xFFu) * s[(c0 + k) / a.across];
-        if constexpr (sizeof(T) == 2) out[k] = __float2bfloat16_rn(v);
-        else out[k] = v;
+      f[k] = c0 + k < a.cols ? fp8_decode(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xFFu) * s[a.across == 1 ? c0 + k : c0 / kBlock] : 0.0f;
+    T* out = static_cast<T*>(a.out) + (size_t)row * a.cols + c0;
+    if (wide) {
+      if constexpr (sizeof(T) == 2) {
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[k]) : "f"(f[2 * k + 1]), "f"(f[2 * k]));
+        *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+        reinterpret_cast<float4*>(out)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(out)[1] = make_float4(f[4], f[5], f[6], f[7]);
       }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c0 + k < a.cols) {
+          if constexpr (sizeof(T) == 2) out[k] = __float2bfloat16_rn(f[k]);
+          else out[k] = f[k];
+        }
+    }
   }
 }
 
@@ -964,8 +981,9 @@ int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scal
   a.down = blocks == FLAME_FP8_BLOCKS_ROWS ? 1 : kBlock;
   a.across = blocks == FLAME_FP8_BLOCKS_COLUMNS ? 1 : kBlock;
   a.scales_across = blocks == FLAME_FP8_BLOCKS_COLUMNS ? (uint32_t)cols : (uint32_t)((cols + 127) / 128);
-  const uint64_t blocks_wanted = ((uint64_t)rows * ((cols + 7) / 8) + 255) / 256;
-  const unsigned grid = (unsigned)(blocks_wanted < 148 * 32 ? blocks_wanted : 148 * 32);
+  // at least one row of threads, so that every column has one
+  const uint64_t across = (cols + 7) / 8, wanted = ((uint64_t)rows * across + 255) / 256, least = (across + 255) / 256;
+  const unsigned grid = (unsigned)(wanted < 148 * 32 ? wanted : least > 148 * 32 ? least : 148 * 32);
   return out_dtype == FLAME_OFFLOAD_DTYPE_F32 ? (int)launch_after(fp8_dequant_kernel<float>, grid, 256, 0, (cudaStream_t)stream, a)
                                               : (int)launch_after(fp8_dequant_kernel<__nv_bfloat16>, grid, 256, 0, (cudaStream_t)stream, a);
 }
