@@ -7,11 +7,13 @@
 //
 // Two launches each way: the first reduces, the second applies.  A thread owns V neighbouring channels and walks down the
 // positions of its chunk, so that a warp reads whole lines of the channels-last rows, and per-channel sums stay in registers.
-// The forward sums are kept about a shift, the group's first element in the sample: x - shift is of the size of the spread and not of
-// the mean, so that sums of squares lose nothing when the mean is large against the spread.  A cluster of thread blocks adds its sums
-// up through distributed shared memory, which leaves the second launch a quarter of them to read; where there are many, a launch
-// of one block a sample adds them up in between.  Everything is added in a fixed order, without atomics: the same inputs give the
-// same bits.
+// A block's forward sums are kept about a shift, the group's first element in its chunk: x - shift is of the size of the spread and not of
+// the mean, so that sums of squares lose nothing when the mean is large against the spread.  (Where that element is an outlier, at a
+// distance D from the others, the block's n elements err by n 2^-24 D^2 at most in a sum that the outlier alone brings to D^2: n is a
+// chunk's here, some thousands, and would be a million with one shift for the sample.)  Blocks are then joined by their mean and sum of
+// squares about it (T. Chan, G. Golub, R. LeVeque, 1983): a cluster's through distributed shared memory, which leaves the second
+// launch a quarter of them to read; where there are many, a launch of a warp for each group joins them in between.  Everything is
+// added in a fixed order, without atomics: the same inputs give the same bits.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -39,7 +41,7 @@ struct NormArgs {
   uint8_t* codes;                // forward, may be NULL: FP8 codes of y, a scale for 128 elements of a row
   float* code_scales;
   float* stats;                  // [B, G, 2]: mean, rstd
-  float2* partial;               // [B, parts, G]: forward sums of x - shift and of its square, backward s1 and s2
+  float2* partial;               // [B, parts, G]: forward mean and sum of squares about it, backward s1 and s2
   float2* channel_partial;       // backward: [B, parts, C]: sums for dbias and dweight
   float2* finished;              // NULL, or [B, G]: what the launch between the two made of the parts
   void* dweight;                 // backward, may be NULL
@@ -50,7 +52,7 @@ struct NormArgs {
   uint32_t parts;                // clusters per sample: chunks / kCluster * slabs
   uint32_t rows_per_chunk;
   uint32_t slabs;                // channel slabs of one thread block's width
-  uint32_t slab_vecs;            // V-wide channel vectors in a slab
+  uint32_t slab_vecs, V;         // V-wide channel vectors in a slab
   float eps;
   int silu, params_f32;
   int stream;                    // x and y together are larger than the L2 cache
@@ -301,10 +303,10 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// `count` pairs of every block's `sh`, pair i at place(i), added over the cluster's blocks in the order of their ranks; each block
-// writes its share of the sums.
-template <typename F>
-__device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, float2* out, F&& place) {
+// `count` pairs of every block's `sh`, pair i at place(i), joined over the cluster's blocks in the order of their ranks; each block
+// joins and writes its share.
+template <typename F, typename J>
+__device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, float2* out, F&& place, J&& join) {
   cluster_sync_all();
   const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(sh));
   for (uint32_t i = cluster_rank() + kCluster * threadIdx.x; i < count; i += kCluster * kThreads) {
@@ -315,16 +317,19 @@ __device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, f
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at + place(i) * 8), "r"(k));
       asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[k].x), "=f"(v[k].y) : "r"(peer) : "memory");
     }
-    float2 t = v[0];
-#pragma unroll
-    for (uint32_t k = 1; k < kCluster; ++k) { t.x += v[k].x; t.y += v[k].y; }
-    out[i] = t;
+    out[i] = join(i, v);
   }
   cluster_sync_all();      // nobody leaves or writes its sums while they are read
 }
+__device__ __forceinline__ float2 add_up(const float2 (&v)[kCluster]) {
+  float2 t = v[0];
+#pragma unroll
+  for (uint32_t k = 1; k < kCluster; ++k) { t.x += v[k].x; t.y += v[k].y; }
+  return t;
+}
 // The slab's channel sums, weighted, added up to the groups that the slab touches: a thread a group, a warp where groups are wide.
-template <typename F>
-__device__ __forceinline__ void join_channels(const NormArgs& a, uint32_t slab_c0, uint32_t width, float2* groups, F&& pair) {
+template <typename F, typename D>
+__device__ __forceinline__ void join_channels(const NormArgs& a, uint32_t slab_c0, uint32_t width, float2* groups, F&& pair, D&& done) {
   const uint32_t lane = threadIdx.x & 31;
   const bool warps = a.cg > 32;
   for (uint32_t g = warps ? threadIdx.x >> 5 : threadIdx.x; g < a.G; g += warps ? kWarps : kThreads) {
@@ -337,32 +342,65 @@ __device__ __forceinline__ void join_channels(const NormArgs& a, uint32_t slab_c
       q += t.y;
     }
     if (warps) { s = warp_sum(s); q = warp_sum(q); }
-    if (!warps || lane == 0) groups[g] = make_float2(s, q);
+    if (!warps || lane == 0) groups[g] = done(g, s, q);
   }
 }
-// The sums of every group of sample b from the parts: eight threads a group take every eighth part each, then join.
-template <typename F>
-__device__ __forceinline__ void join_parts(const NormArgs& a, uint32_t b, F&& done) {
-  for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / 8) {
-    const uint32_t g = g0 + threadIdx.x / 8, k = threadIdx.x % 8;
-    float s = 0.0f, q = 0.0f;
-    if (g < a.G) {
-      const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
+// Elements of group g in channels [c0, c0 + width) and the rows from row0 on, `most` of them at the most.
+__device__ __forceinline__ float elements(const NormArgs& a, uint32_t g, uint32_t c0, uint32_t width, uint64_t row0, uint64_t most) {
+  const uint32_t lo = g * a.cg > c0 ? g * a.cg : c0, hi = (g + 1) * a.cg < c0 + width ? (g + 1) * a.cg : c0 + width;
+  const uint64_t left = a.L > row0 ? a.L - row0 : 0;
+  return lo < hi ? (float)(hi - lo) * (float)(left < most ? left : most) : 0.0f;
+}
+// Those of part i of a sample (a cluster's): i counts the clusters of a slab first.
+__device__ __forceinline__ float elements_of_part(const NormArgs& a, uint32_t i, uint32_t g, uint32_t slab_width) {
+  const uint32_t clusters = a.chunks / kCluster, slab = a.slabs == 1 ? 0 : i / clusters;
+  const uint64_t rows = (uint64_t)a.rows_per_chunk * kCluster;
+  return elements(a, g, slab * slab_width, slab_width, (i - slab * clusters) * rows, rows);
+}
+
+// The parts of a group joined by kLanes neighbouring threads, of which this is number k: forward mean and sum of squares of the whole,
+// backward the sums.
+template <bool kBackward, int kLanes>
+__device__ __forceinline__ float2 join_parts(const NormArgs& a, uint32_t b, uint32_t g, uint32_t k) {
+  const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
+  auto all = [](float v) {
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    return v;
+  };
+  const bool live = g < a.G;
+  float s = 0.0f, q = 0.0f;
+  if (kBackward) {
+    if (live) {
 #pragma unroll 4
-      for (uint32_t i = k; i < a.parts; i += 8) {
+      for (uint32_t i = k; i < a.parts; i += kLanes) {
         const float2 t = in[(size_t)i * a.G];
         s += t.x;
         q += t.y;
       }
     }
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) {
-      s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-      q += __shfl_xor_sync(0xFFFFFFFFu, q, d);
-    }
-    if (g < a.G && k == 0) done(g, s, q);
+    return make_float2(all(s), all(q));
   }
-  __syncthreads();
+  const uint32_t slab_width = a.slabs == 1 ? a.C : a.slab_vecs * a.V;
+  // a part that has elements of the group: the first of its first slab
+  const float shift = live ? in[(size_t)(a.slabs == 1 ? 0 : g * a.cg / slab_width * (a.chunks / kCluster)) * a.G].x : 0.0f;
+  if (live) {
+#pragma unroll 4
+    for (uint32_t i = k; i < a.parts; i += kLanes) {
+      const float n = elements_of_part(a, i, g, slab_width);
+      if (n > 0.0f) s += n * (in[(size_t)i * a.G].x - shift);
+    }
+  }
+  const float mean = shift + all(s) / ((float)a.L * (float)a.cg);
+  if (live) {
+#pragma unroll 4
+    for (uint32_t i = k; i < a.parts; i += kLanes) {
+      const float n = elements_of_part(a, i, g, slab_width);
+      const float2 t = in[(size_t)i * a.G];
+      if (n > 0.0f) q += fmaf(n * (t.x - mean), t.x - mean, t.y);
+    }
+  }
+  return make_float2(mean, all(q));
 }
 
 template <int V>
@@ -374,14 +412,15 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
   const __nv_bfloat16* xs = a.x + (size_t)p.b * a.L * a.C;
   const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
   Walk<1, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
+  const __nv_bfloat16* first_row = xs + (p.rows ? p.row0 : 0) * a.C;      // the chunk's
   F2 shift[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the shift's negative
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) {
     s[i] = q[i] = F2(0.0f, 0.0f);
     float2 t = make_float2(0.0f, 0.0f);
     if (p.live) {
-      t.x = -__bfloat162float(xs[group_of(p.c0 + 2 * i, a.by_cg) * a.cg]);
-      if (V > 1) t.y = -__bfloat162float(xs[group_of(p.c0 + 2 * i + 1, a.by_cg) * a.cg]);
+      t.x = -__bfloat162float(first_row[group_of(p.c0 + 2 * i, a.by_cg) * a.cg]);
+      if (V > 1) t.y = -__bfloat162float(first_row[group_of(p.c0 + 2 * i + 1, a.by_cg) * a.cg]);
     }
     shift[i] = F2(t.x, t.y);
   }
@@ -399,45 +438,60 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
   const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
   join_rows<V>(p, s, q, sh, width);
   float2* groups = sh + kThreads * V;
-  join_channels(a, slab_c0, width, groups, [&](uint32_t c) { return sh[place_of<V>(c - slab_c0, width)]; });
-  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G, [](uint32_t i) { return i; });
+  join_channels(a, slab_c0, width, groups, [&](uint32_t c) { return sh[place_of<V>(c - slab_c0, width)]; }, [&](uint32_t g, float sum, float sum2) {
+    const float n = elements(a, g, slab_c0, width, p.row0, p.rows);
+    if (n == 0.0f) return make_float2(0.0f, 0.0f);
+    const float off = sum / n;
+    // fmaxf would turn the NaN of a NaN or an infinity into 0
+    return make_float2(__bfloat162float(first_row[g * a.cg]) + off, sum2 < INFINITY ? fmaxf(sum2 - sum * off, 0.0f) : NAN);
+  });
+  // mean and sum of squares of the cluster's blocks, joined
+  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G, [](uint32_t i) { return i; },
+               [&](uint32_t g, const float2 (&v)[kCluster]) {
+    const uint64_t row0 = (uint64_t)(p.chunk / kCluster * kCluster) * a.rows_per_chunk;
+    float n[kCluster], total = 0.0f, mean = 0.0f, m2 = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < kCluster; ++k) {
+      n[k] = elements(a, g, slab_c0, width, row0 + (uint64_t)k * a.rows_per_chunk, a.rows_per_chunk);
+      total += n[k];
+    }
+    if (total == 0.0f) return make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t k = 1; k < kCluster; ++k) mean += n[k] > 0.0f ? n[k] * (v[k].x - v[0].x) : 0.0f;      // block 0 has rows where any has
+    mean = v[0].x + mean / total;
+#pragma unroll
+    for (uint32_t k = 0; k < kCluster; ++k) m2 += n[k] > 0.0f ? fmaf(n[k] * (v[k].x - mean), v[k].x - mean, v[k].y) : 0.0f;
+    return make_float2(mean, m2);
+  });
 }
 
-// What the second launch needs of a group's sums: mean and rstd, or backward the means of s1 and s2.
+// What the second launch needs of a group: mean and rstd, or backward the means of s1 and s2.
 template <bool kBackward>
-__device__ __forceinline__ float2 finish(const NormArgs& a, uint32_t b, uint32_t g, float s, float q) {
+__device__ __forceinline__ float2 finish(const NormArgs& a, float2 t) {
   const float inv_n = 1.0f / ((float)a.L * (float)a.cg);
-  if (kBackward) return make_float2(s * inv_n, q * inv_n);
-  const float off = s * inv_n, var = fmaxf(q * inv_n - off * off, 0.0f);
-  // fmaxf would turn the NaN of a group with a NaN or an infinity into 0
-  return make_float2(__bfloat162float(a.x[(size_t)b * a.L * a.C + g * a.cg]) + off, q == q && q < INFINITY ? rsqrtf(var + a.eps) : NAN);
+  if (kBackward) return make_float2(t.x * inv_n, t.y * inv_n);
+  return make_float2(t.x, rsqrtf(t.y * inv_n + a.eps));
 }
 template <bool kBackward>
 __device__ __forceinline__ void finish_all(const NormArgs& a, uint32_t b, float2* out) {
   if (a.finished) {
     for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) out[g] = a.finished[(size_t)b * a.G + g];
-    __syncthreads();
   } else {
-    join_parts(a, b, [&](uint32_t g, float s, float q) { out[g] = finish<kBackward>(a, b, g, s, q); });
+    for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / 8) {      // eight threads a group
+      const uint32_t g = g0 + threadIdx.x / 8;
+      const float2 t = join_parts<kBackward, 8>(a, b, g, threadIdx.x % 8);
+      if (g < a.G && threadIdx.x % 8 == 0) out[g] = finish<kBackward>(a, t);
+    }
   }
+  __syncthreads();
 }
 // A warp for each group of sample blockIdx.y.
 template <bool kBackward>
 __global__ void __launch_bounds__(kThreads) group_finish_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
   const uint32_t g = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y;
-  if (g >= a.G) return;
-  const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
-  float s = 0.0f, q = 0.0f;
-#pragma unroll 4
-  for (uint32_t i = lane; i < a.parts; i += 32) {
-    const float2 t = in[(size_t)i * a.G];
-    s += t.x;
-    q += t.y;
-  }
-  s = warp_sum(s);
-  q = warp_sum(q);
-  if (lane == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, b, g, s, q);
+  const float2 t = join_parts<kBackward, 32>(a, b, g, lane);
+  if (g < a.G && lane == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, t);
 }
 
 // Codes of eight channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
@@ -554,10 +608,12 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
     const float w = param(a.weight, a.params_f32, c, 1.0f);
     const float2 t = sh[place_of<V>(c - slab_c0, width)];
     return make_float2(w * t.x, w * t.y);
-  });
+  }, [](uint32_t, float sum, float sum2) { return make_float2(sum, sum2); });
   const uint32_t part = p.chunk / kCluster;
-  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + part) * a.G, [](uint32_t i) { return i; });
-  join_cluster(sh, width, a.channel_partial + ((size_t)p.b * (a.chunks / kCluster) + part) * a.C + slab_c0, [&](uint32_t c) { return place_of<V>(c, width); });
+  join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + part) * a.G, [](uint32_t i) { return i; },
+               [](uint32_t, const float2 (&v)[kCluster]) { return add_up(v); });
+  join_cluster(sh, width, a.channel_partial + ((size_t)p.b * (a.chunks / kCluster) + part) * a.C + slab_c0, [&](uint32_t c) { return place_of<V>(c, width); },
+               [](uint32_t, const float2 (&v)[kCluster]) { return add_up(v); });
 }
 
 // The blocks of one more sample than there are add the channel sums up to dweight and dbias.
@@ -765,7 +821,7 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   if (finishes(p)) a.finished = reinterpret_cast<float2*>(a.stats);
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
   a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
-  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
+  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs; a.V = (uint32_t)p.V;
   a.eps = eps; a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
   const dim3 grid(p.chunks, p.slabs, (unsigned)B);
   const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
@@ -809,7 +865,7 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   a.dweight = dweight; a.dbias = dbias;
   a.B = (uint32_t)B; a.C = (uint32_t)C; a.G = (uint32_t)G; a.cg = (uint32_t)(C / G); a.L = L;
   a.by_cg = a.cg == 1 ? 0 : (uint32_t)(((1ull << 32) + a.cg - 1) / a.cg);
-  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs;
+  a.chunks = p.chunks; a.parts = p.parts; a.rows_per_chunk = (uint32_t)p.rows_per_chunk; a.slabs = p.slabs; a.slab_vecs = p.slab_vecs; a.V = (uint32_t)p.V;
   a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
   const dim3 grid(p.chunks, p.slabs, (unsigned)B);
   const dim3 more(p.chunks, p.slabs, (unsigned)B + (dweight || dbias ? 1 : 0));

@@ -108,6 +108,18 @@ def test_mean_far_from_zero(cuda_device):
     assert bool((group_norm(same, 4) == 0).all())
 
 
+@pytest.mark.parametrize("positions", [1, 50, 4096, 200000])
+def test_one_element_far_from_the_others(cuda_device, positions):
+    """The first element of a group, a position's only large value: a sum of squares about it would lose the others.  A chunk has at most
+    some thousand elements a group here, which err by n * 2^-24 of the outlier's square together: 2^-13 of the variance, half of that of
+    the output."""
+    x = torch.randn(1, positions, 32, device=cuda_device).to(torch.bfloat16)
+    x[0, 0, 8] = 10000.0
+    y = group_norm(x, 4)
+    r = reference(x, 4, None, None, 1e-5, False, torch.zeros_like(x))
+    assert bool(((y.double() - r["y"]).abs() <= (BF16 + 2.0 ** -14) * r["y"].abs() + FP32 * (1 + r["y"].abs())).all())
+
+
 def test_nonfinite_values_stay_in_their_group(cuda_device):
     x, w, b, _ = inputs((2, 50, 64, 8), cuda_device, torch.float32)
     clean = group_norm(x, 8, w, b, activation="silu")
@@ -179,6 +191,32 @@ def test_views_empty_and_partial_gradients(cuda_device):
     both = torch.autograd.grad(group_norm(t, 4, w2, b2).sum(), (w2, b2))
     assert torch.equal(torch.autograd.grad(group_norm(t, 4, w2, b2.detach()).sum(), w2)[0], both[0])
     assert torch.equal(torch.autograd.grad(group_norm(t, 4, w2.detach(), b2).sum(), b2)[0], both[1])
+
+
+def test_nonfinite_values_of_narrow_groups(cuda_device):
+    """Groups of three channels: pairs and vectors of channels span groups, whose values must not mix."""
+    for c, g in ((24, 8), (30, 10), (15, 5)):
+        x, w, b, dy = inputs((1, 40, c, g), cuda_device, torch.float32)
+        z = x.clone()
+        z[0, 7, 4] = float("nan")
+        outs = []
+        for t in (x, z):
+            t = t.requires_grad_(True)
+            y = group_norm(t, g, w, b, activation="silu")
+            outs.append((y.detach(), torch.autograd.grad(y, t, dy)[0]))
+        for clean, got in zip(*outs):
+            assert bool(torch.isnan(got[0, :, 3:6]).all())
+            keep = [i for i in range(c) if not 3 <= i < 6]
+            assert torch.equal(clean[..., keep], got[..., keep])
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    x = torch.randn(1, 8, 16, device=cuda_device).to(torch.bfloat16).requires_grad_(True)
+    w = torch.randn(16, 16, device=cuda_device).to(torch.bfloat16)
+    for f in (lambda t: group_norm(t, 4), lambda t: fp8_linear(t, w)):
+        first = torch.autograd.grad(f(x).float().square().sum(), x, create_graph=True)[0]
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.float().sum(), x)
 
 
 def test_same_bits_every_time_on_any_stream_and_in_a_graph(cuda_device):
