@@ -229,15 +229,17 @@ extern "C" int flame_dropout(const void* x, const void* residual, void* y, size_
     return (int)cudaErrorInvalidValue;
   }
   if (n == 0) return 0;
-  if (!x || !y) {
-    set_last_error("flame_dropout: null tensor");
+  auto al = [](const void* q, uintptr_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) == 0; };
+  const uintptr_t size = dtype == FLAME_OFFLOAD_DTYPE_BF16 ? 2 : 4;
+  if (!x || !y || !al(x, size) || !al(y, size) || !al(residual, size) || !al(seed_device, 8)) {
+    set_last_error(!x || !y ? "flame_dropout: null tensor" : "flame_dropout: misaligned tensor");
     return (int)cudaErrorInvalidValue;
   }
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
   const double t = nearbyint(p * 4294967296.0);   // 0 .. 2^32
   const uint64_t ti = (uint64_t)t;
   if (ti >> 32) {      // everything is dropped
-    const size_t bytes = n * (dtype == FLAME_OFFLOAD_DTYPE_BF16 ? 2 : 4);
+    const size_t bytes = n * size;
     return residual ? (int)cudaMemcpyAsync(y, residual, bytes, cudaMemcpyDeviceToDevice, (cudaStream_t)stream) : (int)cudaMemsetAsync(y, 0, bytes, (cudaStream_t)stream);
   }
   DropoutArgs a;

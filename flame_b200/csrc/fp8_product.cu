@@ -907,6 +907,7 @@ QuantJob quant_job(const void* x, size_t rows, size_t cols, size_t x_stride, uin
 }
 cudaError_t launch_quant(const QuantJobs& jobs, cudaStream_t stream) {
   const uint64_t tiles = (uint64_t)jobs.job[0].tiles + jobs.job[1].tiles + jobs.job[2].tiles;
+  if (tiles > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
   return tiles == 0 ? cudaSuccess : launch_after(fp8_quant_kernel, (unsigned)tiles, kQuantThreads, 0, stream, jobs);
 }
 // Where a matrix's codes and scales lie in a workspace; moves `at` on.
@@ -920,6 +921,7 @@ Place take(uint8_t*& at, size_t rows, size_t cols, uint32_t mode) {
 enum class Product { kNtTiles, kNtRows, kNnTiles, kTnColumns };
 cudaError_t product(Product kind, const void* a, size_t a_stride, const void* sa, const void* b, size_t b_stride, const void* sb, void* c, size_t c_stride, bool f32,
                     size_t M, size_t N, size_t K, cudaStream_t s) {
+  if (blocks_of(M) * blocks_of(N) > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;      // a result of over 2^45 numbers
   if (K == 0) {   // an empty sum
     const size_t size = f32 ? 4 : 2;
     return cudaMemset2DAsync(c, c_stride * size, 0, N * size, M, s);

@@ -146,7 +146,7 @@ constexpr int kDepth = 8;
 constexpr size_t kRingBytes = (size_t)kDepth * kThreads * 16;
 template <int kN, int V, bool kBack, bool kWhole>
 struct Walk {
-  static constexpr int kD = V == 8 ? kDepth / kN : 1;      // rows on their way
+  [[maybe_unused]] static constexpr int kD = V == 8 ? kDepth / kN : 1;      // rows on their way
   const __nv_bfloat16* const (&src)[kN];
   uint4* ring;
   uint32_t mine, most, skip, at_shared;

@@ -101,6 +101,8 @@ def test_group_norm_entries():
 
 def test_dropout_entry():
     for args, text in (((FAKE, None, FAKE, 8, 0, 1.5, 1, None, 0, None), "p must be"), ((FAKE, None, FAKE, 8, 0, float("nan"), 1, None, 0, None), "p must be"),
-                       ((FAKE, None, FAKE, 8, 3, 0.5, 1, None, 0, None), "dtype"), ((None, None, FAKE, 8, 0, 0.5, 1, None, 0, None), "null")):
+                       ((FAKE, None, FAKE, 8, 3, 0.5, 1, None, 0, None), "dtype"), ((None, None, FAKE, 8, 0, 0.5, 1, None, 0, None), "null"),
+                       ((FAKE + 1, None, FAKE, 8, 0, 0.5, 1, None, 0, None), "misaligned"), ((FAKE, FAKE + 2, FAKE, 8, 1, 0.5, 1, None, 0, None), "misaligned"),
+                       ((FAKE, None, FAKE, 8, 0, 0.5, 1, FAKE + 4, 0, None), "misaligned")):
         refused(text, "flame_dropout", *args)
     assert _lib.lib().flame_dropout(None, None, None, 0, 0, 0.5, 1, None, 0, None) == 0
