@@ -12,7 +12,7 @@
 // distance D from the others, the block's n elements err by n 2^-24 D^2 at most in a sum that the outlier alone brings to D^2: n is a
 // chunk's here, some thousands, and would be a million with one shift for the sample.)  Blocks are then joined by their mean and sum of
 // squares about it (T. Chan, G. Golub, R. LeVeque, 1983): a cluster's through distributed shared memory, which leaves the second
-// launch a quarter of them to read; where there are many, a launch of a warp for each group joins them in between.  Everything is
+// launch a quarter of them to read; where there are many, a launch of a block for each group joins them in between.  Everything is
 // added in a fixed order, without atomics: the same inputs give the same bits.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -358,14 +358,23 @@ __device__ __forceinline__ float elements_of_part(const NormArgs& a, uint32_t i,
   return elements(a, g, slab * slab_width, slab_width, (i - slab * clusters) * rows, rows);
 }
 
-// The parts of a group joined by kLanes neighbouring threads, of which this is number k: forward mean and sum of squares of the whole,
+// The parts of a group joined by kLanes neighbouring threads (8, or the block), of which this is number k: forward mean and sum of squares of the whole,
 // backward the sums.
 template <bool kBackward, int kLanes>
 __device__ __forceinline__ float2 join_parts(const NormArgs& a, uint32_t b, uint32_t g, uint32_t k) {
   const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
   auto all = [](float v) {
 #pragma unroll
-    for (int d = 1; d < kLanes; d <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    for (int d = 1; d < (kLanes < 32 ? kLanes : 32); d <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    if constexpr (kLanes == kThreads) {
+      __shared__ float warps[kWarps];
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = warps[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) v += warps[w];
+    }
     return v;
   };
   const bool live = g < a.G;
@@ -485,13 +494,13 @@ __device__ __forceinline__ void finish_all(const NormArgs& a, uint32_t b, float2
   }
   __syncthreads();
 }
-// A warp for each group of sample blockIdx.y.
+// A block for each group of sample blockIdx.y.  (A warp for each took 19 us at 592 parts, waiting for one load after another.)
 template <bool kBackward>
 __global__ void __launch_bounds__(kThreads) group_finish_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
-  const uint32_t g = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y;
-  const float2 t = join_parts<kBackward, 32>(a, b, g, lane);
-  if (g < a.G && lane == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, t);
+  const uint32_t g = blockIdx.x, b = blockIdx.y;
+  const float2 t = join_parts<kBackward, kThreads>(a, b, g, threadIdx.x);
+  if (threadIdx.x == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, t);
 }
 
 // Codes of eight channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
@@ -830,7 +839,7 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
     constexpr int V = decltype(v)::value;
     cudaError_t e = launch(group_stats_kernel<V>, grid, true, sums, s, a);
     if (e != cudaSuccess) return e;
-    if (a.finished) e = launch(group_finish_kernel<false>, dim3((a.G + kWarps - 1) / kWarps, a.B), false, 0, s, a);
+    if (a.finished) e = launch(group_finish_kernel<false>, dim3(a.G, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
     if constexpr (V == 8) {
       if (a.codes) return launch(group_apply_kernel<8, true>, grid, false, groups, s, a);
@@ -874,7 +883,7 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
     constexpr int V = decltype(v)::value;
     cudaError_t e = launch(group_grad_sums_kernel<V>, grid, true, sums, s, a);
     if (e != cudaSuccess) return e;
-    if (a.finished) e = launch(group_finish_kernel<true>, dim3((a.G + kWarps - 1) / kWarps, a.B), false, 0, s, a);
+    if (a.finished) e = launch(group_finish_kernel<true>, dim3(a.G, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
     return launch(group_grad_apply_kernel<V>, more, false, groups, s, a);
   });
