@@ -718,12 +718,12 @@ Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, boo
   p.slabs = (nvec + kThreads - 1) / kThreads;
   // with slabs, a width that is a multiple of 16 vectors: a block of 128 channels lies in one slab
   p.slab_vecs = p.slabs == 1 ? nvec : kThreads;
-  // All the thread blocks that fit on the SMs at a time, with eight rows a thread at least.  Where each would have over 64, four times
+  // All the thread blocks that fit on the SMs at a time, with eight rows a thread at least.  Where each would have over 64, three times
   // as many: SMs differ in speed, and with one block for each place the slowest is waited for (1024 x 1024 x 128).
   const uint64_t places = (uint64_t)sms * (backward ? 3 : 4), samples = (uint64_t)B * p.slabs;
   uint64_t want = places / samples > 1 ? places / samples : 1;
   const uint32_t row_step = kThreads / p.slab_vecs;
-  if (L / (want * row_step) > 64) want = 4 * places / samples > 1 ? 4 * places / samples : 1;
+  if (L / (want * row_step) > 64) want = 3 * places / samples > 1 ? 3 * places / samples : 1;
   const uint64_t most = (L + (uint64_t)row_step * 8 - 1) / ((uint64_t)row_step * 8);
   uint64_t chunks = want < most ? want : most;
   if (chunks > 4096) chunks = 4096;
