@@ -136,25 +136,24 @@ __device__ __forceinline__ void store(__nv_bfloat16* p, const F2 (&f)[kPairs<V>]
 }
 
 // A thread's way down its rows, kN tensors at a time; kBack: from the last row to the first.  The constructor sends the first rows on
-// their way, run(f) calls f(offset, vectors, live) for each row, offset in elements from the thread's first row; with kWhole also,
-// with live = false, where another thread of the block has a row and this one has none (for shuffles inside f).
+// their way, run(f) calls f(offset, vectors) for each row, offset in elements from the thread's first row.
 //
 // The rows ahead are on their way to shared memory as asynchronous copies, each thread's own in places of its own, so nothing waits
 // for another thread and nothing is held in registers: with one row in flight in registers the two passes over 1024 x 1024 x 128
 // took 72 and 174 us, with four, which left two blocks on an SM, 76 and 152, this way 57 and 95.
 constexpr int kDepth = 8;
 constexpr size_t kRingBytes = (size_t)kDepth * kThreads * 16;
-template <int kN, int V, bool kBack, bool kWhole>
+template <int kN, int V, bool kBack>
 struct Walk {
   [[maybe_unused]] static constexpr int kD = V == 8 ? kDepth / kN : 1;      // rows on their way
   const __nv_bfloat16* const (&src)[kN];
   uint4* ring;
-  uint32_t mine, most, skip, at_shared;
+  uint32_t mine, at_shared;
   ptrdiff_t step, first, next;
 
   // the row of round n, into place j of the ring
   __device__ __forceinline__ void send(uint32_t n, int j) {
-    if (n < most && (!kWhole || (kBack ? n >= skip : n < mine))) {
+    if (n < mine) {
 #pragma unroll
       for (int k = 0; k < kN; ++k)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at_shared + (j * kN + k) * kThreads * 16), "l"(src[k] + next) : "memory");
@@ -164,10 +163,8 @@ struct Walk {
   }
   __device__ __forceinline__ Walk(const __nv_bfloat16* const (&s)[kN], uint32_t rows, uint32_t lane_row, uint32_t row_step, uint32_t C, uint4* r) : src(s), ring(r) {
     mine = rows > lane_row ? (rows - lane_row + row_step - 1) / row_step : 0;
-    most = kWhole ? (rows + row_step - 1) / row_step : mine;
     step = (kBack ? -1 : 1) * (ptrdiff_t)((size_t)row_step * C);
-    first = next = kBack ? -step * ((ptrdiff_t)most - 1) : 0;
-    skip = kBack ? most - mine : 0;      // rounds before this thread's first row, from the back
+    first = next = kBack ? -step * ((ptrdiff_t)mine - 1) : 0;
     at_shared = (uint32_t)__cvta_generic_to_shared(ring + threadIdx.x);
     if constexpr (V == 8) {
 #pragma unroll
@@ -178,31 +175,25 @@ struct Walk {
   __device__ __forceinline__ void run(F&& f) {
     ptrdiff_t at = first;
     if constexpr (V == 8) {
-      for (uint32_t n0 = 0; n0 < most; n0 += kD) {
+      for (uint32_t n0 = 0; n0 < mine; n0 += kD) {
 #pragma unroll
         for (int j = 0; j < kD; ++j) {      // a turn of the ring
-          if (n0 + j >= most) break;
+          if (n0 + j >= mine) break;
           asm volatile("cp.async.wait_group %0;" ::"n"(kD - 1) : "memory");
           Vec<V> v[kN];
-          const bool live = !kWhole || (kBack ? n0 + j >= skip : n0 + j < mine);
-          if (live) {
 #pragma unroll
-            for (int k = 0; k < kN; ++k) { const uint4 w = ring[(j * kN + k) * kThreads + threadIdx.x]; v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
-          }
-          f(at, v, live);
+          for (int k = 0; k < kN; ++k) { const uint4 w = ring[(j * kN + k) * kThreads + threadIdx.x]; v[k] = *reinterpret_cast<const Vec<V>*>(&w); }
+          f(at, v);
           at += step;
           send(n0 + j + kD, j);
         }
       }
     } else {
-      for (uint32_t n = 0; n < most; ++n, at += step) {
+      for (uint32_t n = 0; n < mine; ++n, at += step) {
         Vec<V> v[kN];
-        const bool live = !kWhole || (kBack ? n >= skip : n < mine);
-        if (live) {
 #pragma unroll
-          for (int k = 0; k < kN; ++k) v[k] = *reinterpret_cast<const Vec<V>*>(src[k] + at);
-        }
-        f(at, v, live);
+        for (int k = 0; k < kN; ++k) v[k] = *reinterpret_cast<const Vec<V>*>(src[k] + at);
+        f(at, v);
       }
     }
   }
@@ -412,15 +403,22 @@ __device__ __forceinline__ float2 join_parts(const NormArgs& a, uint32_t b, uint
   return make_float2(mean, all(q));
 }
 
+// Programmatic launches.  The first kernel lets the next one start when all its blocks have waited for what ran before them, so
+// the second kernel may read the call's inputs at once: whatever wrote them is done.  It sends its first rows on their way, past L1,
+// while the first kernel ends, and waits before it reads anything else or writes.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void wait_then_launch() { wait_for_earlier(); launch_next(); }
+
 template <int V>
 __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_constant__ NormArgs a) {
-  pdl_prologue();
+  wait_then_launch();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
   const __nv_bfloat16* xs = a.x + (size_t)p.b * a.L * a.C;
   const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
-  Walk<1, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
+  Walk<1, V, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   const __nv_bfloat16* first_row = xs + (p.rows ? p.row0 : 0) * a.C;      // the chunk's
   F2 shift[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the shift's negative
 #pragma unroll
@@ -433,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
     }
     shift[i] = F2(t.x, t.y);
   }
-  way.run([&](ptrdiff_t, const Vec<V>(&v)[1], bool) {
+  way.run([&](ptrdiff_t, const Vec<V>(&v)[1]) {
     F2 f[kPairs<V>];
     unpack<V>(v[0], f);
 #pragma unroll
@@ -503,11 +501,12 @@ __global__ void __launch_bounds__(kThreads) group_finish_kernel(const __grid_con
   if (threadIdx.x == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, t);
 }
 
-// Codes of eight channels a thread, 16 threads hold a block of 128 channels of a row (C a multiple of 128).
+// Codes of eight channels a thread.  16 neighbouring lanes hold a block of 128 channels of a row (C / 8 and a slab's width are multiples
+// of 16) and have the same rows; the other half of the warp may have one more.
 __device__ __forceinline__ uint2 encode_row_block(const uint4& raw, float& scale) {
   uint32_t m = max_abs2(max_abs2(raw.x, raw.y), max_abs2(raw.z, raw.w));
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) m = max_abs2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  for (int d = 8; d > 0; d >>= 1) m = max_abs2(m, __shfl_xor_sync(0xFFFFu << (threadIdx.x & 16), m, d));
   scale = fp8_scale_of(larger_of(m));
   float y[8];
   unpack8(raw, y);
@@ -533,41 +532,35 @@ __device__ __forceinline__ void load_params(const NormArgs& a, const Place<V>& p
 }
 
 template <int V, bool kCodes>
-__global__ void __launch_bounds__(kThreads, kCodes ? 3 : 4) group_apply_kernel(const __grid_constant__ NormArgs a) {
-  pdl_prologue();
+__global__ void __launch_bounds__(kThreads, 4) group_apply_kernel(const __grid_constant__ NormArgs a) {
+  launch_next();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
   const Place<V> p(a, true);
   // From the chunk's end to its start: what the first launch read last is still in L2.
-  // With codes, 16 neighbouring lanes share a row (C / 8 and the slab's width are multiples of 16): all of them are live or none is.
   const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
   const __nv_bfloat16* const src[1] = {a.x + first};
-  Walk<1, V, true, kCodes> way(src, kCodes || p.live ? p.rows : 0, p.live ? p.lane_row : 0xFFFFFFFFu, p.row_step, a.C, ring);
+  Walk<1, V, true> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
+  wait_for_earlier();
   finish_all<false>(a, p.b, sh);
   if (p.chunk == 0 && p.slab == 0 && a.finished == nullptr)
     for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) reinterpret_cast<float2*>(a.stats)[(size_t)p.b * a.G + g] = sh[g];
   F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>];      // the mean's negative
   load_params<V>(a, p, bias, [&](int i, float w, float2 t, float& m, float& s) { m = -t.x; s = t.y * w; }, sh, mean, scale);
-  way.run([&](ptrdiff_t at, const Vec<V>(&v)[1], bool live) {
+  way.run([&](ptrdiff_t at, const Vec<V>(&v)[1]) {
     F2 f[kPairs<V>];
-#pragma unroll
-    for (int i = 0; i < kPairs<V>; ++i) f[i] = F2(0.0f, 0.0f);
-    if (live) unpack<V>(v[0], f);
+    unpack<V>(v[0], f);
 #pragma unroll
     for (int i = 0; i < kPairs<V>; ++i) {
       const F2 h = fma(add(f[i], mean[i]), scale[i], bias[i]);      // first the difference: a group of equal values gives exactly the bias
       f[i] = a.silu ? mul(h, sigmoid(h)) : h;
     }
-    if (live) store<V>(a.y + first + at, f, a.stream);
+    store<V>(a.y + first + at, f, a.stream);
     if constexpr (kCodes) {
       // the codes are those of the BF16 output
-      const uint4 raw = live ? make_uint4(to_bf16x2(f[0]), to_bf16x2(f[1]), to_bf16x2(f[2]), to_bf16x2(f[3])) : make_uint4(0u, 0u, 0u, 0u);
       float s;
-      const uint2 c = encode_row_block(raw, s);
-      if (live) {
-        *reinterpret_cast<uint2*>(a.codes + first + at) = c;
-        if ((p.vec & 15) == 0) a.code_scales[(first + at) / 128] = s;
-      }
+      *reinterpret_cast<uint2*>(a.codes + first + at) = encode_row_block(make_uint4(to_bf16x2(f[0]), to_bf16x2(f[1]), to_bf16x2(f[2]), to_bf16x2(f[3])), s);
+      if ((p.vec & 15) == 0) a.code_scales[(first + at) / 128] = s;
     }
   });
 }
@@ -581,19 +574,19 @@ __device__ __forceinline__ F2 grad_h(F2 h, F2 dy, int silu) {
 
 template <int V>
 __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __grid_constant__ NormArgs a) {
-  pdl_prologue();
+  wait_then_launch();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
   const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
   const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
-  Walk<2, V, false, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
+  Walk<2, V, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the mean's negative
   load_params<V>(a, p, bias, [&](int, float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, stats, mean, scale);
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) s[i] = q[i] = F2(0.0f, 0.0f);
-  way.run([&](ptrdiff_t, const Vec<V>(&v)[2], bool) {
+  way.run([&](ptrdiff_t, const Vec<V>(&v)[2]) {
     F2 x[kPairs<V>], dy[kPairs<V>];
     unpack<V>(v[0], x);
     unpack<V>(v[1], dy);
@@ -628,10 +621,11 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
 // The blocks of one more sample than there are add the channel sums up to dweight and dbias.
 template <int V>
 __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __grid_constant__ NormArgs a) {
-  pdl_prologue();
+  launch_next();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
   if (blockIdx.z == a.B) {
+    wait_for_earlier();
     // a warp's 32 lanes take 32 neighbouring channels, the eight warps every eighth part
     __shared__ float2 part[kWarps][32];
     const uint32_t lane = threadIdx.x & 31, wp = threadIdx.x >> 5, parts = a.B * (a.chunks / kCluster);
@@ -665,7 +659,8 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
   const Place<V> p(a, true);
   const size_t first = ((size_t)p.b * a.L + p.row0 + p.lane_row) * a.C + p.c0;
   const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
-  Walk<2, V, true, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);      // from the chunk's end, as in the forward pass
+  Walk<2, V, true> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);      // from the chunk's end, as in the forward pass
+  wait_for_earlier();
   finish_all<true>(a, p.b, sh);
   // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
@@ -686,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
     slope[i] = F2(sl[0], sl[1]);
     rest[i] = F2(re[0], re[1]);
   }
-  way.run([&](ptrdiff_t at, const Vec<V>(&v)[2], bool) {
+  way.run([&](ptrdiff_t at, const Vec<V>(&v)[2]) {
     F2 x[kPairs<V>], dy[kPairs<V>];
     unpack<V>(v[0], x);
     unpack<V>(v[1], dy);
@@ -715,9 +710,15 @@ Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, boo
   Plan p;
   p.V = (C % 8 == 0 && aligned16) ? 8 : (C % 2 == 0 && aligned4) ? 2 : 1;
   const uint32_t nvec = C / p.V;
-  p.slabs = (nvec + kThreads - 1) / kThreads;
-  // with slabs, a width that is a multiple of 16 vectors: a block of 128 channels lies in one slab
-  p.slab_vecs = p.slabs == 1 ? nvec : kThreads;
+  // The width of a slab: the one that leaves the fewest threads without a channel, at 1280 channels 80 vectors (three rows in 256
+  // threads) and not 160 (one).  With slabs it is a multiple of 16 vectors: a block of 128 channels lies in one of them.
+  uint32_t best = 0;
+  for (uint32_t slabs = (nvec + kThreads - 1) / kThreads, k = 0; k < 4; ++slabs, ++k) {
+    const uint32_t even = (nvec + slabs - 1) / slabs, width = slabs == 1 ? even : (even + 15) / 16 * 16;
+    if (width > kThreads || (k > 0 && width < 64)) continue;      // 1024 neighbouring bytes at least
+    const uint32_t count = (nvec + width - 1) / width, used = nvec * (kThreads / width) * 1024 / (count * kThreads);   // of 1024
+    if (used > best + 64 * (best > 0)) { best = used; p.slabs = count; p.slab_vecs = width; }
+  }
   // All the thread blocks that fit on the SMs at a time, with eight rows a thread at least.  Where each would have over 64, three times
   // as many: SMs differ in speed, and with one block for each place the slowest is waited for (1024 x 1024 x 128).
   const uint64_t places = (uint64_t)sms * (backward ? 3 : 4), samples = (uint64_t)B * p.slabs;
