@@ -7,10 +7,10 @@
 //
 // Two launches each way: the first reduces, the second applies.  A thread owns V neighbouring channels and walks down the
 // positions of its chunk, so that a warp reads whole lines of the channels-last rows, and per-channel sums stay in registers.
-// A block's forward sums are kept about a shift, the group's first element in its chunk: x - shift is of the size of the spread and not of
-// the mean, so that sums of squares lose nothing when the mean is large against the spread.  (Where that element is an outlier, at a
-// distance D from the others, the block's n elements err by n 2^-24 D^2 at most in a sum that the outlier alone brings to D^2: n is a
-// chunk's here, some thousands, and would be a million with one shift for the sample.)  Blocks are then joined by their mean and sum of
+// A block's forward sums are kept about a shift, the median of the group's first elements in the first, middle and last row of its chunk:
+// x - shift is of the size of the spread and not of the mean, so that sums of squares lose nothing when the mean is large against the
+// spread.  (The first element alone may be an outlier, at a distance D from the others: the chunk's n elements, some thousands, then
+// sum to n D^2 and err by n 2^-24 D^2, where the outlier's own share of the variance is D^2.)  Blocks are then joined by their mean and sum of
 // squares about it (T. Chan, G. Golub, R. LeVeque, 1983): a cluster's through distributed shared memory, which leaves the second
 // launch a quarter of them to read; where there are many, a launch of a block for each group joins them in between.  Everything is
 // added in a fixed order, without atomics: the same inputs give the same bits.
@@ -31,6 +31,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr uint32_t kCluster = 4;
+// Over 64 parts the blocks of the second launch would spend longer on joining them than a launch between the two takes.
+constexpr uint32_t kMostParts = 64;
 
 struct NormArgs {
   const __nv_bfloat16* x;
@@ -227,12 +229,6 @@ __device__ __forceinline__ void params(const void* p, int f32, uint32_t c, float
   }
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-  return v;
-}
-
 // Shared memory: the ring (vectors of eight channels only), then pairs of sums.
 template <int V>
 __device__ __forceinline__ float2* sums_of(uint4* ring) { return reinterpret_cast<float2*>(ring + (V == 8 ? kRingBytes / 16 : 0)); }
@@ -318,40 +314,54 @@ __device__ __forceinline__ float2 add_up(const float2 (&v)[kCluster]) {
   for (uint32_t k = 1; k < kCluster; ++k) { t.x += v[k].x; t.y += v[k].y; }
   return t;
 }
-// The slab's channel sums, weighted, added up to the groups that the slab touches: a thread a group, a warp where groups are wide.
+// The slab's channel sums, weighted, added up to the groups that the slab touches: one, eight or 32 lanes a group.  (20 channels took
+// one thread 1.2 us, 30 cycles for each word from shared memory.)
 template <typename F, typename D>
 __device__ __forceinline__ void join_channels(const NormArgs& a, uint32_t slab_c0, uint32_t width, float2* groups, F&& pair, D&& done) {
-  const uint32_t lane = threadIdx.x & 31;
-  const bool warps = a.cg > 32;
-  for (uint32_t g = warps ? threadIdx.x >> 5 : threadIdx.x; g < a.G; g += warps ? kWarps : kThreads) {
+  const uint32_t lanes = a.cg > 32 ? 32 : a.cg > 8 ? 8 : 1, lane = threadIdx.x & (lanes - 1);
+  for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / lanes) {
+    const uint32_t g = g0 + threadIdx.x / lanes;
     const uint32_t lo = g * a.cg > slab_c0 ? g * a.cg : slab_c0;
     const uint32_t hi = (g + 1) * a.cg < slab_c0 + width ? (g + 1) * a.cg : slab_c0 + width;
     float s = 0.0f, q = 0.0f;
-    for (uint32_t c = warps ? lo + lane : lo; c < hi; c += warps ? 32 : 1) {
-      const float2 t = pair(c);
-      s += t.x;
-      q += t.y;
+    if (g < a.G) {
+      for (uint32_t c = lo + lane; c < hi; c += lanes) {
+        const float2 t = pair(c);
+        s += t.x;
+        q += t.y;
+      }
     }
-    if (warps) { s = warp_sum(s); q = warp_sum(q); }
-    if (!warps || lane == 0) groups[g] = done(g, s, q);
+    for (uint32_t d = lanes / 2; d > 0; d >>= 1) {
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+      q += __shfl_xor_sync(0xFFFFFFFFu, q, d);
+    }
+    if (g < a.G && lane == 0) groups[g] = done(g, s, q);
   }
 }
 // Elements of group g in channels [c0, c0 + width) and the rows from row0 on, `most` of them at the most.
 __device__ __forceinline__ float elements(const NormArgs& a, uint32_t g, uint32_t c0, uint32_t width, uint64_t row0, uint64_t most) {
   const uint32_t lo = g * a.cg > c0 ? g * a.cg : c0, hi = (g + 1) * a.cg < c0 + width ? (g + 1) * a.cg : c0 + width;
   const uint64_t left = a.L > row0 ? a.L - row0 : 0;
-  return lo < hi ? (float)(hi - lo) * (float)(left < most ? left : most) : 0.0f;
+  return lo < hi ? (float)(hi - lo) * (float)(uint32_t)(left < most ? left : most) : 0.0f;      // L is under 2^31
 }
-// Those of part i of a sample (a cluster's): i counts the clusters of a slab first.
+// Those of part i of a sample (a cluster's): i counts the clusters of a slab first.  Every cluster's first block has rows, so 32 bits hold them.
 __device__ __forceinline__ float elements_of_part(const NormArgs& a, uint32_t i, uint32_t g, uint32_t slab_width) {
-  const uint32_t clusters = a.chunks / kCluster, slab = a.slabs == 1 ? 0 : i / clusters;
-  const uint64_t rows = (uint64_t)a.rows_per_chunk * kCluster;
-  return elements(a, g, slab * slab_width, slab_width, (i - slab * clusters) * rows, rows);
+  uint32_t channels = a.cg;
+  if (a.slabs > 1) {
+    const uint32_t clusters = a.chunks / kCluster, slab = i / clusters, c0 = slab * slab_width;
+    const uint32_t lo = g * a.cg > c0 ? g * a.cg : c0, hi = (g + 1) * a.cg < c0 + slab_width ? (g + 1) * a.cg : c0 + slab_width;
+    if (lo >= hi) return 0.0f;
+    channels = hi - lo;
+    i -= slab * clusters;
+  }
+  const uint32_t rows = a.rows_per_chunk * kCluster, left = (uint32_t)a.L - i * rows;
+  return (float)channels * (float)(left < rows ? left : rows);
 }
 
-// The parts of a group joined by kLanes neighbouring threads (8, or the block), of which this is number k: forward mean and sum of squares of the whole,
-// backward the sums.
-template <bool kBackward, int kLanes>
+// The parts of a group joined by kLanes neighbouring threads, of which this is number k, kHeld parts a thread at a time: forward mean
+// and sum of squares of the whole, backward the sums.  Eight threads hold the 64 parts that there can be without a launch between:
+// read once, together (2 x 4096 x 640: 4.5 -> 2 us of the second launch).
+template <bool kBackward, int kLanes, int kHeld>
 __device__ __forceinline__ float2 join_parts(const NormArgs& a, uint32_t b, uint32_t g, uint32_t k) {
   const float2* in = a.partial + (size_t)b * a.parts * a.G + g;
   auto all = [](float v) {
@@ -368,36 +378,42 @@ __device__ __forceinline__ float2 join_parts(const NormArgs& a, uint32_t b, uint
     }
     return v;
   };
-  const bool live = g < a.G;
-  float s = 0.0f, q = 0.0f;
-  if (kBackward) {
-    if (live) {
-#pragma unroll 4
-      for (uint32_t i = k; i < a.parts; i += kLanes) {
-        const float2 t = in[(size_t)i * a.G];
-        s += t.x;
-        q += t.y;
-      }
-    }
-    return make_float2(all(s), all(q));
-  }
+  const uint32_t parts = g < a.G ? a.parts : 0;
   const uint32_t slab_width = a.slabs == 1 ? a.C : a.slab_vecs * a.V;
   // a part that has elements of the group: the first of its first slab
-  const float shift = live ? in[(size_t)(a.slabs == 1 ? 0 : g * a.cg / slab_width * (a.chunks / kCluster)) * a.G].x : 0.0f;
-  if (live) {
-#pragma unroll 4
-    for (uint32_t i = k; i < a.parts; i += kLanes) {
-      const float n = elements_of_part(a, i, g, slab_width);
-      if (n > 0.0f) s += n * (in[(size_t)i * a.G].x - shift);
+  const float shift = !kBackward && parts ? in[(size_t)(a.slabs == 1 ? 0 : g * a.cg / slab_width * (a.chunks / kCluster)) * a.G].x : 0.0f;
+  float2 t[kHeld];
+  auto read = [&](uint32_t i0) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const uint32_t i = i0 + j * kLanes;
+      t[j] = i < parts ? in[(size_t)i * a.G] : make_float2(0.0f, 0.0f);
+    }
+  };
+  auto elements_at = [&](uint32_t i) { return i < parts ? elements_of_part(a, i, g, slab_width) : 0.0f; };
+  float s = 0.0f, q = 0.0f;
+  for (uint32_t i0 = k; i0 < parts; i0 += kHeld * kLanes) {
+    read(i0);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (kBackward) {
+        s += t[j].x;
+        q += t[j].y;
+      } else {
+        const float n = elements_at(i0 + j * kLanes);
+        if (n > 0.0f) s += n * (t[j].x - shift);
+      }
     }
   }
-  const float mean = shift + all(s) / ((float)a.L * (float)a.cg);
-  if (live) {
-#pragma unroll 4
-    for (uint32_t i = k; i < a.parts; i += kLanes) {
-      const float n = elements_of_part(a, i, g, slab_width);
-      const float2 t = in[(size_t)i * a.G];
-      if (n > 0.0f) q += fmaf(n * (t.x - mean), t.x - mean, t.y);
+  s = all(s);
+  if (kBackward) return make_float2(s, all(q));
+  const float mean = shift + s / ((float)a.L * (float)a.cg);
+  for (uint32_t i0 = k; i0 < parts; i0 += kHeld * kLanes) {
+    if (kLanes == kThreads) read(i0);      // eight threads hold them all
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const float n = elements_at(i0 + j * kLanes);
+      if (n > 0.0f) q += fmaf(n * (t[j].x - mean), t[j].x - mean, t[j].y);
     }
   }
   return make_float2(mean, all(q));
@@ -420,14 +436,26 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
   const __nv_bfloat16* const src[1] = {xs + (p.row0 + p.lane_row) * a.C + p.c0};
   Walk<1, V, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   const __nv_bfloat16* first_row = xs + (p.rows ? p.row0 : 0) * a.C;      // the chunk's
+  const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
+  const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
+  float2* groups = sh + kThreads * V;
+  float* shifts = reinterpret_cast<float*>(groups + a.G);
+  const uint32_t g_end = (slab_c0 + width - 1) / a.cg + 1;
+  for (uint32_t g = slab_c0 / a.cg + threadIdx.x; g < g_end; g += kThreads) {
+    const __nv_bfloat16* at = first_row + g * a.cg;
+    const uint32_t last = p.rows ? p.rows - 1 : 0;
+    const float u = __bfloat162float(*at), v = __bfloat162float(at[(size_t)(last / 2) * a.C]), w = __bfloat162float(at[(size_t)last * a.C]);
+    shifts[g] = fmaxf(fminf(u, v), fminf(fmaxf(u, v), w));
+  }
+  __syncthreads();
   F2 shift[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the shift's negative
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) {
     s[i] = q[i] = F2(0.0f, 0.0f);
     float2 t = make_float2(0.0f, 0.0f);
     if (p.live) {
-      t.x = -__bfloat162float(first_row[group_of(p.c0 + 2 * i, a.by_cg) * a.cg]);
-      if (V > 1) t.y = -__bfloat162float(first_row[group_of(p.c0 + 2 * i + 1, a.by_cg) * a.cg]);
+      t.x = -shifts[group_of(p.c0 + 2 * i, a.by_cg)];
+      if (V > 1) t.y = -shifts[group_of(p.c0 + 2 * i + 1, a.by_cg)];
     }
     shift[i] = F2(t.x, t.y);
   }
@@ -441,16 +469,13 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
       q[i] = fma(d, d, q[i]);
     }
   });
-  const uint32_t slab_c0 = p.slab * a.slab_vecs * V;
-  const uint32_t width = a.C - slab_c0 < a.slab_vecs * V ? a.C - slab_c0 : a.slab_vecs * V;
   join_rows<V>(p, s, q, sh, width);
-  float2* groups = sh + kThreads * V;
   join_channels(a, slab_c0, width, groups, [&](uint32_t c) { return sh[place_of<V>(c - slab_c0, width)]; }, [&](uint32_t g, float sum, float sum2) {
     const float n = elements(a, g, slab_c0, width, p.row0, p.rows);
     if (n == 0.0f) return make_float2(0.0f, 0.0f);
     const float off = sum / n;
     // fmaxf would turn the NaN of a NaN or an infinity into 0
-    return make_float2(__bfloat162float(first_row[g * a.cg]) + off, sum2 < INFINITY ? fmaxf(sum2 - sum * off, 0.0f) : NAN);
+    return make_float2(shifts[g] + off, sum2 < INFINITY ? fmaxf(sum2 - sum * off, 0.0f) : NAN);
   });
   // mean and sum of squares of the cluster's blocks, joined
   join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G, [](uint32_t i) { return i; },
@@ -486,7 +511,7 @@ __device__ __forceinline__ void finish_all(const NormArgs& a, uint32_t b, float2
   } else {
     for (uint32_t g0 = 0; g0 < a.G; g0 += kThreads / 8) {      // eight threads a group
       const uint32_t g = g0 + threadIdx.x / 8;
-      const float2 t = join_parts<kBackward, 8>(a, b, g, threadIdx.x % 8);
+      const float2 t = join_parts<kBackward, 8, kMostParts / 8>(a, b, g, threadIdx.x % 8);
       if (g < a.G && threadIdx.x % 8 == 0) out[g] = finish<kBackward>(a, t);
     }
   }
@@ -497,7 +522,7 @@ template <bool kBackward>
 __global__ void __launch_bounds__(kThreads) group_finish_kernel(const __grid_constant__ NormArgs a) {
   pdl_prologue();
   const uint32_t g = blockIdx.x, b = blockIdx.y;
-  const float2 t = join_parts<kBackward, kThreads>(a, b, g, threadIdx.x);
+  const float2 t = join_parts<kBackward, kThreads, 1>(a, b, g, threadIdx.x);
   if (threadIdx.x == 0) a.finished[(size_t)b * a.G + g] = finish<kBackward>(a, t);
 }
 
@@ -513,23 +538,30 @@ __device__ __forceinline__ uint2 encode_row_block(const uint4& raw, float& scale
   return fp8_encode8(y, scale, fp8_factor_of(scale));
 }
 
-// Bias of a thread's channels, and whatever f makes of the weight and the group's statistics of each.
-template <int V, typename F>
-__device__ __forceinline__ void load_params(const NormArgs& a, const Place<V>& p, F2 (&bias)[kPairs<V>], F&& f, const float2* stats, F2 (&u)[kPairs<V>], F2 (&v)[kPairs<V>]) {
-  float w[2 * kPairs<V>] = {}, b[2 * kPairs<V>] = {}, fu[2 * kPairs<V>] = {}, fv[2 * kPairs<V>] = {};
-  if (p.live) {
+// Weight and bias of a thread's channels, and (with) whatever f makes of the weight and the group's statistics of each.
+template <int V>
+struct Params {
+  float w[2 * kPairs<V>] = {}, b[2 * kPairs<V>] = {};
+  __device__ __forceinline__ Params(const NormArgs& a, const Place<V>& p) {
+    if (!p.live) return;
     params<V>(a.weight, a.params_f32, p.c0, 1.0f, reinterpret_cast<float(&)[V]>(w));
     params<V>(a.bias, a.params_f32, p.c0, 0.0f, reinterpret_cast<float(&)[V]>(b));
-#pragma unroll
-    for (int i = 0; i < V; ++i) f(i, w[i], stats[group_of(p.c0 + i, a.by_cg)], fu[i], fv[i]);
   }
+  template <typename F>
+  __device__ __forceinline__ void with(const NormArgs& a, const Place<V>& p, const float2* stats, F&& f, F2 (&bias)[kPairs<V>], F2 (&u)[kPairs<V>], F2 (&v)[kPairs<V>]) const {
+    float fu[2 * kPairs<V>] = {}, fv[2 * kPairs<V>] = {};
+    if (p.live) {
 #pragma unroll
-  for (int i = 0; i < kPairs<V>; ++i) {
-    bias[i] = F2(b[2 * i], b[2 * i + 1]);
-    u[i] = F2(fu[2 * i], fu[2 * i + 1]);
-    v[i] = F2(fv[2 * i], fv[2 * i + 1]);
+      for (int i = 0; i < V; ++i) f(w[i], stats[group_of(p.c0 + i, a.by_cg)], fu[i], fv[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) {
+      bias[i] = F2(b[2 * i], b[2 * i + 1]);
+      u[i] = F2(fu[2 * i], fu[2 * i + 1]);
+      v[i] = F2(fv[2 * i], fv[2 * i + 1]);
+    }
   }
-}
+};
 
 template <int V, bool kCodes>
 __global__ void __launch_bounds__(kThreads, 4) group_apply_kernel(const __grid_constant__ NormArgs a) {
@@ -543,10 +575,11 @@ __global__ void __launch_bounds__(kThreads, 4) group_apply_kernel(const __grid_c
   Walk<1, V, true> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   wait_for_earlier();
   finish_all<false>(a, p.b, sh);
+  const Params<V> params(a, p);
   if (p.chunk == 0 && p.slab == 0 && a.finished == nullptr)
     for (uint32_t g = threadIdx.x; g < a.G; g += kThreads) reinterpret_cast<float2*>(a.stats)[(size_t)p.b * a.G + g] = sh[g];
   F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>];      // the mean's negative
-  load_params<V>(a, p, bias, [&](int i, float w, float2 t, float& m, float& s) { m = -t.x; s = t.y * w; }, sh, mean, scale);
+  params.with(a, p, sh, [](float w, float2 t, float& m, float& s) { m = -t.x; s = t.y * w; }, bias, mean, scale);
   way.run([&](ptrdiff_t at, const Vec<V>(&v)[1]) {
     F2 f[kPairs<V>];
     unpack<V>(v[0], f);
@@ -583,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
   const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
   Walk<2, V, false> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);
   F2 mean[kPairs<V>], scale[kPairs<V>], bias[kPairs<V>], s[kPairs<V>], q[kPairs<V>];      // the mean's negative
-  load_params<V>(a, p, bias, [&](int, float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, stats, mean, scale);
+  Params<V>(a, p).with(a, p, stats, [](float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, bias, mean, scale);
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) s[i] = q[i] = F2(0.0f, 0.0f);
   way.run([&](ptrdiff_t, const Vec<V>(&v)[2]) {
@@ -661,11 +694,12 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
   const __nv_bfloat16* const src[2] = {a.x + first, a.dy + first};
   Walk<2, V, true> way(src, p.live ? p.rows : 0, p.lane_row, p.row_step, a.C, ring);      // from the chunk's end, as in the forward pass
   wait_for_earlier();
+  const Params<V> params(a, p);
   finish_all<true>(a, p.b, sh);
   // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
   F2 scale[kPairs<V>], offset[kPairs<V>], slope[kPairs<V>], rest[kPairs<V>], mean[kPairs<V>];
-  load_params<V>(a, p, offset, [&](int, float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, stats, mean, scale);
+  params.with(a, p, stats, [](float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, offset, mean, scale);
   if (!p.live) return;
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) {
@@ -735,8 +769,7 @@ Plan plan(uint32_t B, uint64_t L, uint32_t C, bool aligned16, bool aligned4, boo
   p.parts = p.chunks / kCluster * p.slabs;
   return p;
 }
-// Over 64 parts the blocks of the second launch would spend longer on adding them up than a launch takes.
-bool finishes(const Plan& p) { return p.parts > 64; }
+bool finishes(const Plan& p) { return p.parts > kMostParts; }
 size_t group_pairs(const Plan& p, uint32_t B, uint32_t G) { return ((size_t)B * p.parts * G + 1) / 2 * 2; }   // whole 16 bytes
 size_t partial_pairs(const Plan& p, uint32_t B, uint32_t C, uint32_t G, bool backward) {
   return group_pairs(p, B, G) + (backward ? (size_t)B * (p.chunks / kCluster) * C : 0) + (finishes(p) && backward ? (size_t)B * G : 0);
@@ -835,10 +868,11 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   a.eps = eps; a.silu = activation == FLAME_ACTIVATION_SILU; a.stream = B * L * C > (24u << 20); a.params_f32 = param_dtype == FLAME_OFFLOAD_DTYPE_F32;
   const dim3 grid(p.chunks, p.slabs, (unsigned)B);
   const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
+  const size_t sums_and_shifts = sums + G * sizeof(float);
   cudaStream_t s = (cudaStream_t)stream;
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    cudaError_t e = launch(group_stats_kernel<V>, grid, true, sums, s, a);
+    cudaError_t e = launch(group_stats_kernel<V>, grid, true, sums_and_shifts, s, a);
     if (e != cudaSuccess) return e;
     if (a.finished) e = launch(group_finish_kernel<false>, dim3(a.G, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
