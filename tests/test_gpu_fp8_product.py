@@ -298,6 +298,51 @@ def test_a_training_step_recorded_in_a_graph(cuda_device):
     assert all(torch.equal(p, q) for p, q in zip(got, step(x, w)))
 
 
+@pytest.mark.parametrize("m,n,k", [(4608, 2304, 1152), (1000, 713, 1331), (130, 515, 257), (1, 256, 128)])
+def test_gradients_beside_each_other_read_this_steps_codes(cuda_device, m, n, k):
+    """The weight gradient's product may begin while the input gradient's ends.  Steps with other numbers in the same memory, without a
+    pause between them, eager and replayed: each equals the products of separately made codes, bit for bit."""
+    g = torch.Generator(device=cuda_device).manual_seed(m)
+    steps = [[torch.randn(s, device=cuda_device, generator=g).mul(4.0 ** (i - 2)).to(torch.bfloat16) for s in ((m, k), (n, k), (m, n))] for i in range(5)]
+    x, w, dy = (torch.empty_like(t) for t in steps[0])
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+
+    def step(i=None):
+        with torch.no_grad():
+            if i is not None:
+                for d, t in zip((x, w, dy), steps[i]):
+                    d.copy_(t)
+        return torch.autograd.grad(fp8_linear(x, w), (x, w), dy)
+
+    def wanted(i):
+        a, b, c = steps[i]
+        rows, columns = quantize_fp8_both(c)
+        return fp8_matmul(rows, quantize_fp8(b, "tiles")), fp8_matmul(columns, quantize_fp8(a, "columns"))
+
+    eager = [step(i) for i in range(5)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    replayed = []
+    for i in range(5):
+        with torch.no_grad():
+            for d, t in zip((x, w, dy), steps[i]):
+                d.copy_(t)
+        graph.replay()
+        replayed.append([t.clone() for t in out])
+    for i in range(5):
+        want = wanted(i)
+        for got in (eager[i], replayed[i]):
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
 def test_no_wait_ran_out(cuda_device):
     import ctypes
     n = ctypes.c_uint(7)
