@@ -232,13 +232,18 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 // Operands lie in shared memory as they lie in global memory: along the contraction (K-major) or along the rows of C (MN-major,
 // the weight of the input gradient and both operands of the weight gradient), which the matrix descriptor says; nothing is
 // transposed.  A block's sum is scaled by one fused multiply-add a number, which is why each block needs an accumulator of its own
-// in tensor memory: they take turns, so that the tensor cores work on one while another is read.  The way from a product's end over
-// the epilogue to the accumulator's next use takes some 1,000 cycles, a block's product 256 to 512: four accumulators of 128 columns
-// hide it, two of 256 (all that tensor memory holds) nearly do.
+// in tensor memory: they take turns, so that the tensor cores work on one while another is read.
+//
+// What bounds it, at 8192^3 on one B200 (a pair's block of 128 is 541 cycles of products): copies and products alone take 333 us, 3.3
+// PFLOP/s; with the accumulators handed to an epilogue that does nothing 383; as it is 470 (2.34 PFLOP/s) with a scale for 128 columns
+// and 654 with one for each.  From a product's end to the epilogue's start pass some 420 cycles, from its release to the next product's
+// start 270, between them the reading, during which products are slower: two accumulators, all that tensor memory holds, hide most of
+// it.  Halves of 128 columns in four accumulators took 620 us, sixteen epilogue warps 500 to 510.  In loops of seconds the power limit
+// of the board comes first (1.7 GHz).
 //
 // Two forms.  kPair, for many tiles: the two SMs of a pair work on one tile of 256 x 256 (cta_group::2), each holds half of either
 // operand, the leader issues the products for both.  Without it a block has a tile of 128 x 128, and where tiles are few (serving,
-// one token) a cluster of up to eight blocks shares one: each takes a range of the contraction, and their sums are joined through
+// one token) a cluster of two or four blocks shares one: each takes a range of the contraction, and their sums are joined through
 // distributed shared memory in the order of the ranks.
 //
 // Every wait gives up after two seconds: the kernel then counts the fault (flame_fp8_product_faults), leaves its copies time to land
@@ -350,19 +355,20 @@ __device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool live)
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4u : 0u) : "memory");
 }
 
-// 16 numbers of each lane, there when tmem_wait() has returned.  With a scale for 128 columns a thread takes 16 columns of one row.  With
-// a scale for each column it takes the layout of 16 x 8 fragments, columns 2 (lane % 4), + 1 of rows lane / 4, + 8 in each of four
+// Numbers of each lane, there when tmem_wait() has returned.  With a scale for 128 columns a thread takes 64 columns of one row.  With a
+// scale for each column it takes the layout of 16 x 8 fragments, columns 2 (lane % 4), + 1 of rows lane / 4, + 8 in each of four
 // fragments: a thread then needs the scales of a quarter of the columns, and reading them for every lane took as long as the products
 // (128 bytes a cycle come from shared memory, whether or not the lanes ask for the same).
-template <bool kFragments>
-__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
-  if constexpr (kFragments)
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
-  else
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr) : "memory");
+#define FLAME_R8(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+__device__ __forceinline__ void tmem_load_row(uint32_t (&r)[64], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+               "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+               : FLAME_R8(0), FLAME_R8(8), FLAME_R8(16), FLAME_R8(24), FLAME_R8(32), FLAME_R8(40), FLAME_R8(48), FLAME_R8(56) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void tmem_load_fragments(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];" : FLAME_R8(0), FLAME_R8(8) : "r"(addr) : "memory");
+}
+#undef FLAME_R8
 // The loads issued so far are done.  What uses them is volatile like this and like the loads, so that the three stay in order.
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
@@ -390,6 +396,11 @@ __device__ __forceinline__ void add_scaled_fragments(uint64_t* acc, const uint32
                  : "+l"(acc[2 * f]), "+l"(acc[2 * f + 1]), "+l"(acc[2 * f + 2]), "+l"(acc[2 * f + 3])
                  : "r"(x[4 * f]), "r"(x[4 * f + 1]), "r"(x[4 * f + 2]), "r"(x[4 * f + 3]), "r"(x[4 * f + 4]), "r"(x[4 * f + 5]), "r"(x[4 * f + 6]), "r"(x[4 * f + 7]),
                    "l"(t[f]), "l"(t[f + 1]), "l"(s_up), "l"(s_down));
+}
+__device__ __forceinline__ bool elect_one() {      // true in one lane of a whole warp
+  uint32_t r;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+  return r != 0;
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -447,10 +458,11 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const uint32_t base = smem_addr(smem);
   const uint32_t bars = base + S::kOffBars;
   auto full = [&](uint32_t s) { return bars + 8 * s; };
-  auto empty = [&](uint32_t s) { return bars + 8 * (kStages + s); };
-  auto acc_full = [&](uint32_t b) { return bars + 8 * (2 * kStages + b); };
-  auto acc_empty = [&](uint32_t b) { return bars + 8 * (2 * kStages + 4 + b); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffBars + 8 * (2 * kStages + 8));
+  // One barrier says that a block's products are done, to the copies, which then may fill its stage again, as well as to the epilogue.
+  // It counts the arrival of the block's scales too.
+  auto done = [&](uint32_t s) { return bars + 8 * (kStages + s); };
+  auto acc_empty = [&](uint32_t b) { return bars + 8 * (2 * kStages + b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kOffBars + 8 * (2 * kStages + 4));
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t group = cluster_size(), rank = cluster_rank();  // a pair, or the blocks that share a tile's contraction
@@ -462,9 +474,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   bool ok = true;
 
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < kStages; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
-    // an accumulator is full when the products are done and the block's scales are there
-    for (uint32_t b = 0; b < kAccs; ++b) { bar_init(acc_full(b), 2); bar_init(acc_empty(b), kPair ? 2 * kEpiWarps : kEpiWarps); }
+    for (uint32_t s = 0; s < kStages; ++s) { bar_init(full(s), 1); bar_init(done(s), 2); }
+    for (uint32_t b = 0; b < kAccs; ++b) bar_init(acc_empty(b), kPair ? 2 * kEpiWarps : kEpiWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -492,9 +503,9 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // The epilogue's sums need more registers than an equal share: 384 threads start with 168 each, 64,512 together; four warps go down
-  // to 88 and eight up to 208, 64,512 again.
+  // to 72 and eight up to 216, 64,512 again.
   if (warp < kEpiWarps) {
-    if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if constexpr (kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const uint32_t quarter = warp & 3, col_off = (warp >> 2) * kCols;
     const uint32_t row = quarter * 32 + lane;
     const uint32_t release = at_rank(acc_empty(0), kPair ? 0 : rank);
@@ -510,45 +521,51 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       for (int i = 0; i < kCols / 2; ++i) acc2[i] = 0ull;
       for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
         const uint32_t b = it % kAccs;
-        ok = ok && bar_wait(acc_full(b), (it / kAccs) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
+        ok = ok && bar_wait(done(it % kStages), (it / kStages) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
         __syncwarp();
         tmem_fence_after();
         if (live) {
           const uint32_t src = tmem + b * kN + col_off + (quarter << 21);   // lane 32 * quarter in the upper 16 bits
-          uint32_t v[2][16];
-          // piece k: 16 columns of the thread's row, or 32 columns of the thread's four fragments in 16 of the warp's rows
-          auto piece = [&](int k) { return kBvec ? src + k / 2 * 32 + ((uint32_t)(k % 2) << 20) : src + k * 16; };
-          tmem_load16<kBvec>(v[0], piece(0));
           const float* sc = reinterpret_cast<const float*>(smem + S::kOffScales + it % kSlots * kScales);
-          uint64_t sa2[kBvec ? 4 : 1];
+          auto free_accumulator = [&]() {       // all is in registers
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(release + 8 * b);
+          };
           if constexpr (kBvec) {
+            // piece k: 32 columns of the thread's four fragments in 16 of the warp's rows; one on its way while another is added
+            uint32_t v[2][16];
+            auto piece = [&](int k) { return src + k / 2 * 32 + ((uint32_t)(k % 2) << 20); };
+            tmem_load_fragments(v[0], piece(0));
+            uint64_t sa[4], sb[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { const uint32_t w = __float_as_uint(sc[quarter * 32 + i * 8 + lane / 4]); sa2[i] = pack2(w, w); }
-          } else {
-            const uint32_t w = __float_as_uint(sc[row] * sc[kTileM + col_off / kBlock]);
-            sa2[0] = pack2(w, w);
-          }
-          uint64_t sb[4];
+            for (int i = 0; i < 4; ++i) { const uint32_t w = __float_as_uint(sc[quarter * 32 + i * 8 + lane / 4]); sa[i] = pack2(w, w); }
 #pragma unroll
-          for (int k = 0; k < kCols / 16; ++k) {
-            uint32_t(&x)[16] = v[k % 2];
-            tmem_wait();
-            if (k + 1 < kCols / 16) {
-              tmem_load16<kBvec>(v[k % 2 ^ 1], piece(k + 1));
-            } else {       // all is in registers: the accumulator is free for a later block
-              tmem_fence_before();
-              __syncwarp();
-              if (lane == 0) bar_arrive_cluster(release + 8 * b);
-            }
-            if constexpr (kBvec) {
+            for (int k = 0; k < kCols / 16; ++k) {
+              tmem_wait();
+              if (k + 1 < kCols / 16) tmem_load_fragments(v[k % 2 ^ 1], piece(k + 1));
+              else free_accumulator();
               if (k % 2 == 0) {
 #pragma unroll
                 for (int f = 0; f < 4; ++f) sb[f] = *reinterpret_cast<const uint64_t*>(sc + kTileM + col_off + k / 2 * 32 + f * 8 + lane % 4 * 2);
               }
-              add_scaled_fragments(acc2 + 8 * k, x, sb, sa2[k % 2 * 2], sa2[k % 2 * 2 + 1]);
-            } else {
+              add_scaled_fragments(acc2 + 8 * k, v[k % 2], sb, sa[k % 2 * 2], sa[k % 2 * 2 + 1]);
+            }
+          } else {
+            // 64 columns at a time and none on its way meanwhile: what counts is how soon the accumulator is free again, and pieces of 16
+            // that overlap with the multiply-adds free it later (8192^3: 490 us against 470).  With a scale for each column the multiply-adds
+            // take twice as long, and overlapping them wins (4096^3, rows: 129 us against 146).
+            uint32_t x[64];
+            tmem_load_row(x, src);
+            const uint32_t w = __float_as_uint(sc[row] * sc[kTileM + col_off / kBlock]);
+            const uint64_t s = pack2(w, w);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) add_scaled(acc2[8 * k + i], x[2 * i], x[2 * i + 1], sa2[0]);
+            for (int k = 0; k < kCols / 64; ++k) {
+              tmem_wait();
+              if (k + 1 == kCols / 64) free_accumulator();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) add_scaled(acc2[32 * k + i], x[2 * i], x[2 * i + 1], s);
+              if (k + 1 < kCols / 64) tmem_load_row(x, src + (k + 1) * 64);
             }
           }
         } else if (lane == 0) {
@@ -630,7 +647,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       }
     }
   } else {
-    if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if constexpr (kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kEpiWarps) {
       if (lane == 0) {
         uint32_t it = 0;
@@ -640,7 +657,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           const int32_t m = (int32_t)(tm * kRows + row_off), n = (int32_t)(tn * kN + (kPair ? rank * kBlock : 0));
           for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
             const uint32_t s = it % kStages;
-            if (!(ok = ok && bar_wait(empty(s), ((it / kStages) & 1) ^ 1))) continue;
+            if (!(ok = ok && bar_wait(done(s), ((it / kStages) & 1) ^ 1))) continue;
             // the leader's barrier counts the bytes of both blocks
             if (!kPair || rank == 0) bar_expect(full(s), kPair ? 2 * S::kStage : S::kOperand + (kAmn ? S::kOperand : p.rows_a * kBlock));
             const uint32_t bar = kPair ? at_rank(full(s), 0) : full(s);
@@ -652,19 +669,27 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
       }
     } else if (warp <= kEpiWarps + 2) {
-      if (lane == 0 && (!kPair || rank == 0)) {
+      if (!kPair || rank == 0) {
+        // The whole warp walks the loop and one lane issues: descriptors then come from the warp's uniform registers.  (In a branch of one
+        // lane each had to be moved there from a lane's, and a block's four products took 480 cycles to issue.)
         const uint32_t mine = tiles > worker ? (tiles - worker + workers - 1) / workers * (kb1 - kb0) : 0;   // of all the block's tiles
-        for (uint32_t it = warp - (kEpiWarps + 1); it < mine; it += 2) {
+        const uint32_t issuer = __shfl_sync(0xFFFFFFFFu, warp, 0) - (kEpiWarps + 1);
+        for (uint32_t it = issuer; it < mine; it += 2) {
           const uint32_t s = it % kStages, b = it % kAccs;
-          if (!(ok = ok && bar_wait(full(s), (it / kStages) & 1) && bar_wait(acc_empty(b), ((it / kAccs) & 1) ^ 1))) continue;
+          ok = ok && bar_wait(full(s), (it / kStages) & 1) && bar_wait(acc_empty(b), ((it / kAccs) & 1) ^ 1);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
           tmem_fence_after();
-          const uint32_t sa = base + s * S::kStage, sb = sa + S::kOperand;
           // 32 deep a step: 32 bytes along a K-major row, 32 rows of 128 bytes of an MN-major tile
+          const uint64_t da = smem_desc<kAmn>(base + s * S::kStage), db = smem_desc<kBmn>(base + s * S::kStage + S::kOperand);
+          const uint32_t acc = tmem + b * kN, at_done = done(s);
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kBlock / 32; ++j)
-            mma_fp8<kPair>(tmem + b * kN, smem_desc<kAmn>(sa + j * (kAmn ? 32 * kBlock : 32)), smem_desc<kBmn>(sb + j * (kBmn ? 32 * kBlock : 32)), kIdesc, j > 0);
-          mma_commit<kPair>(empty(s));
-          mma_commit<kPair>(acc_full(b));
+            for (int j = 0; j < kBlock / 32; ++j)
+              mma_fp8<kPair>(acc, da + (uint64_t)(j * (kAmn ? 32 * kBlock : 32) >> 4), db + (uint64_t)(j * (kBmn ? 32 * kBlock : 32) >> 4), kIdesc, j > 0);
+            mma_commit<kPair>(at_done);
+          }
+          __syncwarp();
         }
       }
     } else {
@@ -725,13 +750,12 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       uint32_t it = 0;
       for (uint32_t t = worker; t < tiles; t += workers)
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t b = it % kAccs;
-          if (it >= kAccs) ok = ok && bar_wait(acc_full(b), ((it / kAccs) & 1) ^ 1);
+          if (it >= kAccs) ok = ok && bar_wait(done((it - kAccs) % kStages), ((it - kAccs) / kStages) & 1);
           __syncwarp();
           copy_next();
           asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");   // block `it` has landed
           __syncwarp();
-          if (lane == 0) bar_arrive(acc_full(b));
+          if (lane == 0) bar_arrive(done(it % kStages));
         }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
