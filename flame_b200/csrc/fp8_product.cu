@@ -880,16 +880,17 @@ cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stre
   p.rows_a = p.M < (uint32_t)kTileM ? (p.M + 7) / 8 * 8 : kTileM;
   p.wide_sa = kAmn && (reinterpret_cast<uintptr_t>(p.sa) & 15u) == 0 && p.sa_stride % 4 == 0;
   p.wide_sb = kBmn && kBvec && (reinterpret_cast<uintptr_t>(p.sb) & 15u) == 0 && p.sb_stride % 4 == 0;
-  // Which form: a round of pairs (256 x 256 tiles, one for two SMs) took 1.0 where a round of single blocks (128 x 128) took 0.635,
-  // measured at 4096^3, 2048^3 and 2304^3 (18.9 and 12.0 us a round at K = 4096); 128 blocks that share the contraction four
-  // at a time (one token, 2048 x 2048) 5.2 us, two at a time 6.0, none 7.5, eight 9.3: clusters of eight wait for a place.
+  // Which form: a round of pairs (256 x 256 tiles, one for two SMs) takes 1.0 where a round of single blocks (128 x 128) takes 0.70,
+  // measured with one round of each: 2048 x 2048 and 1536 x 1536 took 18.8 and 13.2 us at K = 4096, 9.0 and 6.0 us at K = 1024.  128
+  // blocks that share the contraction four at a time (one token, 2048 x 2048) 5.2 us, two at a time 6.0, none 7.5, eight 9.3: clusters
+  // of eight wait for a place.
   const uint64_t pairs = (uint64_t)sms / 2, rounds_of_pairs = ((uint64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) + pairs - 1) / pairs;
   p.tiles_m = (p.M + 127) / 128;
   p.tiles_n = (p.N + 127) / 128;
   const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n, rounds = (tiles + sms - 1) / sms;
   uint32_t splits = 1;
   while (splits < 4 && tiles * splits * 2 <= (uint64_t)sms && splits * 2 <= p.blocks_k) splits *= 2;
-  if (splits == 1 && rounds_of_pairs * 1000 <= rounds * 635) {
+  if (splits == 1 && rounds_of_pairs * 100 <= rounds * 70) {
     p.tiles_m = (p.M + 255) / 256;
     p.tiles_n = (p.N + 255) / 256;
     p.rows_a = kTileM;
