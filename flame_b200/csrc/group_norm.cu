@@ -19,6 +19,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "codec_kernels.cuh"
@@ -145,6 +146,8 @@ __device__ __forceinline__ void store(__nv_bfloat16* p, const F2 (&f)[kPairs<V>]
 // took 72 and 174 us, with four, which left two blocks on an SM, 76 and 152, this way 57 and 95.
 constexpr int kDepth = 8;
 constexpr size_t kRingBytes = (size_t)kDepth * kThreads * 16;
+constexpr uint32_t kMostGroups = 4096;
+constexpr int kMostShared = (int)(kRingBytes + (kThreads * 8 + kMostGroups) * sizeof(float2) + kMostGroups * sizeof(float));
 template <int kN, int V, bool kBack>
 struct Walk {
   [[maybe_unused]] static constexpr int kD = V == 8 ? kDepth / kN : 1;      // rows on their way
@@ -780,7 +783,7 @@ int check(const char* who, uint64_t B, uint64_t L, uint64_t C, uint64_t G, int a
   const char* what = nullptr;
   if (G == 0 || C == 0 || C % G != 0) what = "the channels must be a positive multiple of the groups";
   else if (C > 65536) what = "at most 65536 channels";
-  else if (G > 4096) what = "at most 4096 groups";
+  else if (G > kMostGroups) what = "at most 4096 groups";
   else if (B > 65534 || L > 0x7FFFFFFFull) what = "at most 65534 samples of at most 2^31 - 1 positions";
   else if (activation != FLAME_ACTIVATION_NONE && activation != FLAME_ACTIVATION_SILU) what = "unknown activation";
   else if (param_dtype != FLAME_OFFLOAD_DTYPE_BF16 && param_dtype != FLAME_OFFLOAD_DTYPE_F32) what = "weight and bias must be BF16 or F32";
@@ -793,8 +796,8 @@ int refuse(const char* who, const char* what) {
   return (int)cudaErrorInvalidValue;
 }
 
-template <typename K>
-cudaError_t launch(K kernel, dim3 grid, bool clusters, size_t smem, cudaStream_t stream, const NormArgs& a) {
+template <auto kKernel>
+cudaError_t launch(dim3 grid, bool clusters, size_t smem, cudaStream_t stream, const NormArgs& a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
@@ -815,9 +818,16 @@ cudaError_t launch(K kernel, dim3 grid, bool clusters, size_t smem, cudaStream_t
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  if (smem > 46 * 1024)      // beside two kilobytes that are not dynamic
-    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  if (smem > 46 * 1024) {      // beside two kilobytes that are not dynamic
+    static std::atomic<uint64_t> allowed{0};     // a bit for each device on which the kernel may use this much
+    int dev = 0;
+    if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+      if (const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared)) return e;
+      if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+  }
+  return cudaLaunchKernelEx(&cfg, kKernel, a);
 }
 
 template <typename F>
@@ -872,14 +882,14 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   cudaStream_t s = (cudaStream_t)stream;
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    cudaError_t e = launch(group_stats_kernel<V>, grid, true, sums_and_shifts, s, a);
+    cudaError_t e = launch<group_stats_kernel<V>>(grid, true, sums_and_shifts, s, a);
     if (e != cudaSuccess) return e;
-    if (a.finished) e = launch(group_finish_kernel<false>, dim3(a.G, a.B), false, 0, s, a);
+    if (a.finished) e = launch<group_finish_kernel<false>>(dim3(a.G, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
     if constexpr (V == 8) {
-      if (a.codes) return launch(group_apply_kernel<8, true>, grid, false, groups, s, a);
+      if (a.codes) return launch<group_apply_kernel<8, true>>(grid, false, groups, s, a);
     }
-    return launch(group_apply_kernel<V, false>, grid, false, groups, s, a);
+    return launch<group_apply_kernel<V, false>>(grid, false, groups, s, a);
   });
 }
 
@@ -916,11 +926,11 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
   return (int)by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
-    cudaError_t e = launch(group_grad_sums_kernel<V>, grid, true, sums, s, a);
+    cudaError_t e = launch<group_grad_sums_kernel<V>>(grid, true, sums, s, a);
     if (e != cudaSuccess) return e;
-    if (a.finished) e = launch(group_finish_kernel<true>, dim3(a.G, a.B), false, 0, s, a);
+    if (a.finished) e = launch<group_finish_kernel<true>>(dim3(a.G, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
-    return launch(group_grad_apply_kernel<V>, more, false, groups, s, a);
+    return launch<group_grad_apply_kernel<V>>(more, false, groups, s, a);
   });
 }
 

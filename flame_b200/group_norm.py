@@ -36,26 +36,28 @@ def _sizes(x):
     return b, l, c
 
 
-def _forward(x, weight, bias, groups, eps, activation, codes_wanted):
+def _forward(x, weight, bias, groups, eps, activation, codes_wanted, stats_wanted):
     device = x.device
     b, l, c = _sizes(x)
     y = torch.empty_like(x)
-    stats = torch.empty(b, groups, 2, dtype=torch.float32, device=device)
+    stats = torch.empty(b, groups, 2, dtype=torch.float32, device=device) if stats_wanted else None
     codes = scales = None
     if codes_wanted:
         codes = torch.empty(b * l, c, dtype=torch.uint8, device=device)
         scales = torch.empty(b * l, c // 128, dtype=torch.float32, device=device)
     size = _workspace_bytes(device.index, b, l, c, groups, 0)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    # statistics that nobody reads again lie behind the workspace: an allocation costs a tenth of a small call's time
+    ws = torch.empty(size if stats_wanted else size + 8 * b * groups, dtype=torch.uint8, device=device)
+    at = ws.data_ptr()
     _op.call("flame_group_norm", device, x.data_ptr(), _op.ptr(weight), _op.ptr(bias), y.data_ptr(), _op.ptr(codes), _op.ptr(scales),
-             stats.data_ptr(), b, l, c, groups, eps, activation, _param_dtype(weight, bias), ws.data_ptr(), size)
+             at + size if stats is None else stats.data_ptr(), b, l, c, groups, eps, activation, _param_dtype(weight, bias), at, size)
     return y, stats, codes, scales
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, activation, codes_wanted):
-        y, stats, codes, scales = _forward(x, weight, bias, groups, eps, activation, codes_wanted)
+        y, stats, codes, scales = _forward(x, weight, bias, groups, eps, activation, codes_wanted, True)
         ctx.groups, ctx.activation = groups, activation
         ctx.save_for_backward(x, weight, bias, stats)
         if not codes_wanted:
@@ -105,7 +107,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     """``act((x - mean) * rstd * weight + bias)`` with mean and variance of each sample's groups of channels."""
     _check("group_norm", x, groups, weight, bias, activation)
     if not _op.recorded(x, weight, bias):
-        return _forward(x, weight, bias, groups, float(eps), _ACTIVATIONS[activation], False)[0]
+        return _forward(x, weight, bias, groups, float(eps), _ACTIVATIONS[activation], False, False)[0]
     return _GroupNorm.apply(x, weight, bias, groups, float(eps), _ACTIVATIONS[activation], False)
 
 
@@ -120,5 +122,5 @@ def group_norm_fp8(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] 
     if _op.recorded(x, weight, bias):
         y, codes, scales = _GroupNorm.apply(x, weight, bias, groups, float(eps), _ACTIVATIONS[activation], True)
     else:
-        y, _, codes, scales = _forward(x, weight, bias, groups, float(eps), _ACTIVATIONS[activation], True)
+        y, _, codes, scales = _forward(x, weight, bias, groups, float(eps), _ACTIVATIONS[activation], True, False)
     return y, Fp8Blocks(codes, scales, "rows")
