@@ -4,7 +4,12 @@ Only what the hot path needs: the CUDA kernels and C ABI (``csrc/``,
 ``libflame_offload.so``), and Python mirrors of the reference interface
 (``ActivationOffloadPool``, ``PinnedHostBuffer``, ``PinnedPool``,
 ``CheckpointPolicy`` / ``CheckpointManager``, ``checkpoint_offload``, and
-``BlockOffloader`` for block weights streamed through the same pool).
+``BlockOffloader`` for block weights streamed through the same pool).  Beside
+them stand the operators of the blocks whose tensors move: ``fp8_product`` (FP8
+products with a scale per block of 128, the linear layer made of them),
+``group_norm`` (with its activation, and FP8 codes of the output) and
+``dropout`` (its mask drawn again where it is needed), next to
+``fused_producers``; each module is imported by name.
 
 Importing the package does not load CUDA.  Every operation goes through the
 shared library; there is no CPU or eager fallback, and a missing library is an

@@ -25,7 +25,9 @@ constexpr int kBlock = 128;
 // ---- quantiser ------------------------------------------------------------------
 // A thread block owns a 128 x 128 tile: thread (r, c) = (t / 16, t % 16) holds columns 8c..8c+7 of rows r, r + 16, ..., r + 112
 // as eight 16-byte loads, and keeps them in registers for whichever scales the caller wants: of its rows (four shuffles), of its
-// columns (one shuffle and eight partial maxima through shared memory), or of the tile.  The source is read once for both.
+// columns (one shuffle and eight partial maxima through shared memory), or of the tile.  The source is read once for both.  Bound by
+// memory with one kind of scales (8192 x 8192 rows 33.5 us, tiles 33.1: 6.0 TB/s), by instructions with two (rows and columns 53.7 us,
+// 5.0 TB/s).  Rows that are no multiple of 16 bytes apart are read element by element (1000 x 1331 6.3 us, 1000 x 1328 3.3).
 constexpr int kQuantThreads = 256;
 
 enum : uint32_t { kQuantRows = 1, kQuantTiles = 2, kQuantColumns = 4, kQuantWide = 8 };   // kQuantWide: 16-byte loads are possible
@@ -163,6 +165,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) fp8_quant_kernel(const __gri
 }
 
 // ---- codes back to numbers ---------------------------------------------------------
+// Eight codes a thread, 16 bytes stored: memory bounds it where it is large, the launch where it is small (8192 x 640 6.5 us, 2.4 TB/s).
 __device__ __forceinline__ float fp8_decode(uint32_t c) {   // OCP E4M3, exactly
   uint32_t h;
   asm("{ .reg .b16 v; cvt.u16.u32 v, %1; cvt.rn.f16x2.e4m3x2 %0, v; }" : "=r"(h) : "r"(c));
