@@ -867,7 +867,9 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   if (B == 0 || L == 0) return 0;
   if (!x || !y || !stats || !workspace) return refuse(who, "null tensor");
   if (workspace_bytes < flame_group_norm_workspace_bytes(B, L, C, G, 0)) return refuse(who, "workspace too small");
-  if (!al(x, 2) || !al(y, 2) || !al(stats, 4) || !al(workspace, 16)) return refuse(who, "misaligned tensor");
+  const uintptr_t psize = param_dtype == FLAME_OFFLOAD_DTYPE_F32 ? 4 : 2;
+  if (!al(x, 2) || !al(y, 2) || !al(weight, psize) || !al(bias, psize) || !al(stats, 8) || !al(code_scales, 4) || !al(workspace, 16))
+    return refuse(who, "misaligned tensor (stats: 8 bytes)");
   const bool al16 = al(x, 16) && al(y, 16);
   if (codes && (C % 128 != 0 || !al16 || !al(codes, 8) || !code_scales)) return refuse(who, "codes need channels % 128 == 0, 16-byte aligned tensors and a place for the scales");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
@@ -912,7 +914,8 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   }
   if (!x || !dy || !dx || !stats || !workspace) return refuse(who, "null tensor");
   if (workspace_bytes < flame_group_norm_workspace_bytes(B, L, C, G, 1)) return refuse(who, "workspace too small");
-  if (!al(x, 2) || !al(dy, 2) || !al(dx, 2) || !al(stats, 4) || !al(workspace, 16)) return refuse(who, "misaligned tensor");
+  if (!al(x, 2) || !al(dy, 2) || !al(dx, 2) || !al(weight, psize) || !al(bias, psize) || !al(dweight, psize) || !al(dbias, psize) || !al(stats, 8) || !al(workspace, 16))
+    return refuse(who, "misaligned tensor (stats: 8 bytes)");
   if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
   const Plan p = plan((uint32_t)B, L, (uint32_t)C, al(x, 16) && al(dy, 16) && al(dx, 16), al(x, 4) && al(dy, 4) && al(dx, 4), true, sm_count_here());
   NormArgs a = {};

@@ -99,6 +99,23 @@ def test_group_norm_entries():
     assert lib.flame_group_norm(None, None, None, None, None, None, None, 0, 10, 64, 8, 1e-5, 0, 0, None, 0, None) == 0
 
 
+def test_group_norm_alignment():
+    """Pairs of statistics are written at once, parameters read as what they are."""
+    lib = _lib.lib()
+    size = lib.flame_group_norm_workspace_bytes(2, 10, 128, 8, 0)
+    ok = [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 10, 128, 8, 1e-5, 0, 1, FAKE, size, None]
+    for at, value in ((0, FAKE + 1), (1, FAKE + 2), (2, FAKE + 2), (3, FAKE + 1), (5, FAKE + 2), (6, FAKE + 4)):
+        bad = list(ok)
+        bad[at] = value
+        refused("misaligned", "flame_group_norm", *bad)
+    size = lib.flame_group_norm_workspace_bytes(2, 10, 128, 8, 1)
+    ok = [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 10, 128, 8, 0, 1, FAKE, size, None]
+    for at, value in ((0, FAKE + 1), (1, FAKE + 1), (2, FAKE + 2), (3, FAKE + 2), (4, FAKE + 4), (5, FAKE + 1), (6, FAKE + 2), (7, FAKE + 2)):
+        bad = list(ok)
+        bad[at] = value
+        refused("misaligned", "flame_group_norm_backward", *bad)
+
+
 def test_dropout_entry():
     for args, text in (((FAKE, None, FAKE, 8, 0, 1.5, 1, None, 0, None), "p must be"), ((FAKE, None, FAKE, 8, 0, float("nan"), 1, None, 0, None), "p must be"),
                        ((FAKE, None, FAKE, 8, 3, 0.5, 1, None, 0, None), "dtype"), ((None, None, FAKE, 8, 0, 0.5, 1, None, 0, None), "null"),
