@@ -279,6 +279,50 @@ def test_under_a_pool(cuda_device):
     assert all(torch.equal(p, q) for p, q in zip(want, got)) and all(torch.equal(p, q) for p, q in zip(want, again))
 
 
+# (batch, positions, channels, groups): slabs of channels that end inside groups, the last one narrower; vectors of two channels and of
+# one; as many groups as there may be; parts joined by a launch of their own, groups over several slabs
+@pytest.mark.parametrize("shape", [(1, 300, 1280, 32), (1, 40, 1152, 9), (2, 21, 2568, 8), (1, 50, 1030, 10), (1, 30, 771, 3), (1, 9, 8192, 4096), (1, 5000, 4096, 2),
+                                   (1, 20000, 1280, 32), (3, 4097, 136, 17)])
+def test_ways_to_cut_a_tensor(cuda_device, shape):
+    test_output_and_gradients(cuda_device, shape, torch.float32, "silu")
+
+
+def test_calls_one_behind_the_other(cuda_device):
+    """The second launch of a call begins to read x while the first one ends: x changed in place just before, each output the next
+    input, and a call's input overwritten just behind it give what they give with pauses between."""
+    start = torch.randn(2, 1000, 640, device=cuda_device, generator=torch.Generator(device=cuda_device).manual_seed(7)).to(torch.bfloat16)
+    w = torch.full((640,), 1.5, device=cuda_device)
+
+    def run(x, pause):
+        outs = []
+        for k in range(6):
+            x.mul_(1.25).add_(0.5 * k)
+            pause()
+            y = group_norm(x, 32, w, activation="silu")
+            pause()
+            z, codes = group_norm_fp8(y, 16, w)
+            pause()
+            x.copy_(z)
+            dx, = torch.autograd.grad(group_norm(y.requires_grad_(True), 32, w), y, z)
+            pause()
+            outs += [y.detach().clone(), z, codes.dequantize(), dx]
+        return outs
+
+    want = run(start.clone(), torch.cuda.synchronize)
+    for _ in range(3):
+        for a, b in zip(run(start.clone(), lambda: None), want):
+            assert torch.equal(a, b)
+    x = start.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(x, lambda: None)
+    for _ in range(2):
+        x.copy_(start)
+        graph.replay()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
 def test_refusals(cuda_device):
     x = torch.randn(2, 10, 64, device=cuda_device, dtype=torch.bfloat16)
     w = torch.ones(64, device=cuda_device)
