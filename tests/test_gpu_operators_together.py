@@ -86,6 +86,31 @@ def test_residual_block_against_its_parts_in_64_bits(cuda_device):
         assert torch.equal(model(x), z)
 
 
+def test_two_streams_at_once(cuda_device):
+    """Steps of different sizes, issued in turn on two streams, give what they give one after the other."""
+    jobs = []
+    for k, (channels, positions) in enumerate(((256, 3000), (640, 700))):
+        model = Residual(channels, cuda_device)
+        x = torch.randn(2, positions, channels, device=cuda_device).to(torch.bfloat16)
+        jobs.append((model, x, torch.randn_like(x), torch.cuda.Stream()))
+
+    def step(model, x, dy):
+        t = x.detach().requires_grad_(True)
+        y = model(t)
+        return [y.detach(), *torch.autograd.grad(y, [t, *model.parameters()], dy)]
+
+    want = [step(*job[:3]) for job in jobs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for job in jobs:
+            with torch.cuda.stream(job[3]):
+                got.append(step(*job[:3]))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2]))
+
+
 def test_a_recorded_step_with_a_seed_in_device_memory(cuda_device):
     """Norm, product and dropout, forward and backward, in one graph; each replay draws the mask of the seed it finds."""
     x = torch.randn(1, 512, 128, device=cuda_device).to(torch.bfloat16)
