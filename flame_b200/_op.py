@@ -20,7 +20,7 @@ _FUNCTIONS: dict = {}
 
 def on_gpu(what: str, *tensors) -> torch.device:
     """The one GPU that all the tensors (None is skipped) are on."""
-    device = None
+    index = first = None
     for t in tensors:
         if t is None:
             continue
@@ -28,11 +28,13 @@ def on_gpu(what: str, *tensors) -> torch.device:
             raise InvalidInput(f"{what}: expected a tensor, got {type(t).__name__}")
         if not t.is_cuda:
             raise InvalidInput(f"{what}: the tensors must be on the GPU")
-        if device is None:
-            device = t.device
-        elif t.device != device:
+        if index is None:
+            index, first = t.get_device(), t
+        elif t.get_device() != index:
             raise InvalidInput(f"{what}: the tensors must be on one device")
-    return device
+    if first is None:
+        raise InvalidInput(f"{what}: expected a tensor, got None")
+    return first.device
 
 
 def function(name: str):
@@ -55,6 +57,11 @@ def call(name: str, device: torch.device, *args) -> None:
         if rc == 1:
             raise InvalidInput(_lib.last_error() or f"{name}: invalid argument")
         raise CudaError(f"{name} failed ({rc})")
+
+
+def workspace(like, size: int):
+    """`size` bytes on the device of `like`, a BF16 tensor (which is quicker than to name type and device)."""
+    return like.new_empty((size + 1) // 2)
 
 
 def ptr(t):

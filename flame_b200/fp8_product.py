@@ -85,7 +85,8 @@ def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int]:
     if x.dtype != torch.bfloat16 or x.dim() < 1:
         raise InvalidInput(f"{what}: BF16 tensors of one dimension at least")
     shape = x.shape
-    rows, cols = _rows_of(shape), shape[-1]
+    cols = shape[-1]
+    rows = shape[0] if len(shape) == 2 else _rows_of(shape)
     if x.is_contiguous():
         return rows, cols, cols
     if x.dim() != 2:
@@ -174,14 +175,13 @@ def _weight_args(weight, frozen: Optional[Fp8Blocks]):
 
 
 def _forward(x, codes: Optional[Fp8Blocks], weight, frozen: Optional[Fp8Blocks]) -> torch.Tensor:
-    device = x.device
     m, k, x_stride = _matrix(x, "fp8_linear")
     n, w_args = _weight_args(weight, frozen)
-    y = torch.empty(x.shape[:-1] + (n,), dtype=torch.bfloat16, device=device)
+    y = x.new_empty(x.shape[:-1] + (n,))
     size = _workspace_bytes(m, n, k, 0 if frozen is not None else 2)      # FLAME_FP8_LINEAR_BF16_WEIGHT
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    ws = _op.workspace(x, size)
     given = (None, 0, None) if codes is None else (codes.codes.data_ptr(), codes.stride, codes.scales.data_ptr())
-    _op.call("flame_fp8_linear", device, x.data_ptr(), x_stride, *given, *w_args, 3 if frozen is None else _BLOCKS[frozen.blocks], y.data_ptr(), m, n, k,
+    _op.call("flame_fp8_linear", x.device, x.data_ptr(), x_stride, *given, *w_args, 3 if frozen is None else _BLOCKS[frozen.blocks], y.data_ptr(), m, n, k,
              ws.data_ptr(), size)
     return y
 
@@ -208,13 +208,13 @@ class _Linear(torch.autograd.Function):
         device = dy.device
         dy = dy.contiguous()
         m, k = _rows_of(shape), shape[-1]
-        dx = torch.empty(shape, dtype=torch.bfloat16, device=device) if want_dx else None
-        dw = torch.empty(n, k, dtype=torch.bfloat16, device=device) if want_dw else None
+        dx = dy.new_empty(shape) if want_dx else None
+        dw = dy.new_empty(n, k) if want_dw else None
         w_args = (None, 0, None, 0, None)
         if want_dx:
             w_args = _weight_args(w, Fp8Blocks(w, w_scales, "tiles") if ctx.frozen else None)[1]
         size = _workspace_bytes(m, n, k, 1 if ctx.frozen else 3)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        ws = _op.workspace(dy, size)
         _op.call("flame_fp8_linear_backward", device, dy.data_ptr(), n, _op.ptr(x), _matrix(x, "fp8_linear")[2] if want_dw else 0, *w_args,
                  _op.ptr(dx), _op.ptr(dw), m, n, k, ws.data_ptr(), size)
         return dx, dw, None, None
@@ -226,12 +226,12 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], *, codes
     ``weight`` as ``Fp8Blocks`` is frozen ("tiles", or "rows" where x needs no gradient); as a BF16 tensor it is quantised in the call and
     receives a gradient.  ``codes``: the "rows" codes of x where a producer has written them already (``group_norm_fp8``)."""
     frozen = weight if isinstance(weight, Fp8Blocks) else None
-    w = weight if frozen is None else frozen.codes
-    _op.on_gpu("fp8_linear", x, w, codes.codes if codes is not None else None)
+    _op.on_gpu("fp8_linear", x, weight if frozen is None else frozen.codes, codes.codes if codes is not None else None)
     if frozen is None and (weight.dtype != torch.bfloat16 or weight.dim() != 2):
         raise InvalidInput("fp8_linear: the weight is a BF16 matrix [N, K] or Fp8Blocks")
-    if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
-        raise InvalidShape(f"fp8_linear: x {x.dtype} {tuple(x.shape)} and weight {tuple(w.shape)} do not fit")
+    w_shape = weight.shape
+    if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != w_shape[1]:
+        raise InvalidShape(f"fp8_linear: x {x.dtype} {tuple(x.shape)} and weight {tuple(w_shape)} do not fit")
     if codes is not None and (codes.blocks != "rows" or codes.shape != (_rows_of(x.shape), x.shape[-1])):
         raise InvalidShape("fp8_linear: codes must be the rows of x")
     record = _op.recorded(x, None if frozen is not None else weight)

@@ -47,7 +47,7 @@ def _forward(x, weight, bias, groups, eps, activation, codes_wanted, stats_wante
         scales = torch.empty(b * l, c // 128, dtype=torch.float32, device=device)
     size = _workspace_bytes(device.index, b, l, c, groups, 0)
     # statistics that nobody reads again lie behind the workspace: an allocation costs a tenth of a small call's time
-    ws = torch.empty(size if stats_wanted else size + 8 * b * groups, dtype=torch.uint8, device=device)
+    ws = _op.workspace(x, size if stats_wanted else size + 8 * b * groups)
     at = ws.data_ptr()
     _op.call("flame_group_norm", device, x.data_ptr(), _op.ptr(weight), _op.ptr(bias), y.data_ptr(), _op.ptr(codes), _op.ptr(scales),
              at + size if stats is None else stats.data_ptr(), b, l, c, groups, eps, activation, _param_dtype(weight, bias), at, size)
@@ -75,7 +75,7 @@ class _GroupNorm(torch.autograd.Function):
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         size = _workspace_bytes(device.index, b, l, c, groups, 1)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        ws = _op.workspace(x, size)
         _op.call("flame_group_norm_backward", device, x.data_ptr(), dy.data_ptr(), _op.ptr(weight), _op.ptr(bias), stats.data_ptr(),
                  dx.data_ptr(), _op.ptr(dw), _op.ptr(db), b, l, c, groups, ctx.activation, _param_dtype(weight, bias), ws.data_ptr(), size)
         return dx if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None

@@ -24,6 +24,12 @@ def test_tensors_off_the_gpu_are_refused():
             f()
 
 
+def test_what_is_no_tensor_is_refused():
+    for f in (lambda: quantize_fp8(None), lambda: group_norm(None, 8), lambda: dropout(None, 0.5, seed=1), lambda: fp8_linear([1.0], None)):
+        with pytest.raises(InvalidInput, match="expected a tensor"):
+            f()
+
+
 def test_quantiser_entry():
     ok = [FAKE, 4, 64, 64, FAKE, FAKE, 1, None, None, 64, None]
     for at, value, text in ((6, 7, "blocks must be"), (6, 0, "nothing to make"), (3, 63, "stride"), (9, 48, "stride"), (9, 72, "stride"), (0, None, "null"), (4, None, "null"),
