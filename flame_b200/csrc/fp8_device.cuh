@@ -36,6 +36,18 @@ __device__ __forceinline__ uint32_t fp8_encode2(float lo, float hi) {
 __device__ __forceinline__ uint2 fp8_pack8(const float (&y)[8]) {
   return make_uint2(fp8_encode2(y[0], y[1]) | (fp8_encode2(y[2], y[3]) << 16), fp8_encode2(y[4], y[5]) | (fp8_encode2(y[6], y[7]) << 16));
 }
+// Two elements times their factors, one multiplication for both.
+__device__ __forceinline__ uint64_t fp8_factors(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint32_t fp8_encode2(float lo, float hi, uint64_t factors) {
+  uint16_t r;
+  asm("{ .reg .b64 v; .reg .f32 a, b; mov.b64 v, {%1, %2}; mul.rn.f32x2 v, v, %3; mov.b64 {a, b}, v; cvt.rn.satfinite.e4m3x2.f32 %0, b, a; }"
+      : "=h"(r) : "f"(lo), "f"(hi), "l"(factors));
+  return r;
+}
 // Eight elements of one block.
 __device__ __forceinline__ uint2 fp8_encode8(const float (&x)[8], float scale, float factor) {
   float y[8];

@@ -26,8 +26,8 @@ constexpr int kBlock = 128;
 // A thread block owns a 128 x 128 tile: thread (r, c) = (t / 16, t % 16) holds columns 8c..8c+7 of rows r, r + 16, ..., r + 112
 // as eight 16-byte loads, and keeps them in registers for whichever scales the caller wants: of its rows (four shuffles), of its
 // columns (one shuffle and eight partial maxima through shared memory), or of the tile.  The source is read once for both.  Bound by
-// memory with one kind of scales (8192 x 8192 rows 33.5 us, tiles 33.1: 6.0 TB/s), by instructions with two (rows and columns 53.7 us,
-// 5.0 TB/s).  Rows that are no multiple of 16 bytes apart are read element by element (1000 x 1331 6.3 us, 1000 x 1328 3.3).
+// memory with one kind of scales (8192 x 8192 rows 33.5 us, tiles 33.1: 6.0 TB/s), by instructions with two (rows and columns 51.7 us,
+// 5.2 TB/s).  Rows that are no multiple of 16 bytes apart are read element by element (1000 x 1331 6.3 us, 1000 x 1328 3.3).
 constexpr int kQuantThreads = 256;
 
 enum : uint32_t { kQuantRows = 1, kQuantTiles = 2, kQuantColumns = 4, kQuantWide = 8 };   // kQuantWide: 16-byte loads are possible
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) fp8_quant_kernel(const __gri
       if (t < kBlock && tn * kBlock + t < a.cols) a.col_scales[(size_t)tm * a.cols + tn * kBlock + t] = scales[t];
       const float4 f0 = *reinterpret_cast<const float4*>(factors + lc * 8), f1 = *reinterpret_cast<const float4*>(factors + lc * 8 + 4);
       const float fc[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+      const uint64_t pc[4] = {fp8_factors(f0.x, f0.y), fp8_factors(f0.z, f0.w), fp8_factors(f1.x, f1.y), fp8_factors(f1.z, f1.w)};
       bool divides = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) divides |= fp8_divides(fc[i]);
@@ -154,11 +155,11 @@ __global__ void __launch_bounds__(kQuantThreads, 4) fp8_quant_kernel(const __gri
         if (divides) {
 #pragma unroll 1
           for (int i = 0; i < 8; ++i) f[i] = fp8_divides(factors[lc * 8 + i]) ? __fdiv_rn(f[i], scales[lc * 8 + i]) : __fmul_rn(f[i], factors[lc * 8 + i]);
+          put(a.col_codes, j, fp8_pack8(f));
         } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], fc[i]);
+          put(a.col_codes, j, make_uint2(fp8_encode2(f[0], f[1], pc[0]) | (fp8_encode2(f[2], f[3], pc[1]) << 16),
+                                         fp8_encode2(f[4], f[5], pc[2]) | (fp8_encode2(f[6], f[7], pc[3]) << 16)));
         }
-        put(a.col_codes, j, fp8_pack8(f));
       }
     }
   }
