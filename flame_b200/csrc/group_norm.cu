@@ -16,9 +16,9 @@
 // added in a fixed order, without atomics: the same inputs give the same bits.
 //
 // What bounds it, measured on one B200: memory where x is larger than the L2 cache, which the second launch then reads again (1024 x 1024
-// x 128 with silu: forward 139 us for 537 MB in and out and 268 read twice, 5.8 TB/s; backward 235 us; with codes 175 us); the way
-// through two dependent launches and their joins where it is small (1 x 64 x 1280 forward 8.9 us, backward 11.4; 4 x 4096 x 320 15.9
-// and 20.1; of those 8 us a launch some 3 are the rows, 2 the cluster's join, 2 the joining of the parts).
+// x 128 with silu: forward 139 us for 537 MB in and out and 268 read twice, 5.8 TB/s; backward 231 us; with codes 174 us); the way
+// through two dependent launches and their joins where it is small (1 x 64 x 1280 forward 8.9 us, backward 10.5; 4 x 4096 x 320 15.8
+// and 18.8; of those 8 us a launch some 3 are the rows, 2 the cluster's join, 2 the joining of the parts).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -299,10 +299,9 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // `count` pairs of every block's `sh`, pair i at place(i), joined over the cluster's blocks in the order of their ranks; each block
-// joins and writes its share.
+// joins and writes its share.  Between two cluster_sync_all(): the pairs are there, and nobody leaves or writes them while they are read.
 template <typename F, typename J>
 __device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, float2* out, F&& place, J&& join) {
-  cluster_sync_all();
   const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(sh));
   for (uint32_t i = cluster_rank() + kCluster * threadIdx.x; i < count; i += kCluster * kThreads) {
     float2 v[kCluster];
@@ -314,7 +313,6 @@ __device__ __forceinline__ void join_cluster(const float2* sh, uint32_t count, f
     }
     out[i] = join(i, v);
   }
-  cluster_sync_all();      // nobody leaves or writes its sums while they are read
 }
 __device__ __forceinline__ float2 add_up(const float2 (&v)[kCluster]) {
   float2 t = v[0];
@@ -485,6 +483,7 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
     // fmaxf would turn the NaN of a NaN or an infinity into 0
     return make_float2(shifts[g] + off, sum2 < INFINITY ? fmaxf(sum2 - sum * off, 0.0f) : NAN);
   });
+  cluster_sync_all();
   // mean and sum of squares of the cluster's blocks, joined
   join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + p.chunk / kCluster) * a.G, [](uint32_t i) { return i; },
                [&](uint32_t g, const float2 (&v)[kCluster]) {
@@ -503,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_c
     for (uint32_t k = 0; k < kCluster; ++k) m2 += n[k] > 0.0f ? fmaf(n[k] * (v[k].x - mean), v[k].x - mean, v[k].y) : 0.0f;
     return make_float2(mean, m2);
   });
+  cluster_sync_all();
 }
 
 // What the second launch needs of a group: mean and rstd, or backward the means of s1 and s2.
@@ -653,10 +653,12 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __gr
     return make_float2(w * t.x, w * t.y);
   }, [](uint32_t, float sum, float sum2) { return make_float2(sum, sum2); });
   const uint32_t part = p.chunk / kCluster;
+  cluster_sync_all();
   join_cluster(groups, a.G, a.partial + ((size_t)p.b * a.parts + p.slab * (a.chunks / kCluster) + part) * a.G, [](uint32_t i) { return i; },
                [](uint32_t, const float2 (&v)[kCluster]) { return add_up(v); });
   join_cluster(sh, width, a.channel_partial + ((size_t)p.b * (a.chunks / kCluster) + part) * a.C + slab_c0, [&](uint32_t c) { return place_of<V>(c, width); },
                [](uint32_t, const float2 (&v)[kCluster]) { return add_up(v); });
+  cluster_sync_all();
 }
 
 // The blocks of one more sample than there are add the channel sums up to dweight and dbias.
