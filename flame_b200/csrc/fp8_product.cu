@@ -242,8 +242,9 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 // PFLOP/s; with the accumulators handed to an epilogue that does nothing 383; as it is 470 (2.34 PFLOP/s) with a scale for 128 columns
 // and 654 with one for each.  From a product's end to the epilogue's start pass some 420 cycles, from its release to the next product's
 // start 270, between them the reading, during which products are slower: two accumulators, all that tensor memory holds, hide most of
-// it.  Halves of 128 columns in four accumulators took 620 us, sixteen epilogue warps 500 to 510.  In loops of seconds the power limit
-// of the board comes first (1.7 GHz).
+// it.  Halves of 128 columns in four accumulators took 620 us, tiles of 256 x 192 that the epilogue reads whole before it adds 560,
+// sixteen epilogue warps 500 to 510.  Power counts too: operands of zeros take 410 us, and in loops of seconds the limit of the board
+// comes first (545 us at some 1.5 GHz).
 //
 // Two forms.  kPair, for many tiles: the two SMs of a pair work on one tile of 256 x 256 (cta_group::2), each holds half of either
 // operand, the leader issues the products for both.  Without it a block has a tile of 128 x 128, and where tiles are few (serving,
