@@ -54,8 +54,8 @@ def call(name: str, device: torch.device, *args) -> None:
         with torch.cuda.device(index):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
-        if rc == 1:
-            raise InvalidInput(_lib.last_error() or f"{name}: invalid argument")
+        if rc == 1 and _lib.last_error().startswith(name + ":"):      # not an earlier call's text behind an error of CUDA's
+            raise InvalidInput(_lib.last_error())
         raise CudaError(f"{name} failed ({rc})")
 
 
