@@ -712,21 +712,21 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
   wait_for_earlier();
   const Params<V> params(a, p);
   finish_all<true>(a, p.b, sh);
-  // dx = scale * dh - rstd^2 * m2 * x + what does not depend on the position; h = x * scale + offset
+  // dx = scale * dh - rstd^2 * m2 * (x - mean) - rstd * m1; h = (x - mean) * scale + bias.  First the difference, as in the passes before:
+  // in a group of equal values far from zero a factor and an offset of x would each be large, and h off by what their sum rounds away.
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + (size_t)p.b * a.G;
-  F2 scale[kPairs<V>], offset[kPairs<V>], slope[kPairs<V>], rest[kPairs<V>], mean[kPairs<V>];
-  params.with(a, p, stats, [](float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, offset, mean, scale);
+  F2 scale[kPairs<V>], bias[kPairs<V>], slope[kPairs<V>], rest[kPairs<V>], mean[kPairs<V>];      // the mean's negative
+  params.with(a, p, stats, [](float w, float2 t, float& m, float& sc) { m = -t.x; sc = t.y * w; }, bias, mean, scale);
   if (!p.live) return;
 #pragma unroll
   for (int i = 0; i < kPairs<V>; ++i) {
-    offset[i] = fma(mean[i], scale[i], offset[i]);
     float sl[2] = {}, re[2] = {};
 #pragma unroll
     for (int k = 0; k < 2 && 2 * i + k < V; ++k) {
       const uint32_t g = group_of(p.c0 + 2 * i + k, a.by_cg);
       const float2 t = stats[g], m = sh[g];
       sl[k] = -t.y * t.y * m.y;
-      re[k] = fmaf(-t.x, sl[k], -t.y * m.x);
+      re[k] = -t.y * m.x;
     }
     slope[i] = F2(sl[0], sl[1]);
     rest[i] = F2(re[0], re[1]);
@@ -737,8 +737,8 @@ __global__ void __launch_bounds__(kThreads, 3) group_grad_apply_kernel(const __g
     unpack<V>(v[1], dy);
 #pragma unroll
     for (int i = 0; i < kPairs<V>; ++i) {
-      const F2 dh = grad_h(fma(x[i], scale[i], offset[i]), dy[i], a.silu);
-      x[i] = fma(scale[i], dh, fma(slope[i], x[i], rest[i]));
+      const F2 d = add(x[i], mean[i]), dh = grad_h(fma(d, scale[i], bias[i]), dy[i], a.silu);
+      x[i] = fma(scale[i], dh, fma(slope[i], d, rest[i]));
     }
     store<V>(a.y + first + at, x, a.stream);
   });
