@@ -263,6 +263,14 @@ constexpr int kStagingBytes = 32 * kStagePitch;
 
 __device__ unsigned int g_wait_faults;
 
+// How a product stands to the kernel before it in the stream.  kBehind: it may be placed early (a programmatic launch) and waits for it.
+// kFirst, kBeside: two products of one quantiser's codes, which need nothing of each other.  The first is launched in the ordinary way: it
+// starts when the quantiser is complete, and its writes visible.  The second starts when every block of the first has, so it may read the
+// codes at once, and its blocks begin where the first's have ended, in place of a last round that fills a part of the SMs (4608 x 2304 x
+// 9216, both gradients: 276 -> 245 us).  It reads nothing that the first writes and overwrites nothing that the first reads; it waits for
+// the first before it ends, so that what waits for the second has waited for both.
+enum : uint32_t { kBehind = 0, kFirst, kBeside };
+
 struct ProductArgs {
   const float* sa;
   const float* sb;
@@ -274,7 +282,7 @@ struct ProductArgs {
   uint32_t rows_a;                 // rows of A that a copy brings: fewer than 128 where C has fewer, a multiple of 8
   uint32_t wide;                   // rows of C start on 32 bytes
   uint32_t wide_sa, wide_sb;       // scales that lie along M or N: rows of them start on 16 bytes
-  uint32_t beside;                 // the kernel before in the stream is a product of which this one needs nothing
+  uint32_t order;                  // kBehind, kFirst or kBeside
 };
 
 struct ProductSmem {
@@ -498,13 +506,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   if (kPair) cluster_sync_all();      // the other block's barriers are ready
   tmem_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // The next kernel may be placed when every block has waited for what this one reads, so that a second product of the same operands'
-  // quantiser (`beside`) need not wait for the first: its blocks begin where the first's have ended, in place of a last round that fills
-  // a part of the SMs (4608 x 2304 x 9216, both gradients: 276 -> 245 us).  It reads nothing that the first writes and overwrites nothing
-  // that the first reads; the fence keeps it from numbers that L1 held before the quantiser; it waits for the first before it ends, so
-  // that what waits for this kernel has waited for both.
-  if (p.beside) __threadfence();
-  else asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.order != kBeside) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // The epilogue's sums need more registers than an equal share: 384 threads start with 168 each, 64,512 together; four warps go down
@@ -807,7 +809,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
-  if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.order == kBeside) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -864,7 +866,7 @@ cudaError_t launch_tiles(const Operands& o, const ProductArgs& p, uint32_t group
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (pdl_enabled()) {
+  if (p.order != kFirst && pdl_enabled()) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
@@ -959,7 +961,7 @@ Place take(uint8_t*& at, size_t rows, size_t cols, uint32_t mode) {
 
 enum class Product { kNtTiles, kNtRows, kNnTiles, kTnColumns };
 cudaError_t product(Product kind, const void* a, size_t a_stride, const void* sa, const void* b, size_t b_stride, const void* sb, void* c, size_t c_stride, bool f32,
-                    size_t M, size_t N, size_t K, cudaStream_t s, bool beside = false) {
+                    size_t M, size_t N, size_t K, cudaStream_t s, uint32_t order = kBehind) {
   if (blocks_of(M) * blocks_of(N) > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;      // a result of over 2^45 numbers
   if (K == 0) {   // an empty sum
     const size_t size = f32 ? 4 : 2;
@@ -968,7 +970,7 @@ cudaError_t product(Product kind, const void* a, size_t a_stride, const void* sa
   const Operands o = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b), a_stride, b_stride};
   ProductArgs p = {};
   p.sa = static_cast<const float*>(sa); p.sb = static_cast<const float*>(sb);
-  p.c = c; p.c_stride = c_stride; p.beside = beside;
+  p.c = c; p.c_stride = c_stride; p.order = order;
   p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K;
   p.sa_stride = kind == Product::kTnColumns ? (uint32_t)M : (uint32_t)blocks_of(K);
   p.sb_stride = kind == Product::kTnColumns ? (uint32_t)N : (uint32_t)blocks_of(kind == Product::kNnTiles ? N : K);
@@ -1131,10 +1133,12 @@ int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, s
     }
     if (const cudaError_t e = launch_quant(jobs, s)) return (int)e;
   }
+  // the two side by side; an empty sum's zeros are no product
+  const bool both = dx && dw && any;
   if (dx && M > 0)
-    if (const cudaError_t e = product(Product::kNnTiles, rows.codes, ldn, rows.scales, w_codes, w_code_stride, w_scales, dx, K, false, M, K, N, s)) return (int)e;
-  // behind dx's product, and not behind the zeros that an empty sum leaves there
-  if (dw && N > 0) return (int)product(Product::kTnColumns, cols.codes, ldn, cols.scales, xcols.codes, ldk, xcols.scales, dw, K, false, N, K, M, s, dx && M > 0);
+    if (const cudaError_t e = product(Product::kNnTiles, rows.codes, ldn, rows.scales, w_codes, w_code_stride, w_scales, dx, K, false, M, K, N, s, both ? kFirst : kBehind))
+      return (int)e;
+  if (dw && N > 0) return (int)product(Product::kTnColumns, cols.codes, ldn, cols.scales, xcols.codes, ldk, xcols.scales, dw, K, false, N, K, M, s, both ? kBeside : kBehind);
   return 0;
 }
 

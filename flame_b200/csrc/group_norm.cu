@@ -431,16 +431,16 @@ __device__ __forceinline__ float2 join_parts(const NormArgs& a, uint32_t b, uint
   return make_float2(mean, all(q));
 }
 
-// Programmatic launches.  The first kernel lets the next one start when all its blocks have waited for what ran before them, so
-// the second kernel may read the call's inputs at once: whatever wrote them is done.  It sends its first rows on their way, past L1,
-// while the first kernel ends, and waits before it reads anything else or writes.
+// Launches.  A call's first kernel is launched in the ordinary way: it starts when everything ahead of the call is complete, and its writes
+// visible.  The others are programmatic launches: the second kernel starts when all blocks of the first have, so it may read the call's
+// inputs at once.  It sends its first rows on their way, past L1, while the first kernel ends, and waits before it reads anything else or
+// writes.  (With a programmatic first launch too, the second would read inputs that only the first has waited for.)
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void wait_then_launch() { wait_for_earlier(); launch_next(); }
 
 template <int V>
 __global__ void __launch_bounds__(kThreads, 4) group_stats_kernel(const __grid_constant__ NormArgs a) {
-  wait_then_launch();
+  launch_next();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
@@ -621,7 +621,7 @@ __device__ __forceinline__ F2 grad_h(F2 h, F2 dy, int silu) {
 
 template <int V>
 __global__ void __launch_bounds__(kThreads, 3) group_grad_sums_kernel(const __grid_constant__ NormArgs a) {
-  wait_then_launch();
+  launch_next();
   extern __shared__ uint4 ring[];
   float2* sh = sums_of<V>(ring);
   const Place<V> p(a);
@@ -809,22 +809,23 @@ int refuse(const char* who, const char* what) {
   return (int)cudaErrorInvalidValue;
 }
 
+// first: of a call, in clusters, and behind all that is ahead in the stream
 template <auto kKernel>
-cudaError_t launch(dim3 grid, bool clusters, size_t smem, cudaStream_t stream, const NormArgs& a) {
+cudaError_t launch(dim3 grid, bool first, size_t smem, cudaStream_t stream, const NormArgs& a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
   int n = 0;
-  if (clusters) {
+  if (first) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = kCluster;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (pdl_enabled()) {
+  if (!first && pdl_enabled()) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
