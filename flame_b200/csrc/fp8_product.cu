@@ -251,8 +251,9 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 // one token) a cluster of two or four blocks shares one: each takes a range of the contraction, and their sums are joined through
 // distributed shared memory in the order of the ranks.
 //
-// Every wait gives up after two seconds: the kernel then counts the fault (flame_fp8_product_faults), leaves its copies time to land
-// and returns its tensor memory.
+// Every wait gives up after two seconds.  The warp then arrives at no barrier any more, so that nothing is overwritten that another warp
+// still reads and the waits of the others that depend on it give up too; an epilogue warp writes NaN for what it had not finished.  The
+// kernel counts the warps (flame_fp8_product_faults), leaves its copies time to land and returns its tensor memory.
 constexpr int kEpiWarps = 8;
 constexpr int kProductThreads = 32 * (kEpiWarps + 4);
 constexpr int kTileM = 128;                     // rows of a thread block
@@ -304,17 +305,20 @@ __device__ __forceinline__ uint64_t clock_ns() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// false: two seconds have passed
+// false: two seconds have passed, counting at most a quarter of one between two looks at the clock, which runs on while the context is
+// switched out
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  uint64_t since = 0;
+  uint64_t last = 0;
+  uint32_t waited = 0;
   for (uint32_t n = 0;; ++n) {
     uint32_t done;
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
     if ((n & 255u) == 255u) {
       const uint64_t now = clock_ns();
-      if (since == 0) since = now;
-      else if (now - since > 2000000000ull) { atomicAdd(&g_wait_faults, 1u); return false; }
+      if (last != 0) waited += now - last < 250000000ull ? (uint32_t)(now - last) : 250000000u;
+      if (waited > 2000000000u) return false;
+      last = now;
     }
   }
 }
@@ -517,7 +521,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const uint32_t row = quarter * 32 + lane;
     const uint32_t release = at_rank(acc_empty(0), kPair ? 0 : rank);
     uint32_t it = 0;
-    for (uint32_t t = worker; ok && t < tiles; t += workers) {
+    for (uint32_t t = worker; t < tiles; t += workers) {
       uint32_t tm, tn;
       tile_at(p, t, tm, tn);
       const uint32_t m0 = tm * kRows + row_off + quarter * 32;
@@ -526,9 +530,9 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       uint64_t acc2[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) acc2[i] = 0ull;
-      for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+      for (uint32_t kb = ok ? kb0 : kb1; kb < kb1; ++kb, ++it) {
         const uint32_t b = it % kAccs;
-        ok = ok && bar_wait(done(it % kStages), (it / kStages) & 1);      // after a wait that ran out none is waited for: the loops run to their ends
+        ok = ok && bar_wait(done(it % kStages), (it / kStages) & 1);      // after a wait that ran out none is waited for: the loop runs to its end
         __syncwarp();
         tmem_fence_after();
         if (live) {
@@ -537,7 +541,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           auto free_accumulator = [&]() {       // all is in registers
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive_cluster(release + 8 * b);
+            if (lane == 0 && ok) bar_arrive_cluster(release + 8 * b);
           };
           if constexpr (kBvec) {
             // piece k: 32 columns of the thread's four fragments in 16 of the warp's rows; one on its way while another is added
@@ -575,9 +579,14 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
               if (k + 1 < kCols / 64) tmem_load_row(x, src + (k + 1) * 64);
             }
           }
-        } else if (lane == 0) {
+        } else if (lane == 0 && ok) {
           bar_arrive_cluster(release + 8 * b);
         }
+      }
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) {
+#pragma unroll
+        for (int i = 0; i < kCols / 2; ++i) acc2[i] = pack2(0x7FC00000u, 0x7FC00000u);
       }
       if (kPair || splits == 1) {
         if (!live) continue;
@@ -758,7 +767,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       for (uint32_t t = worker; t < tiles; t += workers)
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
           if (it >= kAccs) ok = ok && bar_wait(done((it - kAccs) % kStages), ((it - kAccs) / kStages) & 1);
-          __syncwarp();
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) continue;
           copy_next();
           asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");   // block `it` has landed
           __syncwarp();
@@ -768,9 +778,14 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
   }
 
-  if (!ok) {      // a wait ran out: the copies and products in flight get a millisecond to end
+  if (__any_sync(0xFFFFFFFFu, !ok)) {      // a wait ran out: the copies and products in flight get a millisecond to end
     const uint64_t since = clock_ns();
     while (clock_ns() - since < 1000000ull) {}
+    if (lane == 0) atomicAdd(&g_wait_faults, 1u);
+    if (!kPair && splits > 1 && warp < kEpiWarps) {      // the share that lies over the pipeline's buffers, now that no copy lands there
+      float* mine = reinterpret_cast<float*>(smem) + (size_t)((warp & 3) * 32 + lane) * (kN + 4) + (warp >> 2) * kCols;
+      for (int i = 0; i < kCols; ++i) mine[i] = __uint_as_float(0x7FC00000u);
+    }
   }
   __syncwarp();
   if (!kPair && splits > 1) {      // one tile for each cluster
@@ -1143,7 +1158,9 @@ int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, s
 }
 
 int flame_fp8_product_faults(unsigned int* count) {
-  if (!count) return (int)cudaErrorInvalidValue;
+  if (!count) return refuse("flame_fp8_product_faults", "null count");
+  // a copy on the default stream would not wait for streams that do not synchronise with it
+  if (const cudaError_t e = cudaDeviceSynchronize()) return (int)e;
   return (int)cudaMemcpyFromSymbol(count, g_wait_faults, sizeof(*count));
 }
 

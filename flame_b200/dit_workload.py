@@ -21,7 +21,7 @@ import torch.nn.functional as F
 from . import checkpoint as ckpt
 from . import fused_producers
 from .dropout import dropout
-from .fp8_product import fp8_linear
+from .fp8_product import check_faults, fp8_linear
 from .activation_offload import ActivationOffloadPool, OffloadCompression
 from .policy import Block, Decision, plan_blocks, probe
 
@@ -193,6 +193,8 @@ def _time_steps(model, opt, x, cos, sin, steps, warmup):
         loss = one()
     e1.record()
     torch.cuda.synchronize()
+    if FP8_LINEARS:
+        check_faults()
     ms, peak = e0.elapsed_time(e1) / steps, torch.cuda.max_memory_allocated()
     # one more, untimed step to see how much the forward pass leaves on the device
     m0 = torch.cuda.memory_allocated()

@@ -13,13 +13,14 @@ operands: there code 0x7F stands for 480.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _op
-from .errors import InvalidInput, InvalidShape, Unsupported
+from .errors import CudaError, InvalidInput, InvalidShape, Unsupported
 
 BLOCK = 128
 _BLOCKS = {"rows": 1, "columns": 2, "tiles": 3}     # FLAME_FP8_BLOCKS_*
@@ -159,6 +160,26 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, *, transpose_b: bool = False, dtype: 
     _op.call("flame_fp8_product", device, a.codes.data_ptr(), a.stride, a.scales.data_ptr(), _BLOCKS[a.blocks], b.codes.data_ptr(), b.stride,
              b.scales.data_ptr(), _BLOCKS[b.blocks], int(bool(transpose_b)), c.data_ptr(), n, _op.DTYPE[dtype], m, n, k)
     return c
+
+
+_seen_faults: dict = {}
+
+
+def check_faults(device: Optional[torch.device] = None) -> None:
+    """Raises ``CudaError`` where a wait inside a product's kernel has given up since the last check: such a product wrote NaN where its
+    result is not known.  Waits for the device (the current one by default), so it belongs where a program waits for it anyway."""
+    index = torch.device(device).index if device is not None else None
+    if index is None:
+        index = torch.cuda.current_device()
+    count = ctypes.c_uint(0)
+    with torch.cuda.device(index):
+        rc = _op.function("flame_fp8_product_faults")(ctypes.byref(count))
+    if rc:
+        raise CudaError(f"flame_fp8_product_faults failed ({rc})")
+    new = count.value - _seen_faults.get(index, 0)
+    _seen_faults[index] = count.value
+    if new:
+        raise CudaError(f"FP8 product: {new} warps on GPU {index} gave up a wait; the products concerned hold NaN")
 
 
 @functools.lru_cache(maxsize=4096)

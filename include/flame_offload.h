@@ -583,8 +583,9 @@ int flame_fp8_linear(const void* x_bf16, size_t x_stride, const void* x_codes, s
 int flame_fp8_linear_backward(const void* dy_bf16, size_t dy_stride, const void* x_bf16, size_t x_stride, const void* w_bf16, size_t w_stride,
                               const void* w_codes, size_t w_code_stride, const void* w_scales, void* dx_bf16, void* dw_bf16, size_t M,
                               size_t N, size_t K, void* workspace, size_t workspace_bytes, void* stream);
-/* How often a wait inside a product's kernel on the current device gave up after two seconds since the library was loaded, in
- * which case that product's result is wrong.  0 unless something else is broken.  Waits for the device. */
+/* How many warps of products' kernels on the current device gave up a wait, after two seconds, since the library was loaded.  Such a
+ * product has NaN where its result is not known.  0 unless something else is broken.  Waits for all work on the device (not while a
+ * stream is being captured). */
 int flame_fp8_product_faults(unsigned int* count);
 
 /* 8b. Group norm with an activation on a channels-last BF16 tensor x [B, L, C] (contiguous): C / G neighbouring channels a
