@@ -8,6 +8,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -69,7 +70,12 @@ def ptr(t):
 
 
 def recorded(*tensors) -> bool:
-    """Whether autograd records a call on these tensors (None is skipped)."""
+    """Whether autograd records a call on these tensors (None is skipped).  A tensor with a forward-mode tangent counts: the recorded form
+    refuses it, where a bare launch would drop the tangent."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
