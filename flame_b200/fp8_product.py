@@ -207,6 +207,25 @@ def _forward(x, codes: Optional[Fp8Blocks], weight, frozen: Optional[Fp8Blocks])
     return y
 
 
+def _rows_again(t: torch.Tensor) -> torch.Tensor:
+    """A saved BF16 tensor as ``_matrix`` reads it: hooks may give it back with strides of their own."""
+    cols = t.shape[-1]
+    if t.is_contiguous() or (t.dim() == 2 and (t.stride(1) == 1 or cols == 1) and (t.shape[0] == 1 or t.stride(0) >= cols)):
+        return t
+    return t.contiguous()
+
+
+def _codes_again(codes: torch.Tensor) -> torch.Tensor:
+    """Saved codes as ``Fp8Blocks`` takes them: hooks that copy leave out the padding of the rows."""
+    rows, cols = codes.shape
+    if rows == 0 or cols == 0:
+        return codes
+    if (codes.stride(1) == 1 or cols == 1) and codes.data_ptr() % 16 == 0 and (rows == 1 or (codes.stride(0) % 16 == 0 and codes.stride(0) >= cols)):
+        return codes
+    padded = codes.new_empty(rows, _padded(cols))[:, :cols]
+    return padded.copy_(codes)
+
+
 class _Linear(torch.autograd.Function):
     """y = x w^T.  Saved for backward: x where the weight is trained (BF16, so that a pool can offload it) and the weight itself.  Its codes
     are made again: keeping them would hold half as much memory again as the weights do, for a few per cent of a step's time."""
@@ -232,7 +251,10 @@ class _Linear(torch.autograd.Function):
         dx = dy.new_empty(shape) if want_dx else None
         dw = dy.new_empty(n, k) if want_dw else None
         w_args = (None, 0, None, 0, None)
+        if want_dw:
+            x = _rows_again(x)
         if want_dx:
+            w, w_scales = (_codes_again(w), w_scales.contiguous()) if ctx.frozen else (_rows_again(w), None)
             w_args = _weight_args(w, Fp8Blocks(w, w_scales, "tiles") if ctx.frozen else None)[1]
         size = _workspace_bytes(m, n, k, 1 if ctx.frozen else 3)
         ws = _op.workspace(dy, size)

@@ -67,7 +67,7 @@ class _GroupNorm(torch.autograd.Function):
 
     @_op.first_order
     def backward(ctx, dy, *_):
-        x, weight, bias, stats = ctx.saved_tensors
+        x, weight, bias, stats = (t if t is None else t.contiguous() for t in ctx.saved_tensors)      # hooks may give them other strides
         device, groups = x.device, ctx.groups
         b, l, c = _sizes(x)
         dy = dy.contiguous()
