@@ -55,9 +55,10 @@ def call(name: str, device: torch.device, *args) -> None:
         with torch.cuda.device(index):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
-        if rc == 1 and _lib.last_error().startswith(name + ":"):      # not an earlier call's text behind an error of CUDA's
-            raise InvalidInput(_lib.last_error())
-        raise CudaError(f"{name} failed ({rc})")
+        text = _lib.last_error()
+        if rc == 1 and text.startswith(name + ":"):      # an error of CUDA's has a text that begins otherwise
+            raise InvalidInput(text)
+        raise CudaError(text or f"{name} failed ({rc})")
 
 
 def workspace(like, size: int):

@@ -27,6 +27,11 @@ FlameOffloadStatus fail_cuda(cudaError_t e, const char* what) {
   return FLAME_OFFLOAD_ERR_CUDA;
 }
 
+int cuda_result(const char* who, cudaError_t e) {
+  if (e != cudaSuccess) fail_cuda(e, (std::string("CUDA error in ") + who).c_str());
+  return (int)e;
+}
+
 bool fault_fires(int kind) {
   if (g_fault_kind.load(std::memory_order_relaxed) != kind) return false;
   if (g_fault_countdown.fetch_sub(1) == 1) {

@@ -11,6 +11,9 @@ namespace flame_b200 {
 void set_last_error(const std::string& msg);
 FlameOffloadStatus fail(FlameOffloadStatus st, const std::string& msg);
 FlameOffloadStatus fail_cuda(cudaError_t e, const char* what);
+// What an operator's entry `who` returns: e, with a text where it is an error.  The text does not begin with the entry's name, as that of
+// an argument it refuses does.
+int cuda_result(const char* who, cudaError_t e);
 
 // Host-side fault injection (tests only): returns true when the call of this
 // kind that is now being made was chosen to fail.

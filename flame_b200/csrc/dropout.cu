@@ -221,6 +221,7 @@ using namespace flame_b200;
 
 extern "C" int flame_dropout(const void* x, const void* residual, void* y, size_t n, int dtype, double p, uint64_t seed,
                              const void* seed_device, uint64_t offset, void* stream) {
+  const char* who = "flame_dropout";
   if (!(p >= 0.0 && p <= 1.0)) {
     set_last_error("flame_dropout: p must be in [0, 1]");
     return (int)cudaErrorInvalidValue;
@@ -236,12 +237,12 @@ extern "C" int flame_dropout(const void* x, const void* residual, void* y, size_
     set_last_error(!x || !y ? "flame_dropout: null tensor" : "flame_dropout: misaligned tensor");
     return (int)cudaErrorInvalidValue;
   }
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   const double t = nearbyint(p * 4294967296.0);   // 0 .. 2^32
   const uint64_t ti = (uint64_t)t;
   if (ti >> 32) {      // everything is dropped
     const size_t bytes = n * size;
-    return residual ? (int)cudaMemcpyAsync(y, residual, bytes, cudaMemcpyDeviceToDevice, (cudaStream_t)stream) : (int)cudaMemsetAsync(y, 0, bytes, (cudaStream_t)stream);
+    return cuda_result(who, residual ? cudaMemcpyAsync(y, residual, bytes, cudaMemcpyDeviceToDevice, (cudaStream_t)stream) : cudaMemsetAsync(y, 0, bytes, (cudaStream_t)stream));
   }
   DropoutArgs a;
   a.x = x; a.residual = residual; a.y = y; a.n = n;
@@ -251,6 +252,6 @@ extern "C" int flame_dropout(const void* x, const void* residual, void* y, size_
   a.t_hi = (uint32_t)(ti >> 16); a.t_lo = (uint32_t)(ti & 0xFFFFu);
   a.scale = (float)(1.0 / (1.0 - p));
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == FLAME_OFFLOAD_DTYPE_BF16) return (int)(seed_device ? launch_dropout_t<__nv_bfloat16, true>(a, s) : launch_dropout_t<__nv_bfloat16, false>(a, s));
-  return (int)(seed_device ? launch_dropout_t<float, true>(a, s) : launch_dropout_t<float, false>(a, s));
+  if (dtype == FLAME_OFFLOAD_DTYPE_BF16) return cuda_result(who, seed_device ? launch_dropout_t<__nv_bfloat16, true>(a, s) : launch_dropout_t<__nv_bfloat16, false>(a, s));
+  return cuda_result(who, seed_device ? launch_dropout_t<float, true>(a, s) : launch_dropout_t<float, false>(a, s));
 }

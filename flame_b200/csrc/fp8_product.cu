@@ -1014,12 +1014,12 @@ int flame_fp8_quant_2d(const void* x, size_t rows, size_t cols, size_t x_stride,
   if (!tile && !row && !col) return refuse(who, "nothing to make");
   if (((tile || row) && (!codes || !scales)) || (col && !column_scales)) return refuse(who, "null tensor");
   if (!al(codes, 16) || !al(column_codes, 16) || !al(scales, 4) || !al(column_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   const QuantJob a = quant_job(x, rows, cols, x_stride, (tile ? kQuantTiles : 0u) | (row ? kQuantRows : 0u) | (col ? kQuantColumns : 0u), codes, scales,
                                column_codes, column_scales, code_stride);
   QuantJobs jobs = {};
   jobs.job[0] = a;
-  return (int)launch_quant(jobs, (cudaStream_t)stream);
+  return cuda_result(who, launch_quant(jobs, (cudaStream_t)stream));
 }
 
 int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scales, int blocks, void* out, int out_dtype, size_t rows,
@@ -1032,7 +1032,7 @@ int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scal
   if (rows == 0 || cols == 0) return 0;
   if (!codes || !scales || !out) return refuse(who, "null tensor");
   if (!al(codes, 16) || !al(scales, 4) || !al(out, out_dtype == FLAME_OFFLOAD_DTYPE_F32 ? 4 : 2)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   DequantArgs a;
   a.codes = static_cast<const uint8_t*>(codes); a.code_stride = code_stride; a.scales = static_cast<const float*>(scales);
   a.rows = (uint32_t)rows; a.cols = (uint32_t)cols; a.out = out;
@@ -1042,8 +1042,8 @@ int flame_fp8_dequant_2d(const void* codes, size_t code_stride, const void* scal
   // at least one row of threads, so that every column has one
   const uint64_t across = (cols + 7) / 8, wanted = ((uint64_t)rows * across + 255) / 256, least = (across + 255) / 256;
   const unsigned grid = (unsigned)(wanted < 148 * 32 ? wanted : least > 148 * 32 ? least : 148 * 32);
-  return out_dtype == FLAME_OFFLOAD_DTYPE_F32 ? (int)launch_after(fp8_dequant_kernel<float>, grid, 256, 0, (cudaStream_t)stream, a)
-                                              : (int)launch_after(fp8_dequant_kernel<__nv_bfloat16>, grid, 256, 0, (cudaStream_t)stream, a);
+  return cuda_result(who, out_dtype == FLAME_OFFLOAD_DTYPE_F32 ? launch_after(fp8_dequant_kernel<float>, grid, 256, 0, (cudaStream_t)stream, a)
+                                                               : launch_after(fp8_dequant_kernel<__nv_bfloat16>, grid, 256, 0, (cudaStream_t)stream, a));
 }
 
 int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales, int a_blocks, const void* b_codes, size_t b_stride,
@@ -1062,8 +1062,8 @@ int flame_fp8_product(const void* a_codes, size_t a_stride, const void* a_scales
   if (!c || !al(c, c_dtype == FLAME_OFFLOAD_DTYPE_F32 ? 4 : 2)) return refuse(who, "null or misaligned output");
   if (K != 0 && (!a_codes || !b_codes || !a_scales || !b_scales)) return refuse(who, "null tensor");
   if (!al(a_codes, 16) || !al(b_codes, 16) || !al(a_scales, 4) || !al(b_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
-  return (int)product(kind, a_codes, a_stride, a_scales, b_codes, b_stride, b_scales, c, c_stride, c_dtype == FLAME_OFFLOAD_DTYPE_F32, M, N, K, (cudaStream_t)stream);
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
+  return cuda_result(who, product(kind, a_codes, a_stride, a_scales, b_codes, b_stride, b_scales, c, c_stride, c_dtype == FLAME_OFFLOAD_DTYPE_F32, M, N, K, (cudaStream_t)stream));
 }
 
 size_t flame_fp8_linear_workspace_bytes(size_t M, size_t N, size_t K, int flags) {
@@ -1088,7 +1088,7 @@ int flame_fp8_linear(const void* x, size_t x_stride, const void* x_codes, size_t
   if (!al(y, 2) || !al(w_codes, 16) || !al(w_scales, 4) || !al(x_codes, 16) || !al(x_scales, 4)) return refuse(who, "misaligned tensor (codes: 16 bytes)");
   if (K > 0 && (!x_codes || w) && (!workspace || !al(workspace, 256) || workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, w ? FLAME_FP8_LINEAR_BF16_WEIGHT : 0)))
     return refuse(who, "workspace too small, or not on 256 bytes");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   cudaStream_t s = (cudaStream_t)stream;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   QuantJobs jobs = {};
@@ -1106,9 +1106,9 @@ int flame_fp8_linear(const void* x, size_t x_stride, const void* x_codes, size_t
     w_scales = q.scales;
     jobs.job[1] = quant_job(w, N, K, w_stride, kQuantTiles, q.codes, q.scales, nullptr, nullptr, w_code_stride);
   }
-  if (const cudaError_t e = launch_quant(jobs, s)) return (int)e;
-  return (int)product(w || w_blocks == FLAME_FP8_BLOCKS_TILES ? Product::kNtTiles : Product::kNtRows, x_codes, x_code_stride, x_scales, w_codes, w_code_stride, w_scales,
-                      y, N, false, M, N, K, s);
+  if (const cudaError_t e = launch_quant(jobs, s)) return cuda_result(who, e);
+  return cuda_result(who, product(w || w_blocks == FLAME_FP8_BLOCKS_TILES ? Product::kNtTiles : Product::kNtRows, x_codes, x_code_stride, x_scales, w_codes, w_code_stride,
+                                  w_scales, y, N, false, M, N, K, s));
 }
 
 int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, size_t x_stride, const void* w, size_t w_stride, const void* w_codes,
@@ -1127,7 +1127,7 @@ int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, s
   if (any && (!workspace || !al(workspace, 256) ||
               workspace_bytes < flame_fp8_linear_workspace_bytes(M, N, K, FLAME_FP8_LINEAR_BACKWARD | (w ? FLAME_FP8_LINEAR_BF16_WEIGHT : 0))))
     return refuse(who, "workspace too small, or not on 256 bytes");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   cudaStream_t s = (cudaStream_t)stream;
   const size_t ldn = up16(N), ldk = up16(K);
   uint8_t* at = static_cast<uint8_t*>(workspace);
@@ -1146,22 +1146,24 @@ int flame_fp8_linear_backward(const void* dy, size_t dy_stride, const void* x, s
       w_code_stride = ldk;
       w_scales = q.scales;
     }
-    if (const cudaError_t e = launch_quant(jobs, s)) return (int)e;
+    if (const cudaError_t e = launch_quant(jobs, s)) return cuda_result(who, e);
   }
   // the two side by side; an empty sum's zeros are no product
   const bool both = dx && dw && any;
   if (dx && M > 0)
     if (const cudaError_t e = product(Product::kNnTiles, rows.codes, ldn, rows.scales, w_codes, w_code_stride, w_scales, dx, K, false, M, K, N, s, both ? kFirst : kBehind))
-      return (int)e;
-  if (dw && N > 0) return (int)product(Product::kTnColumns, cols.codes, ldn, cols.scales, xcols.codes, ldk, xcols.scales, dw, K, false, N, K, M, s, both ? kBeside : kBehind);
+      return cuda_result(who, e);
+  if (dw && N > 0)
+    return cuda_result(who, product(Product::kTnColumns, cols.codes, ldn, cols.scales, xcols.codes, ldk, xcols.scales, dw, K, false, N, K, M, s, both ? kBeside : kBehind));
   return 0;
 }
 
 int flame_fp8_product_faults(unsigned int* count) {
-  if (!count) return refuse("flame_fp8_product_faults", "null count");
+  const char* who = "flame_fp8_product_faults";
+  if (!count) return refuse(who, "null count");
   // a copy on the default stream would not wait for streams that do not synchronise with it
-  if (const cudaError_t e = cudaDeviceSynchronize()) return (int)e;
-  return (int)cudaMemcpyFromSymbol(count, g_wait_faults, sizeof(*count));
+  if (const cudaError_t e = cudaDeviceSynchronize()) return cuda_result(who, e);
+  return cuda_result(who, cudaMemcpyFromSymbol(count, g_wait_faults, sizeof(*count)));
 }
 
 }  // extern "C"

@@ -881,7 +881,7 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
     return refuse(who, "misaligned tensor (stats: 8 bytes)");
   const bool al16 = al(x, 16) && al(y, 16);
   if (codes && (C % 128 != 0 || !al16 || !al(codes, 8) || !code_scales)) return refuse(who, "codes need channels % 128 == 0, 16-byte aligned tensors and a place for the scales");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   const Plan p = plan((uint32_t)B, L, (uint32_t)C, al16, al(x, 4) && al(y, 4), false, sm_count_here());
   NormArgs a = {};
   a.x = static_cast<const __nv_bfloat16*>(x); a.weight = weight; a.bias = bias; a.y = static_cast<__nv_bfloat16*>(y);
@@ -896,7 +896,7 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
   const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
   const size_t sums_and_shifts = sums + G * sizeof(float);
   cudaStream_t s = (cudaStream_t)stream;
-  return (int)by_width(p.V, [&](auto v) {
+  return cuda_result(who, by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
     cudaError_t e = launch<group_stats_kernel<V>>(grid, true, sums_and_shifts, s, a);
     if (e != cudaSuccess) return e;
@@ -906,7 +906,7 @@ int flame_group_norm(const void* x, const void* weight, const void* bias, void* 
       if (a.codes) return launch<group_apply_kernel<8, true>>(grid, false, groups, s, a);
     }
     return launch<group_apply_kernel<V, false>>(grid, false, groups, s, a);
-  });
+  }));
 }
 
 int flame_group_norm_backward(const void* x, const void* dy, const void* weight, const void* bias, const void* stats, void* dx,
@@ -917,15 +917,15 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   cudaStream_t s = (cudaStream_t)stream;
   const size_t psize = param_dtype == FLAME_OFFLOAD_DTYPE_F32 ? 4 : 2;
   if (B == 0 || L == 0) {   // sums over nothing
-    if (dweight) if (const cudaError_t e = cudaMemsetAsync(dweight, 0, C * psize, s)) return (int)e;
-    if (dbias) if (const cudaError_t e = cudaMemsetAsync(dbias, 0, C * psize, s)) return (int)e;
+    if (dweight) if (const cudaError_t e = cudaMemsetAsync(dweight, 0, C * psize, s)) return cuda_result(who, e);
+    if (dbias) if (const cudaError_t e = cudaMemsetAsync(dbias, 0, C * psize, s)) return cuda_result(who, e);
     return 0;
   }
   if (!x || !dy || !dx || !stats || !workspace) return refuse(who, "null tensor");
   if (workspace_bytes < flame_group_norm_workspace_bytes(B, L, C, G, 1)) return refuse(who, "workspace too small");
   if (!al(x, 2) || !al(dy, 2) || !al(dx, 2) || !al(weight, psize) || !al(bias, psize) || !al(dweight, psize) || !al(dbias, psize) || !al(stats, 8) || !al(workspace, 16))
     return refuse(who, "misaligned tensor (stats: 8 bytes)");
-  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return (int)cudaErrorLaunchFailure;
+  if (fault_fires(FLAME_OFFLOAD_FAULT_KERNEL)) return cuda_result(who, cudaErrorLaunchFailure);
   const Plan p = plan((uint32_t)B, L, (uint32_t)C, al(x, 16) && al(dy, 16) && al(dx, 16), al(x, 4) && al(dy, 4) && al(dx, 4), true, sm_count_here());
   NormArgs a = {};
   a.x = static_cast<const __nv_bfloat16*>(x); a.dy = static_cast<const __nv_bfloat16*>(dy); a.weight = weight; a.bias = bias;
@@ -941,14 +941,14 @@ int flame_group_norm_backward(const void* x, const void* dy, const void* weight,
   const dim3 grid(p.chunks, p.slabs, (unsigned)B);
   const dim3 more(p.chunks, p.slabs, (unsigned)B + (dweight || dbias ? 1 : 0));
   const size_t ring = p.V == 8 ? kRingBytes : 0, sums = ring + ((size_t)kThreads * p.V + G) * sizeof(float2), groups = ring + G * sizeof(float2);
-  return (int)by_width(p.V, [&](auto v) {
+  return cuda_result(who, by_width(p.V, [&](auto v) {
     constexpr int V = decltype(v)::value;
     cudaError_t e = launch<group_grad_sums_kernel<V>>(grid, true, sums, s, a);
     if (e != cudaSuccess) return e;
     if (a.finished) e = launch<group_finish_kernel<true>>(dim3(a.G, a.B), false, 0, s, a);
     if (e != cudaSuccess) return e;
     return launch<group_grad_apply_kernel<V>>(more, false, groups, s, a);
-  });
+  }));
 }
 
 }  // extern "C"

@@ -19,7 +19,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from . import _op
+from . import _lib, _op
 from .errors import CudaError, InvalidInput, InvalidShape, Unsupported
 
 BLOCK = 128
@@ -175,7 +175,7 @@ def check_faults(device: Optional[torch.device] = None) -> None:
     with torch.cuda.device(index):
         rc = _op.function("flame_fp8_product_faults")(ctypes.byref(count))
     if rc:
-        raise CudaError(f"flame_fp8_product_faults failed ({rc})")
+        raise CudaError(f"flame_fp8_product_faults failed ({rc}): {_lib.last_error()}")
     new = count.value - _seen_faults.get(index, 0)
     _seen_faults[index] = count.value
     if new:

@@ -534,8 +534,9 @@ FlameOffloadStatus flame_restore_arena_reset(FlameRestoreArena* arena);
 FlameOffloadStatus flame_restore_arena_stats(const FlameRestoreArena* arena, FlameRestoreArenaStats* out);
 
 /* ------------------------------------------------------------------------
- * 8. Operators next to the path (new).  All of them: 0 or a cudaError_t value, with a text in flame_offload_last_error()
- *    where an argument is refused; a few launches on `stream` and nothing else (no allocation, no synchronisation, no
+ * 8. Operators next to the path (new).  All of them: 0 or a cudaError_t value, with a text in flame_offload_last_error():
+ *    "<entry>: ..." (and cudaErrorInvalidValue) where an argument is refused, "CUDA error in <entry>: ..." where a CUDA call
+ *    failed; a few launches on `stream` and nothing else (no allocation, no synchronisation, no
  *    atomics: the same inputs give the same bits), so that they can be recorded in a CUDA graph once each has been called
  *    on the device; outputs must not overlap inputs.
  *
