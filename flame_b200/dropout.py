@@ -9,7 +9,7 @@ each dropout of a model an ``offset`` of its own and changes the ``seed`` from s
 
 A step recorded in a CUDA graph takes ``seed`` as an int64 tensor of one element on the GPU, which is read when the kernel runs:
 write the next seed into it between replays.  Where backward runs outside that graph, leave the tensor alone until it has run
-(autograd refuses a saved tensor that was modified).
+(a seed that was modified is refused).
 
 csrc/dropout.cu defines the numbers: Philox 4x32-10, 32 bits for each element.
 """
@@ -36,14 +36,19 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, residual, p, seed, offset):
         ctx.p, ctx.offset = p, offset
         ctx.seed = None if isinstance(seed, torch.Tensor) else seed
-        ctx.save_for_backward(*((seed,) if ctx.seed is None else ()))
+        if ctx.seed is None:      # autograd does not look at the version of a tensor that goes through saved-tensor hooks
+            ctx.seed_tensor, ctx.seed_version = seed, seed._version
         return _launch(x, residual, p, seed, offset)
 
     @_op.first_order
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
-            seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
+            seed = ctx.seed
+            if seed is None:
+                seed = ctx.seed_tensor
+                if seed._version != ctx.seed_version:
+                    raise RuntimeError("dropout: the seed tensor was modified between forward and backward")
             dx = _launch(dy.contiguous(), None, ctx.p, seed, ctx.offset)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
