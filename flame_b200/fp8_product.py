@@ -269,6 +269,10 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks], *, codes
     ``weight`` as ``Fp8Blocks`` is frozen ("tiles", or "rows" where x needs no gradient); as a BF16 tensor it is quantised in the call and
     receives a gradient.  ``codes``: the "rows" codes of x where a producer has written them already (``group_norm_fp8``)."""
     frozen = weight if isinstance(weight, Fp8Blocks) else None
+    if frozen is None and not isinstance(weight, torch.Tensor):
+        raise InvalidInput(f"fp8_linear: expected a tensor or Fp8Blocks as weight, got {type(weight).__name__}")
+    if codes is not None and not isinstance(codes, Fp8Blocks):
+        raise InvalidInput(f"fp8_linear: codes are Fp8Blocks, got {type(codes).__name__}")
     _op.on_gpu("fp8_linear", x, weight if frozen is None else frozen.codes, codes.codes if codes is not None else None)
     if frozen is None and (weight.dtype != torch.bfloat16 or weight.dim() != 2):
         raise InvalidInput("fp8_linear: the weight is a BF16 matrix [N, K] or Fp8Blocks")
