@@ -118,7 +118,7 @@ __device__ __forceinline__ float value(bool keep, float x, float scale) { return
 // own in places of its own: with one group in flight a thread (in registers) a 9216 x 9216 BF16 tensor took 94 us, the warps waiting
 // for memory four cycles of ten.  Some 20 issue slots an element, half of them the generator's, where the copy rate of BF16 leaves 21:
 // bound by both.  9216 x 9216 on one B200: BF16 71.5 us (4.7 TB/s), with a residual 78.7 us (6.5 TB/s), F32 108 us (6.3 TB/s), with a
-// residual 152 us (6.7 TB/s).
+// residual 152 us (6.7 TB/s), recorded in a CUDA graph and replayed back to back.
 constexpr int kRingBytes = 32 * 1024;
 template <typename T, bool kResidual, bool kDeviceSeed>
 __global__ void __launch_bounds__(kThreads, 4) dropout_kernel(const __grid_constant__ DropoutArgs a) {

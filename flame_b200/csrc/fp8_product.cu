@@ -5,6 +5,9 @@
 //
 // A block runs along the contraction: 1 x 128 of a row ("rows"), 128 x 1 of a column ("columns"), or 128 x 128 ("tiles", a
 // weight, which then serves the product and its transpose with the same codes).
+//
+// Times in this file: calls recorded in a CUDA graph and replayed back to back on one B200, a few milliseconds at a time, so that the
+// board's power limit is not reached unless it says so.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(256) fp8_dequant_kernel(const __grid_constant_
 //
 // What bounds it, at 8192^3 on one B200 (a pair's block of 128 is 541 cycles of products): copies and products alone take 333 us, 3.3
 // PFLOP/s; with the accumulators handed to an epilogue that does nothing 383; as it is 470 (2.34 PFLOP/s) with a scale for 128 columns
-// and 654 with one for each.  From a product's end to the epilogue's start pass some 420 cycles, from its release to the next product's
+// and 660 with one for each.  From a product's end to the epilogue's start pass some 420 cycles, from its release to the next product's
 // start 270, between them the reading, during which products are slower: two accumulators, all that tensor memory holds, hide most of
 // it.  Halves of 128 columns in four accumulators took 620 us, tiles of 256 x 192 that the epilogue reads whole before it adds 560,
 // sixteen epilogue warps 500 to 510.  Power counts too: operands of zeros take 410 us, and in loops of seconds the limit of the board
@@ -903,9 +906,9 @@ cudaError_t launch_product_t(const Operands& o, ProductArgs p, cudaStream_t stre
   p.wide_sa = kAmn && (reinterpret_cast<uintptr_t>(p.sa) & 15u) == 0 && p.sa_stride % 4 == 0;
   p.wide_sb = kBmn && kBvec && (reinterpret_cast<uintptr_t>(p.sb) & 15u) == 0 && p.sb_stride % 4 == 0;
   // Which form: a round of pairs (256 x 256 tiles, one for two SMs) takes 1.0 where a round of single blocks (128 x 128) takes 0.70,
-  // measured with one round of each: 2048 x 2048 and 1536 x 1536 took 18.8 and 13.2 us at K = 4096, 9.0 and 6.0 us at K = 1024.  128
-  // blocks that share the contraction four at a time (one token, 2048 x 2048) 5.2 us, two at a time 6.0, none 7.5, eight 9.3: clusters
-  // of eight wait for a place.
+  // measured with one round of each: 2048 x 2048 and 1536 x 1536 took 18.8 and 13.2 us at K = 4096, 9.0 and 6.0 us at K = 1024.  The 16
+  // tiles of one token against 2048 x 2048 took 5.2 us with four blocks to a tile, 6.0 with two, 7.5 with one and 9.3 with eight:
+  // clusters of eight wait for a place.
   const uint64_t pairs = (uint64_t)sms / 2, rounds_of_pairs = ((uint64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) + pairs - 1) / pairs;
   p.tiles_m = (p.M + 127) / 128;
   p.tiles_n = (p.N + 127) / 128;

@@ -15,10 +15,13 @@
 // launch a quarter of them to read; where there are many, a launch of a block for each group joins them in between.  Everything is
 // added in a fixed order, without atomics: the same inputs give the same bits.
 //
-// What bounds it, measured on one B200: memory where x is larger than the L2 cache, which the second launch then reads again (1024 x 1024
-// x 128 with silu: forward 139 us for 537 MB in and out and 268 read twice, 5.8 TB/s; backward 231 us; with codes 174 us); the way
-// through two dependent launches and their joins where it is small (1 x 64 x 1280 forward 8.9 us, backward 10.5; 4 x 4096 x 320 15.8
-// and 18.8; of those 8 us a launch some 3 are the rows, 2 the cluster's join, 2 the joining of the parts).
+// What bounds it, measured on one B200 (calls recorded in a CUDA graph and replayed back to back): memory where x is larger than the L2
+// cache, which the second launch then reads again (1024 x 1024 x 128 with silu: forward 139 us for 537 MB in and out and 268 read twice,
+// 5.8 TB/s; with codes 191 us; 1 x 524288 x 128 forward and backward 203 us); the way through two dependent launches and their joins where it is
+// small (1 x 64 x 1280 forward 9.1 us, and backward 20.1; 4 x 4096 x 320 15.2 and 34.5; of those 8 us a launch some 3 are the rows, 2 the
+// cluster's join, 2 the joining of the parts).
+//
+// Squares are binary32 numbers: a group with values further than 1e19 from the others has NaN.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>

@@ -589,8 +589,11 @@ int flame_fp8_linear_backward(const void* dy_bf16, size_t dy_stride, const void*
  * stream is being captured). */
 int flame_fp8_product_faults(unsigned int* count);
 
-/* 8b. Group norm with an activation on a channels-last BF16 tensor x [B, L, C] (contiguous): C / G neighbouring channels a
- *     group, mean and variance over L x C/G elements, h = (x - mean) * rstd * weight + bias, y = h or silu(h), fp32 inside.
+/* 8b. Group norm with an activation on a channels-last BF16 tensor x [B, L, C] (contiguous; at most 65,534 samples, 2^31 - 1
+ *     positions, 65,536 channels and 4,096 groups): C / G neighbouring channels a
+ *     group, mean and variance over L x C/G elements, h = (x - mean) * rstd * weight + bias, y = h or silu(h), fp32 inside (silu
+ *     is 0 under h = -41.6 and NaN at -infinity; a group whose squares about a value of its own overflow, with values further
+ *     than 1e19 apart, is NaN).
  *     weight, bias [C]: param_dtype (FLAME_OFFLOAD_DTYPE_*), NULL = 1 and 0.  stats [B, G, 2] fp32 (8-byte aligned) receives mean and
  *     rstd = 1/sqrt(variance + eps), which the backward pass reads.  codes / code_scales (may be NULL; C % 128 == 0): FP8
  *     codes of y with ROWS blocks ([B*L, C], stride C).  workspace: flame_group_norm_workspace_bytes, 16-byte aligned,
